@@ -303,6 +303,135 @@ int swl_sample_device(const float* d_logits, int32_t nseq, int32_t vocab, int64_
                       const int32_t* d_eos, int32_t n_eos, const int32_t* d_ban_eos, int32_t* d_counts,
                       int32_t update_counts, const float* d_uniform, int32_t* d_out, void* cuda_stream);
 
+/* ---- KV cache held in 4 bits (no counterpart in the reference, whose cache
+ * is f32: QwenCPUModel.swift:285-367 keeps K and V rows per layer) --------
+ *
+ * For callers that run their own attention layers, or hold more or longer
+ * conversations than an f32 cache allows: device-resident pages of 4-bit
+ * keys and values, written, read back, attended to and trimmed by the five
+ * calls below. They allocate nothing, wait for nothing, take lengths and
+ * page tables from device memory (so a captured CUDA graph replays with new
+ * ones) and run on the device that holds the pages.
+ *
+ * Values: per slot, kv head and `group` (64 or 128) consecutive channels an
+ * f16 scale s and bias b and 4-bit codes, value = s * code + b; b =
+ * f16(min), s = f16((max - min) / 15), code = round((x - b) / s) in 0..15. A
+ * group that holds a NaN or an infinity, or whose b or s f16 does not hold
+ * (|x| above 65504), reads back as NaN. Keys are stored as given (after any
+ * rotation), so the order of the slots carries no meaning beyond the causal
+ * rule below.
+ *
+ * Pages: `pages` (16-byte aligned device memory) holds num_pages pages of
+ * swl_kv4_page_bytes bytes, each page_size (16, 32, 64 or 128) slots of every
+ * kv head; the layout inside is the library's own. Slots [j * page_size,
+ * (j + 1) * page_size) of sequence i are in page
+ * page_table[i * table_stride + j]. Sequences may share pages that nobody
+ * appends to. */
+typedef struct swl_kv4_cache {
+  void* pages;
+  const int32_t* page_table; /* device */
+  int64_t table_stride;      /* entries between sequences */
+  int32_t num_pages, page_size, kv_heads;
+  int32_t head_dim; /* 64, 128 or 256 */
+  int32_t group;    /* 64 or 128, at most head_dim */
+} swl_kv4_cache;
+
+/* A batch: rows start[i] .. start[i + 1] - 1 of the token buffers are the new
+ * tokens of sequence i (any number, 0 included), which take its last slots:
+ * lens[i] counts the slots with the new ones. total bounds the rows, max_new
+ * the new tokens of one sequence, max_len the slots of one sequence (a length
+ * outside [0, max_len] is held to it). Rows from start[nseq] on are neither
+ * read nor written. status (device int32, may be NULL; never cleared): bit 0,
+ * a bounded wait inside a kernel gave up and the results are incomplete; bit
+ * 1, a length outside [0, max_len] or a page outside the pool (such slots
+ * are skipped as if masked). */
+typedef struct swl_kv4_batch {
+  const int32_t* start; /* device [nseq + 1], ascending */
+  const int32_t* lens;  /* device [nseq] */
+  int32_t nseq, total, max_new, max_len;
+  int32_t* status;
+} swl_kv4_batch;
+
+/* Rows of a token buffer: element c of head h of row j is at data +
+ * (j * token_stride + h * head_stride + c) elements; the elements of a head
+ * are adjacent. */
+typedef struct swl_kv4_rows {
+  const void* data;
+  int64_t token_stride, head_stride;
+} swl_kv4_rows;
+
+/* Bytes of one page, or a negative SWL_ERR_* status. */
+int64_t swl_kv4_page_bytes(int32_t kv_heads, int32_t head_dim, int32_t group, int32_t page_size);
+
+/* Quantises the batch's new keys and values (dtype 0 f32, 1 bf16, 2 f16) into
+ * their slots. When lens[i] is below the number of new tokens the first ones
+ * have no slot and are dropped. d_weights ([nseq][kv_heads][weights_stride],
+ * may be NULL) is set to 0 at the new slots. */
+int swl_kv4_append_device(const swl_kv4_cache* cache, const swl_kv4_batch* batch, int32_t dtype, const swl_kv4_rows* k,
+                          const swl_kv4_rows* v, float* d_weights, int64_t weights_stride, void* cuda_stream);
+
+/* Dequantises the same slots into the rows of k and v (rounded once to
+ * dtype). */
+int swl_kv4_read_device(const swl_kv4_cache* cache, const swl_kv4_batch* batch, int32_t dtype, const swl_kv4_rows* k,
+                        const swl_kv4_rows* v, void* cuda_stream);
+
+/* Attention of the batch's rows over the cache (their own keys and values are
+ * appended already): query head h of `heads` reads kv head
+ * h / (heads / kv_heads); token t of n new ones sees slots 0 .. len - n + t;
+ * out = softmax(scale * q k^T) v, times sigmoid(gate) when gate.data is given
+ * (QwenCPUModel.swift:345-367). A row that sees no slot gets zeros. lse (may
+ * be NULL): [total][heads] the natural logarithm of each row's softmax sum
+ * (-infinity for an empty row). weights (may be NULL):
+ * [nseq][kv_heads][weights_stride]; every slot's softmax weight, summed over
+ * the new tokens and the kv head's query heads, is added to it. Sums are f32
+ * in a fixed order: the same call gives the same bits. q, out and gate have
+ * one dtype; out must not overlap q or gate. work: device memory of
+ * swl_kv4_attention_workspace bytes (16-byte aligned), used by one call at a
+ * time; its contents need no initialisation. */
+typedef struct swl_kv4_attention {
+  int32_t dtype, heads;
+  float scale;
+  swl_kv4_rows q, out, gate;
+  float* lse;
+  float* weights;
+  int64_t weights_stride;
+  void* work;
+  int64_t work_bytes;
+} swl_kv4_attention;
+int64_t swl_kv4_attention_workspace(const swl_kv4_cache* cache, const swl_kv4_batch* batch, int32_t heads);
+int swl_kv4_attention_device(const swl_kv4_cache* cache, const swl_kv4_batch* batch, const swl_kv4_attention* attention,
+                             void* cuda_stream);
+
+/* Eviction: every (sequence, kv head) keeps at most `keep` slots: the first
+ * `first`, the last `recent`, and of the others those with the largest weight
+ * (ties to the lowest slot; NaN counts as -infinity), each head its own. The
+ * survivors, in order, are copied to slots 0, 1, ... of dst_table
+ * ([nseq][dst_stride] pages of the same pool that hold none of the source's
+ * slots still in use: sources stay as they are, so pages that other sequences
+ * share are safe). new_lens[i] = min(lens[i], keep); new_weights
+ * ([nseq][kv_heads][new_weights_stride], may be NULL) takes the survivors'
+ * weights; kept ([nseq][kv_heads][kept_stride], may be NULL) their old slots.
+ * What lies behind the survivors is left as it was. batch.start is not used.
+ * work: swl_kv4_evict_workspace bytes (4-byte aligned), needed only when kept
+ * is NULL. */
+typedef struct swl_kv4_evict {
+  int32_t keep, first, recent;
+  const float* weights;
+  int64_t weights_stride;
+  const int32_t* dst_table;
+  int64_t dst_stride;
+  int32_t* new_lens;
+  float* new_weights;
+  int64_t new_weights_stride;
+  int32_t* kept;
+  int64_t kept_stride;
+  void* work;
+  int64_t work_bytes;
+} swl_kv4_evict;
+int64_t swl_kv4_evict_workspace(const swl_kv4_cache* cache, const swl_kv4_batch* batch, int32_t keep);
+int swl_kv4_evict_device(const swl_kv4_cache* cache, const swl_kv4_batch* batch, const swl_kv4_evict* evict,
+                         void* cuda_stream);
+
 /* Model-free kernels on host buffers, for kernel-level parity tests:
  * y = W x for one MLX-affine matrix (sdtype 0 f32, 1 bf16, 2 f16) ... */
 int swl_kernel_gemv_affine(const uint32_t* packed, const void* scales, const void* biases, int sdtype, int out_dim,

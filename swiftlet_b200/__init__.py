@@ -63,6 +63,35 @@ class swl_affine_matrix(C.Structure):
                 ("cols", C.c_int32), ("bits", C.c_int32), ("group", C.c_int32), ("scale_dtype", C.c_int32)]
 
 
+class swl_kv4_cache(C.Structure):
+    """Pages of a 4-bit KV cache and the sequences' page table (device addresses; see include/swiftlet_cuda.h)."""
+    _fields_ = [("pages", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("num_pages", C.c_int32),
+                ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("group", C.c_int32)]
+
+
+class swl_kv4_batch(C.Structure):
+    """Sequences of a call on a 4-bit KV cache: device [nseq + 1] row starts and [nseq] lengths, host bounds, status word."""
+    _fields_ = [("start", C.c_void_p), ("lens", C.c_void_p), ("nseq", C.c_int32), ("total", C.c_int32),
+                ("max_new", C.c_int32), ("max_len", C.c_int32), ("status", C.c_void_p)]
+
+
+class swl_kv4_rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class swl_kv4_attention(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("scale", C.c_float), ("q", swl_kv4_rows), ("out", swl_kv4_rows),
+                ("gate", swl_kv4_rows), ("lse", C.c_void_p), ("weights", C.c_void_p), ("weights_stride", C.c_int64),
+                ("work", C.c_void_p), ("work_bytes", C.c_int64)]
+
+
+class swl_kv4_evict(C.Structure):
+    _fields_ = [("keep", C.c_int32), ("first", C.c_int32), ("recent", C.c_int32), ("weights", C.c_void_p),
+                ("weights_stride", C.c_int64), ("dst_table", C.c_void_p), ("dst_stride", C.c_int64), ("new_lens", C.c_void_p),
+                ("new_weights", C.c_void_p), ("new_weights_stride", C.c_int64), ("kept", C.c_void_p),
+                ("kept_stride", C.c_int64), ("work", C.c_void_p), ("work_bytes", C.c_int64)]
+
+
 class swl_pool_info(C.Structure):
     _fields_ = [(n, C.c_int64) for n in (
         "expert_stride", "slot_count", "allocated_slots", "hits", "misses", "resident_bytes")]
@@ -115,6 +144,15 @@ _SIGNATURES = {
     "swl_trace_dump": (_I, [_P, C.c_char_p]),
     "swl_kernel_gemv_affine": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P]),
     "swl_kernel_expert_swiglu": (_I, [_P] * 9 + [_I, _I, _I, _I, _I, _P, _P]),
+    "swl_kv4_page_bytes": (_I64, [C.c_int32] * 4),
+    "swl_kv4_append_device": (_I, [C.POINTER(swl_kv4_cache), C.POINTER(swl_kv4_batch), C.c_int32, C.POINTER(swl_kv4_rows),
+                                   C.POINTER(swl_kv4_rows), _P, _I64, _P]),
+    "swl_kv4_read_device": (_I, [C.POINTER(swl_kv4_cache), C.POINTER(swl_kv4_batch), C.c_int32, C.POINTER(swl_kv4_rows),
+                                 C.POINTER(swl_kv4_rows), _P]),
+    "swl_kv4_attention_workspace": (_I64, [C.POINTER(swl_kv4_cache), C.POINTER(swl_kv4_batch), C.c_int32]),
+    "swl_kv4_attention_device": (_I, [C.POINTER(swl_kv4_cache), C.POINTER(swl_kv4_batch), C.POINTER(swl_kv4_attention), _P]),
+    "swl_kv4_evict_workspace": (_I64, [C.POINTER(swl_kv4_cache), C.POINTER(swl_kv4_batch), C.c_int32]),
+    "swl_kv4_evict_device": (_I, [C.POINTER(swl_kv4_cache), C.POINTER(swl_kv4_batch), C.POINTER(swl_kv4_evict), _P]),
     "swl_expert_swiglu_noalloc": (_I, [C.POINTER(swl_affine_matrix)] * 3 + [_P, _P, _P, _P]),
 }
 
@@ -465,6 +503,73 @@ def sample_device(d_logits: int, nseq: int, vocab: int, row_stride: int, *, temp
     _check(lib().swl_sample_device(v(d_logits), int(nseq), int(vocab), int(row_stride), C.byref(o), v(d_suppress),
                                    int(n_suppress), v(d_eos), int(n_eos), v(d_ban_eos), v(d_counts),
                                    int(bool(update_counts)), v(d_uniform), v(d_out), v(stream)))
+
+
+def _size(n: int) -> int:
+    if n < 0:
+        _check(int(n))
+    return int(n)
+
+
+def kv4_page_bytes(kv_heads: int, head_dim: int, group: int = 64, page_size: int = 64) -> int:
+    """Bytes of one page of a 4-bit KV cache (swl_kv4_page_bytes)."""
+    return _size(lib().swl_kv4_page_bytes(kv_heads, head_dim, group, page_size))
+
+
+def _kv4_rows(d: int, strides, heads: int, hd: int) -> swl_kv4_rows:
+    ts, hs = strides or (heads * hd, hd)
+    return swl_kv4_rows(d or None, ts, hs)
+
+
+def kv4_append_device(cache: swl_kv4_cache, batch: swl_kv4_batch, d_k: int, d_v: int, *, dtype: int = 0, k_strides=None,
+                      v_strides=None, d_weights: int = 0, weights_stride: int = 0, stream: int = 0) -> None:
+    """Quantises the batch's new keys and values into their slots (swl_kv4_append_device).
+    dtype 0 f32, 1 bf16, 2 f16; strides are (token, head) in elements, dense [rows][kv_heads][head_dim] by default."""
+    k = _kv4_rows(d_k, k_strides, cache.kv_heads, cache.head_dim)
+    v = _kv4_rows(d_v, v_strides, cache.kv_heads, cache.head_dim)
+    _check(lib().swl_kv4_append_device(cache, batch, dtype, k, v, d_weights or None, weights_stride, stream or None))
+
+
+def kv4_read_device(cache: swl_kv4_cache, batch: swl_kv4_batch, d_k: int, d_v: int, *, dtype: int = 0, k_strides=None,
+                    v_strides=None, stream: int = 0) -> None:
+    """Dequantises the slots of the batch's tokens into dense or strided rows (swl_kv4_read_device)."""
+    k = _kv4_rows(d_k, k_strides, cache.kv_heads, cache.head_dim)
+    v = _kv4_rows(d_v, v_strides, cache.kv_heads, cache.head_dim)
+    _check(lib().swl_kv4_read_device(cache, batch, dtype, k, v, stream or None))
+
+
+def kv4_attention_workspace(cache: swl_kv4_cache, batch: swl_kv4_batch, heads: int) -> int:
+    """Bytes of workspace that kv4_attention_device needs for such a batch."""
+    return _size(lib().swl_kv4_attention_workspace(cache, batch, heads))
+
+
+def kv4_attention_device(cache: swl_kv4_cache, batch: swl_kv4_batch, heads: int, d_q: int, d_out: int, *, scale: float,
+                         dtype: int = 0, q_strides=None, out_strides=None, d_gate: int = 0, gate_strides=None,
+                         d_lse: int = 0, d_weights: int = 0, weights_stride: int = 0, d_work: int = 0, work_bytes: int = 0,
+                         stream: int = 0) -> None:
+    """Causal attention of the batch's rows over a 4-bit KV cache (swl_kv4_attention_device)."""
+    hd = cache.head_dim
+    a = swl_kv4_attention(dtype, heads, scale, _kv4_rows(d_q, q_strides, heads, hd), _kv4_rows(d_out, out_strides, heads, hd),
+                          _kv4_rows(d_gate, gate_strides, heads, hd), d_lse or None, d_weights or None, weights_stride,
+                          d_work or None, work_bytes)
+    _check(lib().swl_kv4_attention_device(cache, batch, a, stream or None))
+
+
+def kv4_evict_workspace(cache: swl_kv4_cache, batch: swl_kv4_batch, keep: int) -> int:
+    """Bytes of workspace that kv4_evict_device needs when it is given no d_kept."""
+    return _size(lib().swl_kv4_evict_workspace(cache, batch, keep))
+
+
+def kv4_evict_device(cache: swl_kv4_cache, batch: swl_kv4_batch, keep: int, *, d_weights: int, weights_stride: int,
+                     d_dst_table: int, dst_stride: int, d_new_lens: int, first: int = 0, recent: int = 0,
+                     d_new_weights: int = 0, new_weights_stride: int = 0, d_kept: int = 0, kept_stride: int = 0,
+                     d_work: int = 0, work_bytes: int = 0, stream: int = 0) -> None:
+    """Keeps the `keep` slots of largest accumulated weight of every sequence and kv head, copied to the pages of
+    another table (swl_kv4_evict_device)."""
+    e = swl_kv4_evict(keep, first, recent, d_weights or None, weights_stride, d_dst_table or None, dst_stride,
+                      d_new_lens or None, d_new_weights or None, new_weights_stride, d_kept or None, kept_stride,
+                      d_work or None, work_bytes)
+    _check(lib().swl_kv4_evict_device(cache, batch, e, stream or None))
 
 
 EP_ID_BYTES = 128
