@@ -1,4 +1,25 @@
-// Attention over the 4-bit KV cache (layout: kv4.h).
+// Attention over the 4-bit KV cache for few query rows a sequence (single
+// tokens above all), and the accumulation of attention weights.
+//
+// With codes c, group scales s and biases b of a slot t (kv4.h), e = c - 7.5
+// and b' = b + 7.5 s (the group's middle, so that neither part carries a
+// large common term):
+//   q.k_t = sum_g s_tg (sum_{i in g} q_i e_ti) + b'_tg (sum_{i in g} q_i)
+//   out_i = sum_t (p_t s_tg) e_ti + sum_t p_t b'_tg          (i in group g)
+// e is exact in f16, so both inner sums are matrix products of exact 4-bit
+// operands: mma.m16n8k16 (f16, f32 accumulators) with 16 slots x 16 channels
+// of codes against the 8 query columns of a kv head, per group, and 16
+// channels x 16 slots against the weights p s. For f32 inputs q and p s go in
+// as two f16 terms each (22 bits); for 16-bit inputs q is exact (bf16) or
+// itself (f16) and p s is rounded to 11 bits. Softmax statistics, group sums
+// and outputs are f32. Columns are scaled by powers of two on their way into
+// f16 (q by its largest element, p by the largest group scale seen), which
+// changes no bit of the result but keeps both terms in range.
+//
+// Bound: the cache's bytes (2 (D / 2 + 4 D / g) a slot and kv head). The
+// unpacking costs 10 ALU instructions per 8 codes, about two thirds of the
+// issue slots at the HBM rate, which is why codes go to the tensor cores
+// unscaled and the scales are applied to the 16 x 8 results instead.
 #include <algorithm>
 
 #include "kcommon.cuh"
@@ -9,110 +30,747 @@ namespace swl {
 
 namespace {
 
-// One warp per (row, head): the lane's head_dim / 32 channels of q, an online
-// softmax over the slots the row sees, one slot at a time.
-constexpr int SA_WARPS = 8;
+constexpr int AT_WARPS = 8;                 // consumer warps, 16 slots of a tile each
+constexpr int AT_THREADS = AT_WARPS * 32 + 32;  // and one producer warp
+constexpr int AT_TILE = 16 * AT_WARPS;      // slots of a tile
+constexpr int AT_COLS = 8;                  // query columns (token, head) of an item: the MMA's N
+constexpr int AT_GRID = 148;                // one CTA per SM
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-template <int HD>
-__device__ __forceinline__ void sa_slot(const Kv4Geo& g, const uint8_t* base, int t, int lane, float (&x)[HD / 32]) {
-  constexpr int E = HD / 32;
-  const int c0 = lane * E, unit = (c0 % 64) / 8;
-  const uint8_t* p = base + t * (HD / 2) + (unit ^ kv4_swz(HD, t)) * (HD / 16) + c0 / 64 * 4 + c0 % 8 / 2;
-  uint32_t w = 0;
-  for (int b = 0; b < E / 2; ++b) w |= uint32_t(p[b]) << (8 * b);
-  const float2 sb = kv4_param(reinterpret_cast<const uint32_t*>(base + g.seg * (HD / 2))[t * g.ng + c0 / g.group]);
-#pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = fmaf(sb.x, float((w >> (4 * e)) & 15u), sb.y);
+// ------------------------------------------------------------ primitives --
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transpose of an 8 x 8 matrix of 16-bit elements spread over the warp.
+__device__ __forceinline__ uint32_t movm(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// Nibbles 0 and 1 of both halves of a word as two f16 pairs, each minus 7.5:
+// a code at bits 1..4 of 0x6000 (512, step 0.5) is 512 + c, at bits 5..8
+// 512 + 16 c; both results are exact.
+__device__ __forceinline__ void unpack2(uint32_t x, uint32_t& n0, uint32_t& n1) {
+  const __half2 m0 = u2h(0xe00fe00fu);                    // -519.5
+  const __half2 m1 = u2h(0xd0f0d0f0u), r = u2h(0x2c002c00u);  // -39.5, 1 / 16
+  n0 = h2u(__hadd2(u2h((x & 0x001e001eu) | 0x60006000u), m0));
+  n1 = h2u(__hfma2(u2h((x & 0x01e001e0u) | 0x60006000u), r, m1));
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+  return r;
+}
+// N consecutive words of shared or global memory as one vector load.
+template <int N>
+__device__ __forceinline__ void ldv(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+__device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// ------------------------------------------------------------------ work --
+// The work is the list of all (sequence, column block, kv head) items, each of
+// ceil(len / 128) tiles (one at least); a CTA takes an equal, contiguous share
+// of all tiles, so ragged batches and single long sequences spread alike.
+// Every warp finds its place from the lengths in device memory: nothing of the
+// split is known to the host.
+struct Place {
+  int seq, item;   // item within the sequence: column block * kvh + kv head
+  int tile;        // first tile of this share within the item
+  int row0, n, len, tiles, items;
+};
+
+__device__ __forceinline__ void load_seq(const Kv4AttnArgs& a, int seq, Place& p) {
+  p.seq = seq;
+  p.n = kv4_new(a.b, seq, p.row0);
+  p.len = kv4_len(a.b, seq);
+  p.tiles = max(1, (p.len + AT_TILE - 1) / AT_TILE);
+  p.items = (int)(((int64_t)p.n * a.rep + AT_COLS - 1) / AT_COLS) * a.g.kvh;
 }
 
-template <int HD>
-__global__ void __launch_bounds__(SA_WARPS * 32) k_kv4_attn_rows(const Kv4AttnArgs a) {
-  constexpr int E = HD / 32;
+__device__ __forceinline__ int64_t warp_incl(int64_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
+__device__ __forceinline__ int64_t total_tiles(const Kv4AttnArgs& a) {
   const int lane = threadIdx.x & 31;
-  const int64_t wid = int64_t(blockIdx.x) * SA_WARPS + (threadIdx.x >> 5);
-  const int j = int(wid / a.heads), hq = int(wid % a.heads), h = hq / a.rep;
-  if (j >= a.b.total) return;
-  const int seq = kv4_seq_of(a.b, j);
-  if (seq < 0) return;
-  int row0;
-  const int n = kv4_new(a.b, seq, row0), len = kv4_len(a.b, seq);
-  const int last = min(len - 1, len - n + (j - row0));
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = kv4_ld(a.q.p, a.dt, j * a.q.ts + hq * a.q.hs + lane * E + e);
-    o[e] = 0.f;
-  }
-  for (int s = 0; s <= last; ++s) {
-    const uint8_t* blk = kv4_block(a.g, a.g.table, a.g.tstride, seq, h, s, a.b.status);
-    if (!blk) continue;
-    float k[E], v[E], d = 0.f;
-    sa_slot<HD>(a.g, blk, s & (a.g.seg - 1), lane, k);
-    sa_slot<HD>(a.g, blk + a.g.blk / 2, s & (a.g.seg - 1), lane, v);
-#pragma unroll
-    for (int e = 0; e < E; ++e) d = fmaf(q[e], k[e], d);
-    const float x = warp_sum(d) * a.scale, mn = fmaxf(m, x);
-    const float al = expf(m - mn), p = expf(x - mn);
-    l = l * al + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(p, v[e], o[e] * al);
-    m = mn;
+  int64_t sum = 0;
+  for (int i = lane; i < a.b.nseq; i += 32) {
+    Place p;
+    load_seq(a, i, p);
+    sum += int64_t(p.tiles) * p.items;
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    float r = l > 0.f || l != l ? o[e] / l : 0.f;
-    if (a.gate.p) r *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, j * a.gate.ts + hq * a.gate.hs + lane * E + e));
-    kv4_st(a.out.p, a.dt, j * a.out.ts + hq * a.out.hs + lane * E + e, r);
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// Place of tile number `flat` (0 <= flat < total).
+__device__ __forceinline__ Place find_place(const Kv4AttnArgs& a, int64_t flat) {
+  const int lane = threadIdx.x & 31;
+  int64_t base = 0;
+  Place p;
+  for (int i0 = 0; i0 < a.b.nseq; i0 += 32) {
+    int64_t cnt = 0;
+    if (i0 + lane < a.b.nseq) {
+      load_seq(a, i0 + lane, p);
+      cnt = int64_t(p.tiles) * p.items;
+    }
+    const int64_t incl = warp_incl(cnt, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, base + incl > flat);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int64_t before = base + __shfl_sync(0xffffffffu, incl - cnt, src);
+      load_seq(a, i0 + src, p);
+      p.item = int((flat - before) / p.tiles);
+      p.tile = int((flat - before) % p.tiles);
+      return p;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  p = Place{0, 0, 0, 0, 0, 0, 1, 0};
+  return p;
+}
+
+__device__ __forceinline__ void next_item(const Kv4AttnArgs& a, Place& p) {
+  p.tile = 0;
+  if (++p.item < p.items) return;
+  p.item = 0;
+  int s = p.seq + 1;
+  for (; s < a.b.nseq; ++s) {
+    load_seq(a, s, p);
+    if (p.items) return;
+  }
+}
+
+// ------------------------------------------------------- query columns ----
+// Column c of block cb of a sequence's new rows: token (8 cb + c) / rep, query
+// head h * rep + (8 cb + c) % rep.
+template <int HD, bool SPLIT>
+struct QStage {
+  static constexpr int KS = HD / 16;  // k steps
+  static constexpr int W = SPLIT ? 4 : 2;
+  uint32_t frag[KS * 32 * W];        // B fragments: {hi b0, hi b1[, lo b0, lo b1]} per k step and lane
+  float sum[AT_COLS][HD / 64];       // sums of the scaled column over each 64 channels
+  float mul[AT_COLS];                // score = mul * (scaled sum), in units of log2
+  int lim[AT_COLS];                  // last slot the column sees (INT_MAX: unused column)
+};
+
+// Warp w stages column w. Word l of the row (8 channels) is lane l's.
+template <int HD, bool SPLIT>
+__device__ __forceinline__ void stage_q(const Kv4AttnArgs& a, const Place& p, int h, int cb, int col, int lane, QStage<HD, SPLIT>* qs) {
+  const int ci = cb * AT_COLS + col, t = ci / a.rep, hq = h * a.rep + ci % a.rep;
+  const bool on = t < p.n;
+  const bool act = lane < HD / 8;
+  float x[8];
+  float am = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = on && act ? kv4_ld(a.q.p, a.dt, (p.row0 + t) * a.q.ts + hq * a.q.hs + lane * 8 + e) : 0.f;
+    am = fmaxf(am, fabsf(x[e]));
+  }
+  am = warp_max(am);
+  // largest element to [2^12, 2^13); a column of zeros or infinities as it is
+  int ex = am > 0.f && am < INFINITY ? 12 - (int(__float_as_uint(am) >> 23) - 127) : 0;
+  ex = max(-100, min(100, ex));
+  const float up = __int_as_float((127 + ex) << 23);
+  float s = 0.f;
+  uint32_t hi[8], lo[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] *= up;
+    s += x[e];
+    const __half hh = __float2half_rn(x[e]);
+    hi[e] = __half_as_ushort(hh);
+    if (SPLIT) lo[e] = __half_as_ushort(__float2half_rn(x[e] - __half2float(hh)));
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (act) {
+    if ((lane & 7) == 0) qs->sum[col][lane >> 3] = s;
+    const int wi = lane >> 3, u = lane & 7;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const int ks = (wi * 2 + (u >> 2)) * 2 + st;
+      uint32_t* f = qs->frag + (ks * 32 + col * 4 + (u & 3)) * QStage<HD, SPLIT>::W;
+      const uint32_t h0 = hi[2 * st] | hi[2 * st + 4] << 16, h1 = hi[2 * st + 1] | hi[2 * st + 5] << 16;
+      if (SPLIT)
+        *reinterpret_cast<uint4*>(f) = make_uint4(h0, h1, lo[2 * st] | lo[2 * st + 4] << 16, lo[2 * st + 1] | lo[2 * st + 5] << 16);
+      else
+        *reinterpret_cast<uint2*>(f) = make_uint2(h0, h1);
+    }
   }
   if (lane == 0) {
-    float* lse = a.lse ? a.lse : reinterpret_cast<float*>(a.work);
-    lse[int64_t(j) * a.heads + hq] = m + logf(l);
+    qs->mul[col] = a.scale * LOG2E * __int_as_float((127 - ex) << 23);
+    qs->lim[col] = on ? p.len - p.n + t : 0x7fffffff;
   }
 }
 
-// Weights: one warp per (sequence, kv head, slot) adds exp(s - lse) over the
-// rows that see the slot, in row order.
-template <int HD>
-__global__ void __launch_bounds__(SA_WARPS * 32) k_kv4_weights_rows(const Kv4AttnArgs a) {
-  constexpr int E = HD / 32;
-  const int lane = threadIdx.x & 31, seq = blockIdx.z, h = blockIdx.y;
-  const int s = blockIdx.x * SA_WARPS + (threadIdx.x >> 5);
-  int row0;
-  const int n = kv4_new(a.b, seq, row0), len = kv4_len(a.b, seq);
-  if (s >= len) return;
-  const uint8_t* blk = kv4_block(a.g, a.g.table, a.g.tstride, seq, h, s, a.b.status);
-  if (!blk) return;
-  float k[E], sum = 0.f;
-  sa_slot<HD>(a.g, blk, s & (a.g.seg - 1), lane, k);
-  const float* lse = a.lse ? a.lse : reinterpret_cast<const float*>(a.work);
-  for (int i = max(0, s - (len - n)); i < n; ++i)
-    for (int r = 0; r < a.rep; ++r) {
-      const int j = row0 + i, hq = h * a.rep + r;
-      float d = 0.f;
+// The scores of 16 slots (rows r = lane / 4 and r + 8 of the fragment) against
+// the 8 columns, before the column factor: kw = the rows' words of units c and
+// c + 4 (c = lane % 4), kp = their params.
+template <int HD, int GROUP, bool SPLIT, typename QF>
+__device__ __forceinline__ void scores(const uint32_t (&kw)[2][2][HD / 64], const uint32_t (&kp)[2][HD / GROUP],
+                                       const float (&qsum)[2][HD / GROUP], QF qf, float (&sc)[4]) {
+  sc[0] = sc[1] = sc[2] = sc[3] = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) d = fmaf(kv4_ld(a.q.p, a.dt, j * a.q.ts + hq * a.q.hs + lane * E + e), k[e], d);
-      sum += expf(warp_sum(d) * a.scale - lse[int64_t(j) * a.heads + hq]);
+  for (int g = 0; g < HD / GROUP; ++g) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < GROUP / 64; ++w) {
+      const int wi = g * (GROUP / 64) + w;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const uint32_t x0 = st ? kw[hf][0][wi] >> 7 : kw[hf][0][wi] << 1, x1 = st ? kw[hf][1][wi] >> 7 : kw[hf][1][wi] << 1;
+          uint32_t a0, a1, a2, a3;
+          unpack2(x0, a0, a2);
+          unpack2(x1, a1, a3);
+          uint32_t b[SPLIT ? 4 : 2];
+          qf((wi * 2 + hf) * 2 + st, b);
+          mma16816(acc, a0, a1, a2, a3, b[0], b[1]);
+          if constexpr (SPLIT) mma16816(acc, a0, a1, a2, a3, b[2], b[3]);
+        }
     }
-  if (lane == 0) a.weights[(int64_t(seq) * a.g.kvh + h) * a.wstride + s] += sum;
+    const float2 s0 = kv4_param(kp[0][g]), s1 = kv4_param(kp[1][g]);
+    const float m0 = fmaf(7.5f, s0.x, s0.y), m1 = fmaf(7.5f, s1.x, s1.y);
+    sc[0] = fmaf(s0.x, acc[0], fmaf(m0, qsum[0][g], sc[0]));
+    sc[1] = fmaf(s0.x, acc[1], fmaf(m0, qsum[1][g], sc[1]));
+    sc[2] = fmaf(s1.x, acc[2], fmaf(m1, qsum[0][g], sc[2]));
+    sc[3] = fmaf(s1.x, acc[3], fmaf(m1, qsum[1][g], sc[3]));
+  }
 }
 
+template <int HD, int GROUP, bool SPLIT>
+struct AttnShared {
+  static constexpr int ROW = HD / 2 + 4 * (HD / GROUP);
+  static constexpr int TILE_BYTES = 2 * AT_TILE * ROW;
+  static constexpr int STAGES = HD == 256 ? 4 : 8;
+  alignas(128) uint8_t ring[STAGES][TILE_BYTES];
+  float red[AT_WARPS][AT_COLS * HD];  // outputs of the warps, in fragment order
+  QStage<HD, SPLIT> q;
+  float m[AT_WARPS][AT_COLS], l[AT_WARPS][AT_COLS];
+  uint64_t full[STAGES], empty[STAGES];
+  int bad[STAGES];  // pieces of the tile whose page id is outside the pool
+};
+
+// Floats of one partial result: max, sum, outputs.
+__host__ __device__ constexpr int part_floats(int hd) { return 2 * AT_COLS + AT_COLS * hd; }
+
+__device__ __forceinline__ float* attn_lse(const Kv4AttnArgs& a) { return a.lse ? a.lse : reinterpret_cast<float*>(a.work); }
+__device__ __forceinline__ float* attn_parts(const Kv4AttnArgs& a) {
+  return reinterpret_cast<float*>(a.work + (int64_t(a.b.total) * a.heads * 4 + 15) / 16 * 16);
+}
+
+// Eight consecutive outputs of a row, gated.
+__device__ __forceinline__ void write_out(const Kv4AttnArgs& a, int64_t row, int hq, int ch, const float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float r = v[e];
+    if (a.gate.p) r *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch + e));
+    kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch + e, r);
+  }
+}
+
+template <int HD, int GROUP, bool SPLIT>
+__global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a) {
+  using Sh = AttnShared<HD, GROUP, SPLIT>;
+  constexpr int NG = HD / GROUP, NW = HD / 64, KS = HD / 16, S = Sh::STAGES;
+  extern __shared__ __align__(128) uint8_t at_raw[];
+  Sh& sh = *reinterpret_cast<Sh*>(at_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.empty[s], AT_WARPS);
+    }
+    mbar_init_fence();
+  }
+  pdl_launch();
+  const int64_t total = total_tiles(a);
+  const int64_t r0 = total * blockIdx.x / gridDim.x, r1 = total * (blockIdx.x + 1) / gridDim.x;
+  __syncthreads();
+  if (r0 == r1) return;
+  Place p = find_place(a, r0);
+  const Kv4Geo& g = a.g;
+
+  if (warp == AT_WARPS) {
+    // -------------------------------------------------------- producer ----
+    // One bulk copy per block of the tile (keys, values and params of up to
+    // 64 slots of the kv head lie together); the lanes look the pages up.
+    const int seg = g.seg, np = AT_TILE / seg;
+    int j = 0;
+    bool ok = true;
+    for (int64_t f = r0; f < r1 && ok; next_item(a, p)) {
+      const int h = p.item % g.kvh;
+      const int t1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
+      for (int t = p.tile; t < t1; ++t, ++j, ++f) {
+        const int s = j % S;
+        if (!mbar_wait(&sh.empty[s], ((j / S) & 1) ^ 1)) { ok = false; break; }
+        const int slot = t * AT_TILE + lane * seg;
+        const bool want = lane < np && slot < p.len;
+        const uint8_t* src = want ? kv4_block(g, g.table, g.tstride, p.seq, h, slot, a.b.status) : nullptr;
+        const unsigned have = __ballot_sync(0xffffffffu, src != nullptr), bad = __ballot_sync(0xffffffffu, want && !src);
+        if (lane == 0) {
+          sh.bad[s] = int(bad);
+          mbar_expect_tx(&sh.full[s], unsigned(__popc(have)) * unsigned(g.blk));
+        }
+        __syncwarp();
+        if (src) bulk_g2s_keep(sh.ring[s] + lane * g.blk, src, unsigned(g.blk), &sh.full[s]);
+      }
+    }
+    if (!ok) {
+      // a consumer did not free its slot: report it, and let the copies in
+      // flight land before the CTA may end
+      if (lane == 0 && a.b.status) atomicOr(a.b.status, 1);
+      for (int i = max(0, j - S); i < j; ++i) mbar_wait(&sh.full[i % S], (i / S) & 1);
+    }
+    return;
+  }
+
+  // ---------------------------------------------------------- consumers ----
+  const int r = lane >> 2, c = lane & 3;
+  const int piece = warp * 16 / g.seg, trow = (warp * 16) & (g.seg - 1);
+  const int kbase = piece * g.blk, vbase = kbase + g.blk / 2, pbase = g.seg * (HD / 2);
+  // offsets of this lane's vectors within a block (constant over the tiles)
+  const int koff0 = (trow + r) * (HD / 2) + ((c ^ kv4_swz(HD, r)) * (HD / 16));
+  const int koff1 = (trow + r) * (HD / 2) + (((c + 4) ^ kv4_swz(HD, r)) * (HD / 16));
+  const int voff0 = (trow + 2 * c) * (HD / 2) + ((r ^ kv4_swz(HD, 2 * c)) * (HD / 16));
+  const int voff1 = (trow + 2 * c + 1) * (HD / 2) + ((r ^ kv4_swz(HD, 2 * c + 1)) * (HD / 16));
+  int j = 0;
+  bool ok = true;
+  for (int64_t f = r0; f < r1; next_item(a, p)) {
+    const int h = p.item % g.kvh, cb = p.item / g.kvh;
+    const int tb = p.tile, t1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
+    f += t1 - tb;
+    stage_q<HD, SPLIT>(a, p, h, cb, warp, lane, &sh.q);
+    bar_consumers();
+    uint32_t qf[KS][SPLIT ? 4 : 2];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) ldv(reinterpret_cast<const uint8_t*>(sh.q.frag + (k * 32 + lane) * QStage<HD, SPLIT>::W), qf[k]);
+    float qsum[2][NG], mul[2];
+    int lim[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      mul[q] = sh.q.mul[2 * c + q];
+      lim[q] = sh.q.lim[2 * c + q];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        qsum[q][i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < GROUP / 64; ++w) qsum[q][i] += sh.q.sum[2 * c + q][i * (GROUP / 64) + w];
+      }
+    }
+    const int free_to = __reduce_min_sync(0xffffffffu, min(lim[0], lim[1]));  // every column sees slots up to here
+    float o[NW * 4][4];
+    float pb[NG][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int K = 0;             // p carries a factor 2^K (K = 14 - exponent of the largest value scale)
+    unsigned smax = 0u;    // that scale's bits
+#pragma unroll
+    for (int i = 0; i < NW * 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) pb[i][0] = pb[i][1] = 0.f;
+
+    for (int t = tb; t < t1; ++t, ++j) {
+      const int s = j % S;
+      if (ok && !mbar_wait(&sh.full[s], (j / S) & 1)) {
+        ok = false;
+        if (lane == 0 && a.b.status) atomicOr(a.b.status, 1);
+      }
+      const int s0 = t * AT_TILE + warp * 16;
+      if (s0 < p.len) {
+        const uint8_t* st = sh.ring[s];
+        const bool lost = (sh.bad[s] >> piece) & 1;
+        const bool live0 = !lost && s0 + r < p.len, live1 = !lost && s0 + r + 8 < p.len;
+        const bool edge = lost || s0 + 15 > free_to || s0 + 15 >= p.len;
+        uint32_t kw[2][2][NW], kp[2][NG], vp[2][NG], vw[4][NW];
+        ldv(st + kbase + koff0, kw[0][0]);
+        ldv(st + kbase + koff0 + 8 * (HD / 2), kw[0][1]);
+        ldv(st + kbase + koff1, kw[1][0]);
+        ldv(st + kbase + koff1 + 8 * (HD / 2), kw[1][1]);
+        ldv(st + kbase + pbase + (trow + r) * NG * 4, kp[0]);
+        ldv(st + kbase + pbase + (trow + r + 8) * NG * 4, kp[1]);
+        ldv(st + vbase + pbase + (trow + r) * NG * 4, vp[0]);
+        ldv(st + vbase + pbase + (trow + r + 8) * NG * 4, vp[1]);
+        ldv(st + vbase + voff0, vw[0]);
+        ldv(st + vbase + voff1, vw[1]);
+        ldv(st + vbase + voff0 + 8 * (HD / 2), vw[2]);
+        ldv(st + vbase + voff1 + 8 * (HD / 2), vw[3]);
+        float x[4];
+        scores<HD, GROUP, SPLIT>(kw, kp, qsum, [&](int k, uint32_t (&b)[SPLIT ? 4 : 2]) {
+#pragma unroll
+          for (int i = 0; i < (SPLIT ? 4 : 2); ++i) b[i] = qf[k][i];
+        }, x);
+        bool see[4] = {true, true, true, true};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= mul[i & 1];
+        if (edge) {
+          // what a column does not see: no weight, whatever the memory holds
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            see[i] = (i < 2 ? live0 : live1) && s0 + r + (i < 2 ? 0 : 8) <= lim[i & 1];
+            if (!see[i]) x[i] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            if (!live0) vp[0][i] = 0u;
+            if (!live1) vp[1][i] = 0u;
+          }
+        }
+        // running maximum of each column, and of the value scales; a NaN
+        // score counts as infinity, so that the column ends as NaN
+        auto up_nan = [](float v) { return v != v ? INFINITY : v; };
+        float mx[2] = {fmaxf(up_nan(x[0]), up_nan(x[2])), fmaxf(up_nan(x[1]), up_nan(x[3]))};
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], d));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], d));
+        }
+        unsigned sb = 0u;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) sb = max(sb, max(vp[0][i] & 0x7fffu, vp[1][i] & 0x7fffu));
+        sb = __reduce_max_sync(0xffffffffu, min(sb, 0x7bffu));
+        const bool grow = sb > smax;
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1]) || grow) {
+          int dk = 0;
+          if (grow) {
+            smax = sb;
+            const int e = int(__float_as_uint(__half2float(__ushort_as_half((unsigned short)sb))) >> 23) - 127;
+            dk = 14 - e - K;
+            K = 14 - e;
+          }
+          const float up = ex2(float(dk));
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float mn = fmaxf(m[q], mx[q]);
+            const float al = m[q] == -INFINITY ? 0.f : ex2(m[q] - mn) * up;
+            m[q] = mn;
+            l[q] *= al;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) pb[i][q] *= al;
+#pragma unroll
+            for (int i = 0; i < NW * 4; ++i) {
+              o[i][q] *= al;
+              o[i][q + 2] *= al;
+            }
+          }
+        }
+        float pr[4];
+        {
+          const float mk0 = m[0] == -INFINITY ? 0.f : m[0] - float(K), mk1 = m[1] == -INFINITY ? 0.f : m[1] - float(K);
+          pr[0] = ex2(x[0] - mk0);
+          pr[1] = ex2(x[1] - mk1);
+          pr[2] = ex2(x[2] - mk0);
+          pr[3] = ex2(x[3] - mk1);
+        }
+        l[0] += pr[0] + pr[2];
+        l[1] += pr[1] + pr[3];
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          const float2 v0 = kv4_param(vp[0][gi]), v1 = kv4_param(vp[1][gi]);
+          const float b0 = fmaf(7.5f, v0.x, v0.y), b1 = fmaf(7.5f, v1.x, v1.y);
+          float ps[4] = {pr[0] * v0.x, pr[1] * v0.x, pr[2] * v1.x, pr[3] * v1.x};
+          float pm[4] = {pr[0] * b0, pr[1] * b0, pr[2] * b1, pr[3] * b1};
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!see[i]) ps[i] = pm[i] = 0.f;
+          }
+          pb[gi][0] += pm[0] + pm[2];
+          pb[gi][1] += pm[1] + pm[3];
+          const __half2 h0 = __floats2half2_rn(ps[0], ps[1]), h1 = __floats2half2_rn(ps[2], ps[3]);
+          const uint32_t bh0 = movm(h2u(h0)), bh1 = movm(h2u(h1));
+          uint32_t bl0 = 0, bl1 = 0;
+          if (SPLIT) {
+            const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+            bl0 = movm(h2u(__floats2half2_rn(ps[0] - f0.x, ps[1] - f0.y)));
+            bl1 = movm(h2u(__floats2half2_rn(ps[2] - f1.x, ps[3] - f1.y)));
+          }
+#pragma unroll
+          for (int w = 0; w < GROUP / 64; ++w) {
+            const int wi = gi * (GROUP / 64) + w;
+#pragma unroll
+            for (int pt = 0; pt < 2; ++pt) {
+              const uint32_t sel = pt ? 0x7632u : 0x5410u;
+              const uint32_t ab = prmt(vw[0][wi], vw[1][wi], sel), cd = prmt(vw[2][wi], vw[3][wi], sel);
+#pragma unroll
+              for (int st2 = 0; st2 < 2; ++st2) {
+                uint32_t a0, a1, a2, a3;
+                unpack2(st2 ? ab >> 7 : ab << 1, a0, a1);
+                unpack2(st2 ? cd >> 7 : cd << 1, a2, a3);
+                float(&d)[4] = o[wi * 4 + pt * 2 + st2];
+                mma16816(d, a0, a1, a2, a3, bh0, bh1);
+                if (SPLIT) mma16816(d, a0, a1, a2, a3, bl0, bl1);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[s]);
+    }
+
+    // ---- the item's share is done: combine the warps ----
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        l[q] += __shfl_xor_sync(0xffffffffu, l[q], d);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) pb[i][q] += __shfl_xor_sync(0xffffffffu, pb[i][q], d);
+      }
+    if (r == 0) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        sh.m[warp][2 * c + q] = m[q];
+        sh.l[warp][2 * c + q] = l[q] * ex2(float(-K));
+      }
+    }
+    bar_consumers();
+    float fw[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < AT_WARPS; ++w) M = fmaxf(M, sh.m[w][2 * c + q]);
+      fw[q] = m[q] == -INFINITY ? 0.f : ex2(m[q] - M) * ex2(float(-K));
+    }
+    // [word][column parity][k][lane]: k-th of 8 channels that a lane holds of a 64-channel block for a column
+#pragma unroll
+    for (int wi = 0; wi < NW; ++wi)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          sh.red[warp][((wi * 2 + q) * 8 + k) * 32 + lane] =
+              m[q] == -INFINITY ? 0.f : (o[wi * 4 + k / 2][q + 2 * (k & 1)] + pb[wi / (GROUP / 64)][q]) * fw[q];
+    bar_consumers();
+    const int e = threadIdx.x >> 6, q = (threadIdx.x >> 5) & 1;  // 64-channel block, column parity
+    if (e < NW) {
+      const int col = 2 * c + q;
+      float v[8], M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < AT_WARPS; ++w) M = fmaxf(M, sh.m[w][col]);
+#pragma unroll
+      for (int w = 0; w < AT_WARPS; ++w) {
+        const float mw = sh.m[w][col];
+        if (mw != -INFINITY) L += sh.l[w][col] * ex2(mw - M);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[k] = 0.f;
+#pragma unroll
+        for (int w = 0; w < AT_WARPS; ++w) v[k] += sh.red[w][((e * 2 + q) * 8 + k) * 32 + lane];
+      }
+      const int ch = e * 64 + r * 8;
+      if (tb == 0 && t1 == p.tiles) {
+        const int ci = cb * AT_COLS + col, tok = ci / a.rep, hq = h * a.rep + ci % a.rep;
+        if (tok < p.n) {
+          const float inv = M == -INFINITY ? 0.f : 1.f / L;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] *= inv;
+          write_out(a, p.row0 + tok, hq, ch, v);
+          if (ch == 0) attn_lse(a)[int64_t(p.row0 + tok) * a.heads + hq] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * LN2;
+        }
+      } else {
+        // an item that goes on in another CTA: slot 0 if it began before this CTA, slot 1 if it begins here
+        float* part = attn_parts(a) + (int64_t(blockIdx.x) * 2 + (tb == 0 ? 1 : 0)) * part_floats(HD);
+        if (ch == 0) {
+          part[col] = M;
+          part[AT_COLS + col] = L;
+        }
+        float4* d = reinterpret_cast<float4*>(part + 2 * AT_COLS + col * HD + ch);
+        d[0] = make_float4(v[0], v[1], v[2], v[3]);
+        d[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
+  }
+}
+
+// Joins the parts of the item that begins in share x and goes on: one block per
+// (share, column).
 template <int HD>
-void run_rows(const Kv4AttnArgs& a, cudaStream_t st) {
-  const int64_t warps = int64_t(a.b.total) * a.heads;
-  launch(k_kv4_attn_rows<HD>, dim3(unsigned((warps + SA_WARPS - 1) / SA_WARPS)), dim3(SA_WARPS * 32), 0, st, false, a);
+__global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
+  const int nc = gridDim.x, x = blockIdx.x, col = blockIdx.y;
+  const int64_t total = total_tiles(a);
+  const int64_t r0 = total * x / nc, r1 = total * (x + 1) / nc;
+  Place p = {};
+  if (r0 < r1) p = find_place(a, r1 - 1);
+  const int64_t begin = r1 - 1 - p.tile, end = begin + p.tiles;
+  const int h = p.item % a.g.kvh, cb = p.item / a.g.kvh;
+  const int ci = cb * AT_COLS + col, tok = ci / a.rep, hq = h * a.rep + ci % a.rep;
+  pdl_wait();  // by every block: this launch ends after the one before it
+  if (r0 == r1 || begin < r0 || end <= r1 || tok >= p.n) return;
+  __shared__ float wt[AT_GRID];
+  __shared__ float red[32];
+  const float* parts = attn_parts(a);
+  auto part = [&](int i) { return parts + (int64_t(i) * 2 + (i == x ? 1 : 0)) * part_floats(HD); };
+  // shares x .. last hold parts of the item (those without tiles none)
+  int last = x;
+  while (last + 1 < nc && total * (last + 1) / nc < end) ++last;
+  const int np = last - x + 1;
+  float M = -INFINITY;
+  for (int i = threadIdx.x; i < np; i += HD) {
+    const bool has = total * (x + i + 1) / nc > total * (x + i) / nc;
+    const float mi = has ? __ldcg(part(x + i) + col) : -INFINITY;
+    wt[i] = mi;
+    M = fmaxf(M, mi);
+  }
+  M = warp_max(M);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = M;
+  __syncthreads();
+  M = red[0];
+  for (int w = 1; w < HD / 32; ++w) M = fmaxf(M, red[w]);
+  __syncthreads();
+  float L = 0.f;
+  for (int i = threadIdx.x; i < np; i += HD) {
+    const float mi = wt[i], f = mi == -INFINITY ? 0.f : ex2(mi - M);
+    if (mi != -INFINITY) L += __ldcg(part(x + i) + AT_COLS + col) * f;
+    wt[i] = f;
+  }
+  L = block_sum(L, red);
+  float v = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < np; ++i) {
+    const float f = wt[i];
+    if (f != 0.f) v = fmaf(f, __ldcg(part(x + i) + 2 * AT_COLS + col * HD + threadIdx.x), v);
+  }
+  v = M == -INFINITY ? 0.f : v / L;
+  const int64_t row = p.row0 + tok;
+  const int ch = threadIdx.x;
+  if (a.gate.p) v *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch));
+  kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, v);
+  if (ch == 0) attn_lse(a)[row * a.heads + hq] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * LN2;
+}
+
+// ------------------------------------------------------- accumulated weight --
+// weights[t] += sum over the columns that see slot t of exp(score - lse), the
+// scores computed again from the keys alone (half the cache's bytes; writing
+// them out and reading them back would be as much at 8 query heads a kv head
+// and would need space of rows x slots). A CTA owns 128 slots of a kv head and
+// walks all the sequence's columns, so every sum has one order.
+template <int HD, int GROUP, bool SPLIT>
+__global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs a) {
+  constexpr int NG = HD / GROUP, NW = HD / 64;
+  __shared__ __align__(16) QStage<HD, SPLIT> sq[2];
+  __shared__ float slse[2][AT_COLS];
+  const Kv4Geo& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int h = blockIdx.y;
+  Place p;
+  load_seq(a, blockIdx.z, p);
+  const int tile0 = blockIdx.x * AT_TILE;
+  if (tile0 >= p.len || p.n == 0) return;
+  const int s0 = tile0 + warp * 16;
+  const uint8_t* blk = s0 < p.len ? kv4_block(g, g.table, g.tstride, p.seq, h, s0, a.b.status) : nullptr;
+  uint32_t kw[2][2][NW], kp[2][NG];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = (s0 & (g.seg - 1)) + r + 8 * i;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) kw[0][i][w] = kw[1][i][w] = 0u;
+#pragma unroll
+    for (int w = 0; w < NG; ++w) kp[i][w] = 0u;
+    if (blk) {
+      ldv(blk + t * (HD / 2) + (c ^ kv4_swz(HD, t)) * (HD / 16), kw[0][i]);
+      ldv(blk + t * (HD / 2) + ((c + 4) ^ kv4_swz(HD, t)) * (HD / 16), kw[1][i]);
+      ldv(blk + g.seg * (HD / 2) + t * NG * 4, kp[i]);
+    }
+  }
+  const float* lse = attn_lse(a);
+  const int ncb = (p.n * a.rep + AT_COLS - 1) / AT_COLS;
+  // the first column block with a token that sees the tile's first slot
+  const int first = int(max(int64_t(0), int64_t(tile0) - (p.len - p.n)) * a.rep / AT_COLS);
+  float w0 = 0.f, w1 = 0.f;
+  for (int cb = first; cb < ncb; ++cb) {
+    QStage<HD, SPLIT>& q = sq[cb & 1];
+    stage_q<HD, SPLIT>(a, p, h, cb, warp, lane, &q);
+    if (lane == 0) {
+      const int ci = cb * AT_COLS + warp, tok = ci / a.rep;
+      slse[cb & 1][warp] = tok < p.n ? lse[int64_t(p.row0 + tok) * a.heads + h * a.rep + ci % a.rep] * LOG2E : INFINITY;
+    }
+    __syncthreads();
+    float qsum[2][NG], x[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        qsum[k][i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < GROUP / 64; ++w) qsum[k][i] += q.sum[2 * c + k][i * (GROUP / 64) + w];
+      }
+    scores<HD, GROUP, SPLIT>(kw, kp, qsum, [&](int k, uint32_t (&b)[SPLIT ? 4 : 2]) {
+      ldv(reinterpret_cast<const uint8_t*>(q.frag + (k * 32 + lane) * QStage<HD, SPLIT>::W), b);
+    }, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = i & 1, slot = s0 + r + (i < 2 ? 0 : 8);
+      const bool see = slot <= q.lim[2 * c + k] && cb * AT_COLS + 2 * c + k < p.n * a.rep;
+      const float e = see ? ex2(fmaf(x[i], q.mul[2 * c + k], -slse[cb & 1][2 * c + k])) : 0.f;
+      if (i < 2) w0 += e; else w1 += e;
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    w0 += __shfl_xor_sync(0xffffffffu, w0, d);
+    w1 += __shfl_xor_sync(0xffffffffu, w1, d);
+  }
+  if (c == 0 && blk) {
+    float* w = a.weights + (int64_t(p.seq) * g.kvh + h) * a.wstride;
+    if (s0 + r < p.len) w[s0 + r] += w0;
+    if (s0 + r + 8 < p.len) w[s0 + r + 8] += w1;
+  }
+}
+
+template <int HD, int GROUP, bool SPLIT>
+void run(const Kv4AttnArgs& a, cudaStream_t st) {
+  launch(k_kv4_attn<HD, GROUP, SPLIT>, dim3(AT_GRID), dim3(AT_THREADS), sizeof(AttnShared<HD, GROUP, SPLIT>), st, false, a);
+  launch(k_kv4_attn_join<HD>, dim3(AT_GRID, AT_COLS), dim3(HD), 0, st, true, a);
   if (a.weights && a.b.max_len > 0)
-    launch(k_kv4_weights_rows<HD>, dim3((a.b.max_len + SA_WARPS - 1) / SA_WARPS, a.g.kvh, a.b.nseq), dim3(SA_WARPS * 32), 0, st,
+    launch(k_kv4_weights<HD, GROUP, SPLIT>, dim3((a.b.max_len + AT_TILE - 1) / AT_TILE, a.g.kvh, a.b.nseq), dim3(AT_WARPS * 32), 0, st,
            false, a);
+}
+
+template <int HD, int GROUP>
+void run_dt(const Kv4AttnArgs& a, cudaStream_t st) {
+  if (a.dt == DT_F32) run<HD, GROUP, true>(a, st);
+  else run<HD, GROUP, false>(a, st);
 }
 
 }  // namespace
 
-int64_t kv4_attention_work(const Kv4Geo& g, const Kv4Batch& b, int heads) { return std::max<int64_t>(16, int64_t(b.total) * heads * 4); }
+int64_t kv4_attention_work(const Kv4Geo& g, const Kv4Batch& b, int heads) {
+  return (int64_t(b.total) * heads * 4 + 15) / 16 * 16 + int64_t(AT_GRID) * 2 * part_floats(g.hd) * 4;
+}
 
 void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
-  if (a.g.hd == 64) run_rows<64>(a, st);
-  else if (a.g.hd == 128) run_rows<128>(a, st);
-  else run_rows<256>(a, st);
+  if (a.g.hd == 64) run_dt<64, 64>(a, st);
+  else if (a.g.hd == 128) a.g.group == 64 ? run_dt<128, 64>(a, st) : run_dt<128, 128>(a, st);
+  else a.g.group == 64 ? run_dt<256, 64>(a, st) : run_dt<256, 128>(a, st);
 }
 
 }  // namespace swl
