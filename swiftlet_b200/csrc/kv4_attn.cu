@@ -6,20 +6,25 @@
 // large common term):
 //   q.k_t = sum_g s_tg (sum_{i in g} q_i e_ti) + b'_tg (sum_{i in g} q_i)
 //   out_i = sum_t (p_t s_tg) e_ti + sum_t p_t b'_tg          (i in group g)
-// e is exact in f16, so both inner sums are matrix products of exact 4-bit
-// operands: mma.m16n8k16 (f16, f32 accumulators) with 16 slots x 16 channels
-// of codes against the 8 query columns of a kv head, per group, and 16
-// channels x 16 slots against the weights p s. For f32 inputs q and p s go in
-// as two f16 terms each (22 bits); for 16-bit inputs q is exact (bf16) or
+// Codes are exact in f16, so both inner sums are matrix products of exact
+// 4-bit operands: mma.m16n8k16 (f16, f32 accumulators) with 16 slots x 16
+// channels of codes against the 8 query columns of a kv head, per group, and
+// 16 channels x 16 slots against the weights p s. For f32 inputs q and p s go
+// in as two f16 terms each (22 bits); for 16-bit inputs q is exact (bf16) or
 // itself (f16) and p s is rounded to 11 bits. Softmax statistics, group sums
 // and outputs are f32. Columns are scaled by powers of two on their way into
 // f16 (q by its largest element, p by the largest group scale seen), which
 // changes no bit of the result but keeps both terms in range.
+// For 16-bit inputs e = c, b' = b: one LOP3 a pair. For f32 inputs e = c -
+// 7.5 and b' = b + 7.5 s, the middle of the group (10 instructions per 8 codes
+// instead of 5): the accumulators truncate, so a sum is off by its largest
+// partial sums, and with codes of one sign those are twice the score's (its
+// error then measured 7.6e-6 on scores of 1.5) and 150 times the output's (at
+// 128k equal weights).
 //
-// Bound: the cache's bytes (2 (D / 2 + 4 D / g) a slot and kv head). The
-// unpacking costs 10 ALU instructions per 8 codes, about two thirds of the
-// issue slots at the HBM rate, which is why codes go to the tensor cores
-// unscaled and the scales are applied to the 16 x 8 results instead.
+// Bound: the cache's bytes (2 (D / 2 + 4 D / g) a slot and kv head), next to
+// the instructions of unpacking and weighting, which is why codes go to the
+// tensor cores unscaled and the scales are applied to the 16 x 8 results.
 #include <algorithm>
 
 #include "kcommon.cuh"
@@ -30,11 +35,13 @@ namespace swl {
 
 namespace {
 
-constexpr int AT_WARPS = 8;                 // consumer warps, 16 slots of a tile each
-constexpr int AT_THREADS = AT_WARPS * 32 + 32;  // and one producer warp
-constexpr int AT_TILE = 16 * AT_WARPS;      // slots of a tile
+constexpr int AT_WARPS = 16;                // four per scheduler: the chains of a 16-slot unit need them to overlap
+constexpr int AT_THREADS = AT_WARPS * 32;
+constexpr int AT_UNIT = 16;                 // slots a warp takes at a time: the MMA's M (keys) and K (values)
+constexpr int AT_TILE = 128;                // slots of a tile, the grain in which work is shared out
 constexpr int AT_COLS = 8;                  // query columns (token, head) of an item: the MMA's N
 constexpr int AT_GRID = 148;                // one CTA per SM
+constexpr int WT_WARPS = 8;                 // warps of the weight kernel: one tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // ------------------------------------------------------------ primitives --
@@ -44,23 +51,27 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Transpose of an 8 x 8 matrix of 16-bit elements spread over the warp.
 __device__ __forceinline__ uint32_t movm(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// Nibbles 0 and 1 of both halves of a word as two f16 pairs, each minus 7.5:
-// a code at bits 1..4 of 0x6000 (512, step 0.5) is 512 + c, at bits 5..8
-// 512 + 16 c; both results are exact.
-__device__ __forceinline__ void unpack2(uint32_t x, uint32_t& n0, uint32_t& n1) {
+// Nibbles 0 and 1 of both halves of a word as two f16 pairs. Plain: the bits
+// themselves, subnormals 2^-24 c and 2^-20 c. Centred: c - 7.5; a code at bits
+// 1..4 of 0x6000 (512, step 0.5) is 512 + c, at bits 5..8 512 + 16 c, and both
+// results are exact (x is the word shifted left by one).
+__device__ __forceinline__ void unpack_plain(uint32_t x, uint32_t& n0, uint32_t& n1) {
+  n0 = x & 0x000f000fu;
+  n1 = x & 0x00f000f0u;
+}
+__device__ __forceinline__ void unpack_centred(uint32_t x, uint32_t& n0, uint32_t& n1) {
   const __half2 m0 = u2h(0xe00fe00fu);                    // -519.5
   const __half2 m1 = u2h(0xd0f0d0f0u), r = u2h(0x2c002c00u);  // -39.5, 1 / 16
   n0 = h2u(__hadd2(u2h((x & 0x001e001eu) | 0x60006000u), m0));
@@ -84,7 +95,6 @@ __device__ __forceinline__ void ldv(const uint8_t* p, uint32_t (&w)[N]) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
-__device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // ------------------------------------------------------------------ work --
 // The work is the list of all (sequence, column block, kv head) items, each of
@@ -174,7 +184,7 @@ struct QStage {
   static constexpr int KS = HD / 16;  // k steps
   static constexpr int W = SPLIT ? 4 : 2;
   uint32_t frag[KS * 32 * W];        // B fragments: {hi b0, hi b1[, lo b0, lo b1]} per k step and lane
-  float sum[AT_COLS][HD / 64];       // sums of the scaled column over each 64 channels
+  float sum[AT_COLS][HD / 64];       // sums of the scaled column over each 64 channels, in the codes' unit
   float mul[AT_COLS];                // score = mul * (scaled sum), in units of log2
   int lim[AT_COLS];                  // last slot the column sees (INT_MAX: unused column)
 };
@@ -203,14 +213,15 @@ __device__ __forceinline__ void stage_q(const Kv4AttnArgs& a, const Place& p, in
   for (int e = 0; e < 8; ++e) {
     x[e] *= up;
     s += x[e];
-    const __half hh = __float2half_rn(x[e]);
+    const float y = !SPLIT && (e & 1) ? x[e] * 0.0625f : x[e];  // odd nibbles come unpacked as 16 c
+    const __half hh = __float2half_rn(y);
     hi[e] = __half_as_ushort(hh);
-    if (SPLIT) lo[e] = __half_as_ushort(__float2half_rn(x[e] - __half2float(hh)));
+    if (SPLIT) lo[e] = __half_as_ushort(__float2half_rn(y - __half2float(hh)));
   }
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (act) {
-    if ((lane & 7) == 0) qs->sum[col][lane >> 3] = s;
+    if ((lane & 7) == 0) qs->sum[col][lane >> 3] = SPLIT ? s : s * 0x1p-24f;
     const int wi = lane >> 3, u = lane & 7;
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
@@ -224,7 +235,7 @@ __device__ __forceinline__ void stage_q(const Kv4AttnArgs& a, const Place& p, in
     }
   }
   if (lane == 0) {
-    qs->mul[col] = a.scale * LOG2E * __int_as_float((127 - ex) << 23);
+    qs->mul[col] = a.scale * LOG2E * __int_as_float((127 - ex) << 23) * (SPLIT ? 1.f : 0x1p24f);
     qs->lim[col] = on ? p.len - p.n + t : 0x7fffffff;
   }
 }
@@ -246,36 +257,42 @@ __device__ __forceinline__ void scores(const uint32_t (&kw)[2][2][HD / 64], cons
       for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          const uint32_t x0 = st ? kw[hf][0][wi] >> 7 : kw[hf][0][wi] << 1, x1 = st ? kw[hf][1][wi] >> 7 : kw[hf][1][wi] << 1;
           uint32_t a0, a1, a2, a3;
-          unpack2(x0, a0, a2);
-          unpack2(x1, a1, a3);
+          if (SPLIT) {
+            unpack_centred(st ? kw[hf][0][wi] >> 7 : kw[hf][0][wi] << 1, a0, a2);
+            unpack_centred(st ? kw[hf][1][wi] >> 7 : kw[hf][1][wi] << 1, a1, a3);
+          } else {
+            unpack_plain(st ? kw[hf][0][wi] >> 8 : kw[hf][0][wi], a0, a2);
+            unpack_plain(st ? kw[hf][1][wi] >> 8 : kw[hf][1][wi], a1, a3);
+          }
           uint32_t b[SPLIT ? 4 : 2];
           qf((wi * 2 + hf) * 2 + st, b);
           mma16816(acc, a0, a1, a2, a3, b[0], b[1]);
           if constexpr (SPLIT) mma16816(acc, a0, a1, a2, a3, b[2], b[3]);
         }
     }
-    const float2 s0 = kv4_param(kp[0][g]), s1 = kv4_param(kp[1][g]);
-    const float m0 = fmaf(7.5f, s0.x, s0.y), m1 = fmaf(7.5f, s1.x, s1.y);
-    sc[0] = fmaf(s0.x, acc[0], fmaf(m0, qsum[0][g], sc[0]));
-    sc[1] = fmaf(s0.x, acc[1], fmaf(m0, qsum[1][g], sc[1]));
-    sc[2] = fmaf(s1.x, acc[2], fmaf(m1, qsum[0][g], sc[2]));
-    sc[3] = fmaf(s1.x, acc[3], fmaf(m1, qsum[1][g], sc[3]));
+    float2 s0 = kv4_param(kp[0][g]), s1 = kv4_param(kp[1][g]);
+    if (SPLIT) {  // the middle of the group
+      s0.y = fmaf(7.5f, s0.x, s0.y);
+      s1.y = fmaf(7.5f, s1.x, s1.y);
+    }
+    sc[0] = fmaf(s0.x, acc[0], fmaf(s0.y, qsum[0][g], sc[0]));
+    sc[1] = fmaf(s0.x, acc[1], fmaf(s0.y, qsum[1][g], sc[1]));
+    sc[2] = fmaf(s1.x, acc[2], fmaf(s1.y, qsum[0][g], sc[2]));
+    sc[3] = fmaf(s1.x, acc[3], fmaf(s1.y, qsum[1][g], sc[3]));
   }
 }
 
 template <int HD, int GROUP, bool SPLIT>
 struct AttnShared {
-  static constexpr int ROW = HD / 2 + 4 * (HD / GROUP);
-  static constexpr int TILE_BYTES = 2 * AT_TILE * ROW;
-  static constexpr int STAGES = HD == 256 ? 4 : 8;
-  alignas(128) uint8_t ring[STAGES][TILE_BYTES];
-  float red[AT_WARPS][AT_COLS * HD];  // outputs of the warps, in fragment order
+  static constexpr int CODES = AT_UNIT * HD / 2, PARAMS = AT_UNIT * 4 * (HD / GROUP);  // bytes of a unit's keys (values)
+  static constexpr int UNIT_BYTES = 2 * (CODES + PARAMS);
+  static constexpr int STAGES = HD == 256 ? 3 : HD == 128 ? 6 : 8;  // units in flight a warp: about 14 KB
+  static constexpr int SLICE = STAGES * UNIT_BYTES;                 // one warp's ring, its outputs at the end of an item
+  static_assert(SLICE >= AT_COLS * HD * 4, "a warp's outputs fit its ring");
+  alignas(128) uint8_t ring[AT_WARPS][SLICE];
   QStage<HD, SPLIT> q;
-  float m[AT_WARPS][AT_COLS], l[AT_WARPS][AT_COLS];
-  uint64_t full[STAGES], empty[STAGES];
-  int bad[STAGES];  // pieces of the tile whose page id is outside the pool
+  float m[AT_WARPS][AT_COLS], l[AT_WARPS][AT_COLS], f[AT_WARPS];  // maxima, sums, factors 2^-K of the warps
 };
 
 // Floats of one partial result: max, sum, outputs.
@@ -286,92 +303,73 @@ __device__ __forceinline__ float* attn_parts(const Kv4AttnArgs& a) {
   return reinterpret_cast<float*>(a.work + (int64_t(a.b.total) * a.heads * 4 + 15) / 16 * 16);
 }
 
-// Eight consecutive outputs of a row, gated.
-__device__ __forceinline__ void write_out(const Kv4AttnArgs& a, int64_t row, int hq, int ch, const float (&v)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float r = v[e];
-    if (a.gate.p) r *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch + e));
-    kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch + e, r);
-  }
+// One output of a row, gated.
+__device__ __forceinline__ void write_out(const Kv4AttnArgs& a, int64_t row, int hq, int ch, float v) {
+  if (a.gate.p) v *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch));
+  kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, v);
 }
 
 template <int HD, int GROUP, bool SPLIT>
 __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a) {
   using Sh = AttnShared<HD, GROUP, SPLIT>;
-  constexpr int NG = HD / GROUP, NW = HD / 64, KS = HD / 16, S = Sh::STAGES;
+  constexpr int NG = HD / GROUP, NW = HD / 64, S = Sh::STAGES;
   extern __shared__ __align__(128) uint8_t at_raw[];
   Sh& sh = *reinterpret_cast<Sh*>(at_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < S; ++s) {
-      mbar_init(&sh.full[s], 1);
-      mbar_init(&sh.empty[s], AT_WARPS);
-    }
-    mbar_init_fence();
-  }
   pdl_launch();
   const int64_t total = total_tiles(a);
   const int64_t r0 = total * blockIdx.x / gridDim.x, r1 = total * (blockIdx.x + 1) / gridDim.x;
-  __syncthreads();
   if (r0 == r1) return;
   Place p = find_place(a, r0);
   const Kv4Geo& g = a.g;
-
-  if (warp == AT_WARPS) {
-    // -------------------------------------------------------- producer ----
-    // One bulk copy per block of the tile (keys, values and params of up to
-    // 64 slots of the kv head lie together); the lanes look the pages up.
-    const int seg = g.seg, np = AT_TILE / seg;
-    int j = 0;
-    bool ok = true;
-    for (int64_t f = r0; f < r1 && ok; next_item(a, p)) {
-      const int h = p.item % g.kvh;
-      const int t1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
-      for (int t = p.tile; t < t1; ++t, ++j, ++f) {
-        const int s = j % S;
-        if (!mbar_wait(&sh.empty[s], ((j / S) & 1) ^ 1)) { ok = false; break; }
-        const int slot = t * AT_TILE + lane * seg;
-        const bool want = lane < np && slot < p.len;
-        const uint8_t* src = want ? kv4_block(g, g.table, g.tstride, p.seq, h, slot, a.b.status) : nullptr;
-        const unsigned have = __ballot_sync(0xffffffffu, src != nullptr), bad = __ballot_sync(0xffffffffu, want && !src);
-        if (lane == 0) {
-          sh.bad[s] = int(bad);
-          mbar_expect_tx(&sh.full[s], unsigned(__popc(have)) * unsigned(g.blk));
-        }
-        __syncwarp();
-        if (src) bulk_g2s_keep(sh.ring[s] + lane * g.blk, src, unsigned(g.blk), &sh.full[s]);
-      }
-    }
-    if (!ok) {
-      // a consumer did not free its slot: report it, and let the copies in
-      // flight land before the CTA may end
-      if (lane == 0 && a.b.status) atomicOr(a.b.status, 1);
-      for (int i = max(0, j - S); i < j; ++i) mbar_wait(&sh.full[i % S], (i / S) & 1);
-    }
-    return;
-  }
-
-  // ---------------------------------------------------------- consumers ----
   const int r = lane >> 2, c = lane & 3;
-  const int piece = warp * 16 / g.seg, trow = (warp * 16) & (g.seg - 1);
-  const int kbase = piece * g.blk, vbase = kbase + g.blk / 2, pbase = g.seg * (HD / 2);
-  // offsets of this lane's vectors within a block (constant over the tiles)
-  const int koff0 = (trow + r) * (HD / 2) + ((c ^ kv4_swz(HD, r)) * (HD / 16));
-  const int koff1 = (trow + r) * (HD / 2) + (((c + 4) ^ kv4_swz(HD, r)) * (HD / 16));
-  const int voff0 = (trow + 2 * c) * (HD / 2) + ((r ^ kv4_swz(HD, 2 * c)) * (HD / 16));
-  const int voff1 = (trow + 2 * c + 1) * (HD / 2) + ((r ^ kv4_swz(HD, 2 * c + 1)) * (HD / 16));
-  int j = 0;
-  bool ok = true;
+  uint8_t* ring = sh.ring[warp];
+  // this lane's vectors within a unit's keys and values
+  const int koff0 = r * (HD / 2) + (c ^ kv4_swz(HD, r)) * (HD / 16), koff1 = r * (HD / 2) + ((c + 4) ^ kv4_swz(HD, r)) * (HD / 16);
+  const int voff0 = 2 * c * (HD / 2) + (r ^ kv4_swz(HD, 2 * c)) * (HD / 16);
+  const int voff1 = (2 * c + 1) * (HD / 2) + (r ^ kv4_swz(HD, 2 * c + 1)) * (HD / 16);
+  const int nblk = g.page / g.seg;
+
   for (int64_t f = r0; f < r1; next_item(a, p)) {
     const int h = p.item % g.kvh, cb = p.item / g.kvh;
     const int tb = p.tile, t1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
     f += t1 - tb;
-    stage_q<HD, SPLIT>(a, p, h, cb, warp, lane, &sh.q);
-    bar_consumers();
-    uint32_t qf[KS][SPLIT ? 4 : 2];
+    // units u0, u0 + 16, ... < u1 are this warp's
+    const int u0 = tb * (AT_TILE / AT_UNIT) + warp, u1 = min(t1 * (AT_TILE / AT_UNIT), (p.len + AT_UNIT - 1) / AT_UNIT);
+    const int* tab = g.table + p.seq * g.tstride;
+    auto page_of = [&](int u) { return u < u1 ? __ldg(tab + ((u * AT_UNIT) >> g.pshift)) : 0; };
+    unsigned lost = 0u;  // bit s: the page of stage s is outside the pool
+    // the unit's keys, their params, values and theirs by 16-byte copies into this warp's own stage
+    auto issue = [&](int u, int pg, int s) {
+      lost &= ~(1u << s);
+      if (u < u1) {
+        if (unsigned(pg) < unsigned(g.npages)) {
+          const int slot = u * AT_UNIT, t = slot & (g.seg - 1);
+          const uint8_t* blk = g.pages + pg * g.page_bytes + int64_t(h * nblk + (slot & (g.page - 1)) / g.seg) * g.blk;
+          const uint8_t* kc = blk + t * (HD / 2) + lane * 16;
+          uint8_t* d = ring + s * Sh::UNIT_BYTES;
+          constexpr int NC = Sh::CODES / 512, NP = Sh::PARAMS / 16;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) ldv(reinterpret_cast<const uint8_t*>(sh.q.frag + (k * 32 + lane) * QStage<HD, SPLIT>::W), qf[k]);
+          for (int i = 0; i < NC; ++i) {
+            cp_async16(d + i * 512 + lane * 16, kc + i * 512);
+            cp_async16(d + Sh::CODES + Sh::PARAMS + i * 512 + lane * 16, kc + g.blk / 2 + i * 512);
+          }
+          const int hv = lane >> 4, lp = lane & 15;
+          if (lp < NP)
+            cp_async16(d + Sh::CODES + hv * (Sh::CODES + Sh::PARAMS) + lp * 16,
+                       blk + hv * (g.blk / 2) + g.seg * (HD / 2) + t * NG * 4 + lp * 16);
+        } else {
+          lost |= 1u << s;
+          if (lane == 0 && a.b.status) atomicOr(a.b.status, KV4_BAD);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < S; ++s) issue(u0 + s * AT_WARPS, page_of(u0 + s * AT_WARPS), s);
+    int pg = page_of(u0 + S * AT_WARPS);
+    if (warp < AT_COLS) stage_q<HD, SPLIT>(a, p, h, cb, warp, lane, &sh.q);
+    __syncthreads();
     float qsum[2][NG], mul[2];
     int lim[2];
 #pragma unroll
@@ -395,146 +393,163 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
 #pragma unroll
     for (int i = 0; i < NG; ++i) pb[i][0] = pb[i][1] = 0.f;
 
-    for (int t = tb; t < t1; ++t, ++j) {
-      const int s = j % S;
-      if (ok && !mbar_wait(&sh.full[s], (j / S) & 1)) {
-        ok = false;
-        if (lane == 0 && a.b.status) atomicOr(a.b.status, 1);
-      }
-      const int s0 = t * AT_TILE + warp * 16;
-      if (s0 < p.len) {
-        const uint8_t* st = sh.ring[s];
-        const bool lost = (sh.bad[s] >> piece) & 1;
-        const bool live0 = !lost && s0 + r < p.len, live1 = !lost && s0 + r + 8 < p.len;
-        const bool edge = lost || s0 + 15 > free_to || s0 + 15 >= p.len;
-        uint32_t kw[2][2][NW], kp[2][NG], vp[2][NG], vw[4][NW];
-        ldv(st + kbase + koff0, kw[0][0]);
-        ldv(st + kbase + koff0 + 8 * (HD / 2), kw[0][1]);
-        ldv(st + kbase + koff1, kw[1][0]);
-        ldv(st + kbase + koff1 + 8 * (HD / 2), kw[1][1]);
-        ldv(st + kbase + pbase + (trow + r) * NG * 4, kp[0]);
-        ldv(st + kbase + pbase + (trow + r + 8) * NG * 4, kp[1]);
-        ldv(st + vbase + pbase + (trow + r) * NG * 4, vp[0]);
-        ldv(st + vbase + pbase + (trow + r + 8) * NG * 4, vp[1]);
-        ldv(st + vbase + voff0, vw[0]);
-        ldv(st + vbase + voff1, vw[1]);
-        ldv(st + vbase + voff0 + 8 * (HD / 2), vw[2]);
-        ldv(st + vbase + voff1 + 8 * (HD / 2), vw[3]);
-        float x[4];
+    int s = 0;
+    for (int u = u0; u < u1; u += AT_WARPS) {
+      cp_async_wait_group<S - 1>();
+      __syncwarp();
+      const int s0 = u * AT_UNIT;
+      const uint8_t* st = ring + s * Sh::UNIT_BYTES;
+      const uint8_t* sv = st + Sh::CODES + Sh::PARAMS;
+      const bool gone = (lost >> s) & 1;
+      const bool edge = gone || s0 + 15 > free_to || s0 + 15 >= p.len;
+      float x[4];
+      {
+        uint32_t kw[2][2][NW], kp[2][NG];
+        ldv(st + koff0, kw[0][0]);
+        ldv(st + koff0 + 8 * (HD / 2), kw[0][1]);
+        ldv(st + koff1, kw[1][0]);
+        ldv(st + koff1 + 8 * (HD / 2), kw[1][1]);
+        ldv(st + Sh::CODES + r * NG * 4, kp[0]);
+        ldv(st + Sh::CODES + (r + 8) * NG * 4, kp[1]);
         scores<HD, GROUP, SPLIT>(kw, kp, qsum, [&](int k, uint32_t (&b)[SPLIT ? 4 : 2]) {
-#pragma unroll
-          for (int i = 0; i < (SPLIT ? 4 : 2); ++i) b[i] = qf[k][i];
+          ldv(reinterpret_cast<const uint8_t*>(sh.q.frag + (k * 32 + lane) * QStage<HD, SPLIT>::W), b);
         }, x);
-        bool see[4] = {true, true, true, true};
+      }
+      uint32_t vp[2][NG], vw[4][NW];
+      ldv(sv + Sh::CODES + r * NG * 4, vp[0]);
+      ldv(sv + Sh::CODES + (r + 8) * NG * 4, vp[1]);
+      ldv(sv + voff0, vw[0]);
+      ldv(sv + voff1, vw[1]);
+      ldv(sv + voff0 + 8 * (HD / 2), vw[2]);
+      ldv(sv + voff1 + 8 * (HD / 2), vw[3]);
+      unsigned see = 15u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= mul[i & 1];
+      for (int i = 0; i < 4; ++i) x[i] *= mul[i & 1];
+      if (edge) {
+        // what a column does not see: no weight, whatever the memory holds
+        const bool live0 = !gone && s0 + r < p.len, live1 = !gone && s0 + r + 8 < p.len;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((i < 2 ? live0 : live1) && s0 + r + (i < 2 ? 0 : 8) <= lim[i & 1])) {
+            see &= ~(1u << i);
+            x[i] = -INFINITY;
+          }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          if (!live0) vp[0][i] = 0u;
+          if (!live1) vp[1][i] = 0u;
+        }
+      }
+      // running maximum of each column, and of the value scales; a NaN score
+      // counts as infinity, so that the column ends as NaN
+      auto up_nan = [](float v) { return v != v ? INFINITY : v; };
+      float mx[2] = {fmaxf(up_nan(x[0]), up_nan(x[2])), fmaxf(up_nan(x[1]), up_nan(x[3]))};
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], d));
+        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], d));
+      }
+      unsigned sb = 0u;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) sb = max(sb, max(vp[0][i] & 0x7fffu, vp[1][i] & 0x7fffu));
+      sb = __reduce_max_sync(0xffffffffu, min(sb, 0x7bffu));
+      const bool grow = sb > smax;
+      if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1]) || grow) {
+        int dk = 0;
+        if (grow) {
+          smax = sb;
+          const int e = int(__float_as_uint(__half2float(__ushort_as_half((unsigned short)sb))) >> 23) - 127;
+          dk = 14 - e - K;
+          K = 14 - e;
+        }
+        const float up = ex2(float(dk));
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float mn = fmaxf(m[q], mx[q]);
+          const float al = m[q] == -INFINITY ? 0.f : ex2(m[q] - mn) * up;
+          m[q] = mn;
+          l[q] *= al;
+#pragma unroll
+          for (int i = 0; i < NG; ++i) pb[i][q] *= al;
+#pragma unroll
+          for (int i = 0; i < NW * 4; ++i) {
+            o[i][q] *= al;
+            o[i][q + 2] *= al;
+          }
+        }
+      }
+      float pr[4];
+      {
+        const float mk0 = m[0] == -INFINITY ? 0.f : m[0] - float(K), mk1 = m[1] == -INFINITY ? 0.f : m[1] - float(K);
+        pr[0] = ex2(x[0] - mk0);
+        pr[1] = ex2(x[1] - mk1);
+        pr[2] = ex2(x[2] - mk0);
+        pr[3] = ex2(x[3] - mk1);
+      }
+      l[0] += pr[0] + pr[2];
+      l[1] += pr[1] + pr[3];
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) {
+        float2 v0 = kv4_param(vp[0][gi]), v1 = kv4_param(vp[1][gi]);
+        if (SPLIT) {  // the middle of the group
+          v0.y = fmaf(7.5f, v0.x, v0.y);
+          v1.y = fmaf(7.5f, v1.x, v1.y);
+        }
+        float ps[4] = {pr[0] * v0.x, pr[1] * v0.x, pr[2] * v1.x, pr[3] * v1.x};
         if (edge) {
-          // what a column does not see: no weight, whatever the memory holds
+          float pm[4] = {pr[0] * v0.y, pr[1] * v0.y, pr[2] * v1.y, pr[3] * v1.y};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            see[i] = (i < 2 ? live0 : live1) && s0 + r + (i < 2 ? 0 : 8) <= lim[i & 1];
-            if (!see[i]) x[i] = -INFINITY;
-          }
-#pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            if (!live0) vp[0][i] = 0u;
-            if (!live1) vp[1][i] = 0u;
-          }
-        }
-        // running maximum of each column, and of the value scales; a NaN
-        // score counts as infinity, so that the column ends as NaN
-        auto up_nan = [](float v) { return v != v ? INFINITY : v; };
-        float mx[2] = {fmaxf(up_nan(x[0]), up_nan(x[2])), fmaxf(up_nan(x[1]), up_nan(x[3]))};
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], d));
-          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], d));
-        }
-        unsigned sb = 0u;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) sb = max(sb, max(vp[0][i] & 0x7fffu, vp[1][i] & 0x7fffu));
-        sb = __reduce_max_sync(0xffffffffu, min(sb, 0x7bffu));
-        const bool grow = sb > smax;
-        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1]) || grow) {
-          int dk = 0;
-          if (grow) {
-            smax = sb;
-            const int e = int(__float_as_uint(__half2float(__ushort_as_half((unsigned short)sb))) >> 23) - 127;
-            dk = 14 - e - K;
-            K = 14 - e;
-          }
-          const float up = ex2(float(dk));
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const float mn = fmaxf(m[q], mx[q]);
-            const float al = m[q] == -INFINITY ? 0.f : ex2(m[q] - mn) * up;
-            m[q] = mn;
-            l[q] *= al;
-#pragma unroll
-            for (int i = 0; i < NG; ++i) pb[i][q] *= al;
-#pragma unroll
-            for (int i = 0; i < NW * 4; ++i) {
-              o[i][q] *= al;
-              o[i][q + 2] *= al;
-            }
-          }
-        }
-        float pr[4];
-        {
-          const float mk0 = m[0] == -INFINITY ? 0.f : m[0] - float(K), mk1 = m[1] == -INFINITY ? 0.f : m[1] - float(K);
-          pr[0] = ex2(x[0] - mk0);
-          pr[1] = ex2(x[1] - mk1);
-          pr[2] = ex2(x[2] - mk0);
-          pr[3] = ex2(x[3] - mk1);
-        }
-        l[0] += pr[0] + pr[2];
-        l[1] += pr[1] + pr[3];
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          const float2 v0 = kv4_param(vp[0][gi]), v1 = kv4_param(vp[1][gi]);
-          const float b0 = fmaf(7.5f, v0.x, v0.y), b1 = fmaf(7.5f, v1.x, v1.y);
-          float ps[4] = {pr[0] * v0.x, pr[1] * v0.x, pr[2] * v1.x, pr[3] * v1.x};
-          float pm[4] = {pr[0] * b0, pr[1] * b0, pr[2] * b1, pr[3] * b1};
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!see[i]) ps[i] = pm[i] = 0.f;
-          }
+          for (int i = 0; i < 4; ++i)
+            if (!((see >> i) & 1)) ps[i] = pm[i] = 0.f;
           pb[gi][0] += pm[0] + pm[2];
           pb[gi][1] += pm[1] + pm[3];
-          const __half2 h0 = __floats2half2_rn(ps[0], ps[1]), h1 = __floats2half2_rn(ps[2], ps[3]);
-          const uint32_t bh0 = movm(h2u(h0)), bh1 = movm(h2u(h1));
-          uint32_t bl0 = 0, bl1 = 0;
-          if (SPLIT) {
-            const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-            bl0 = movm(h2u(__floats2half2_rn(ps[0] - f0.x, ps[1] - f0.y)));
-            bl1 = movm(h2u(__floats2half2_rn(ps[2] - f1.x, ps[3] - f1.y)));
-          }
+        } else {
+          pb[gi][0] = fmaf(pr[2], v1.y, fmaf(pr[0], v0.y, pb[gi][0]));
+          pb[gi][1] = fmaf(pr[3], v1.y, fmaf(pr[1], v0.y, pb[gi][1]));
+        }
+        const __half2 h0 = __floats2half2_rn(ps[0], ps[1]), h1 = __floats2half2_rn(ps[2], ps[3]);
+        const uint32_t bh0 = movm(h2u(h0)), bh1 = movm(h2u(h1));
+        uint32_t bl0 = 0, bl1 = 0;
+        if (SPLIT) {
+          const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+          bl0 = movm(h2u(__floats2half2_rn(ps[0] - f0.x, ps[1] - f0.y)));
+          bl1 = movm(h2u(__floats2half2_rn(ps[2] - f1.x, ps[3] - f1.y)));
+        }
 #pragma unroll
-          for (int w = 0; w < GROUP / 64; ++w) {
-            const int wi = gi * (GROUP / 64) + w;
+        for (int w = 0; w < GROUP / 64; ++w) {
+          const int wi = gi * (GROUP / 64) + w;
 #pragma unroll
-            for (int pt = 0; pt < 2; ++pt) {
-              const uint32_t sel = pt ? 0x7632u : 0x5410u;
-              const uint32_t ab = prmt(vw[0][wi], vw[1][wi], sel), cd = prmt(vw[2][wi], vw[3][wi], sel);
+          for (int pt = 0; pt < 2; ++pt) {
+            const uint32_t sel = pt ? 0x7632u : 0x5410u;
+            const uint32_t ab = prmt(vw[0][wi], vw[1][wi], sel), cd = prmt(vw[2][wi], vw[3][wi], sel);
 #pragma unroll
-              for (int st2 = 0; st2 < 2; ++st2) {
-                uint32_t a0, a1, a2, a3;
-                unpack2(st2 ? ab >> 7 : ab << 1, a0, a1);
-                unpack2(st2 ? cd >> 7 : cd << 1, a2, a3);
-                float(&d)[4] = o[wi * 4 + pt * 2 + st2];
-                mma16816(d, a0, a1, a2, a3, bh0, bh1);
-                if (SPLIT) mma16816(d, a0, a1, a2, a3, bl0, bl1);
+            for (int st2 = 0; st2 < 2; ++st2) {
+              uint32_t a0, a1, a2, a3;
+              if (SPLIT) {
+                unpack_centred(st2 ? ab >> 7 : ab << 1, a0, a1);
+                unpack_centred(st2 ? cd >> 7 : cd << 1, a2, a3);
+              } else {
+                unpack_plain(st2 ? ab >> 8 : ab, a0, a1);
+                unpack_plain(st2 ? cd >> 8 : cd, a2, a3);
               }
+              float(&d)[4] = o[wi * 4 + pt * 2 + st2];
+              mma16816(d, a0, a1, a2, a3, bh0, bh1);
+              if (SPLIT) mma16816(d, a0, a1, a2, a3, bl0, bl1);
             }
           }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[s]);
+      issue(u + S * AT_WARPS, pg, s);
+      pg = page_of(u + (S + 1) * AT_WARPS);
+      s = s + 1 == S ? 0 : s + 1;
     }
+    cp_async_wait_all();
+    __syncwarp();
 
-    // ---- the item's share is done: combine the warps ----
+    // ---- the item's share is done: combine the warps. A warp leaves its
+    // outputs in its own ring: [word][column parity][k][lane], the k-th of the
+    // 8 channels of a 64-channel block that the lane holds for a column ----
 #pragma unroll
     for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
@@ -547,53 +562,46 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         sh.m[warp][2 * c + q] = m[q];
-        sh.l[warp][2 * c + q] = l[q] * ex2(float(-K));
+        sh.l[warp][2 * c + q] = l[q];
       }
     }
-    bar_consumers();
-    float fw[2];
+    if (lane == 0) sh.f[warp] = ex2(float(-K));
+    float* red = reinterpret_cast<float*>(ring);
+    // codes as they stand carry 2^-24, and 16 where the nibble is odd
+    constexpr float E0 = SPLIT ? 1.f : 0x1p24f, E1 = SPLIT ? 1.f : 0x1p20f;
+    if (u0 < u1)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      float M = -INFINITY;
+      for (int wi = 0; wi < NW; ++wi)
 #pragma unroll
-      for (int w = 0; w < AT_WARPS; ++w) M = fmaxf(M, sh.m[w][2 * c + q]);
-      fw[q] = m[q] == -INFINITY ? 0.f : ex2(m[q] - M) * ex2(float(-K));
-    }
-    // [word][column parity][k][lane]: k-th of 8 channels that a lane holds of a 64-channel block for a column
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-    for (int wi = 0; wi < NW; ++wi)
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          sh.red[warp][((wi * 2 + q) * 8 + k) * 32 + lane] =
-              m[q] == -INFINITY ? 0.f : (o[wi * 4 + k / 2][q + 2 * (k & 1)] + pb[wi / (GROUP / 64)][q]) * fw[q];
-    bar_consumers();
-    const int e = threadIdx.x >> 6, q = (threadIdx.x >> 5) & 1;  // 64-channel block, column parity
+          for (int k = 0; k < 8; ++k)
+            red[((wi * 2 + q) * 8 + k) * 32 + lane] = fmaf(o[wi * 4 + k / 2][q + 2 * (k & 1)], k & 1 ? E1 : E0, pb[wi / (GROUP / 64)][q]);
+    __syncthreads();
+    // four outputs a thread
+    const int e = threadIdx.x >> 7, q = (threadIdx.x >> 6) & 1, hf = (threadIdx.x >> 5) & 1;
     if (e < NW) {
       const int col = 2 * c + q;
-      float v[8], M = -INFINITY, L = 0.f;
+      float v[4] = {0.f, 0.f, 0.f, 0.f}, M = -INFINITY, L = 0.f;
 #pragma unroll
       for (int w = 0; w < AT_WARPS; ++w) M = fmaxf(M, sh.m[w][col]);
 #pragma unroll
       for (int w = 0; w < AT_WARPS; ++w) {
         const float mw = sh.m[w][col];
-        if (mw != -INFINITY) L += sh.l[w][col] * ex2(mw - M);
-      }
+        if (mw == -INFINITY) continue;  // nothing seen by this warp
+        const float fw = ex2(mw - M) * sh.f[w];
+        L = fmaf(sh.l[w][col], fw, L);
+        const float* rw = reinterpret_cast<const float*>(sh.ring[w]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        v[k] = 0.f;
-#pragma unroll
-        for (int w = 0; w < AT_WARPS; ++w) v[k] += sh.red[w][((e * 2 + q) * 8 + k) * 32 + lane];
+        for (int k = 0; k < 4; ++k) v[k] = fmaf(rw[((e * 2 + q) * 8 + hf * 4 + k) * 32 + lane], fw, v[k]);
       }
-      const int ch = e * 64 + r * 8;
+      const int ch = e * 64 + r * 8 + hf * 4;
       if (tb == 0 && t1 == p.tiles) {
         const int ci = cb * AT_COLS + col, tok = ci / a.rep, hq = h * a.rep + ci % a.rep;
         if (tok < p.n) {
           const float inv = M == -INFINITY ? 0.f : 1.f / L;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] *= inv;
-          write_out(a, p.row0 + tok, hq, ch, v);
+          for (int k = 0; k < 4; ++k) write_out(a, p.row0 + tok, hq, ch + k, v[k] * inv);
           if (ch == 0) attn_lse(a)[int64_t(p.row0 + tok) * a.heads + hq] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * LN2;
         }
       } else {
@@ -603,11 +611,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
           part[col] = M;
           part[AT_COLS + col] = L;
         }
-        float4* d = reinterpret_cast<float4*>(part + 2 * AT_COLS + col * HD + ch);
-        d[0] = make_float4(v[0], v[1], v[2], v[3]);
-        d[1] = make_float4(v[4], v[5], v[6], v[7]);
+        *reinterpret_cast<float4*>(part + 2 * AT_COLS + col * HD + ch) = make_float4(v[0], v[1], v[2], v[3]);
       }
     }
+    __syncthreads();  // the rings are free again
   }
 }
 
@@ -661,10 +668,8 @@ __global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
   }
   v = M == -INFINITY ? 0.f : v / L;
   const int64_t row = p.row0 + tok;
-  const int ch = threadIdx.x;
-  if (a.gate.p) v *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch));
-  kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, v);
-  if (ch == 0) attn_lse(a)[row * a.heads + hq] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * LN2;
+  write_out(a, row, hq, threadIdx.x, v);
+  if (threadIdx.x == 0) attn_lse(a)[row * a.heads + hq] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * LN2;
 }
 
 // ------------------------------------------------------- accumulated weight --
@@ -674,7 +679,7 @@ __global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
 // and would need space of rows x slots). A CTA owns 128 slots of a kv head and
 // walks all the sequence's columns, so every sum has one order.
 template <int HD, int GROUP, bool SPLIT>
-__global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs a) {
   constexpr int NG = HD / GROUP, NW = HD / 64;
   __shared__ __align__(16) QStage<HD, SPLIT> sq[2];
   __shared__ float slse[2][AT_COLS];
@@ -751,7 +756,7 @@ void run(const Kv4AttnArgs& a, cudaStream_t st) {
   launch(k_kv4_attn<HD, GROUP, SPLIT>, dim3(AT_GRID), dim3(AT_THREADS), sizeof(AttnShared<HD, GROUP, SPLIT>), st, false, a);
   launch(k_kv4_attn_join<HD>, dim3(AT_GRID, AT_COLS), dim3(HD), 0, st, true, a);
   if (a.weights && a.b.max_len > 0)
-    launch(k_kv4_weights<HD, GROUP, SPLIT>, dim3((a.b.max_len + AT_TILE - 1) / AT_TILE, a.g.kvh, a.b.nseq), dim3(AT_WARPS * 32), 0, st,
+    launch(k_kv4_weights<HD, GROUP, SPLIT>, dim3((a.b.max_len + AT_TILE - 1) / AT_TILE, a.g.kvh, a.b.nseq), dim3(WT_WARPS * 32), 0, st,
            false, a);
 }
 
