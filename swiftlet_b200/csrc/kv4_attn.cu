@@ -35,10 +35,11 @@ namespace swl {
 
 namespace {
 
-constexpr int AT_WARPS = 16;                // four per scheduler: the chains of a 16-slot unit need them to overlap
+constexpr int AT_WARPS = 12;                // three per scheduler at 168 registers
 constexpr int AT_THREADS = AT_WARPS * 32;
 constexpr int AT_UNIT = 16;                 // slots a warp takes at a time: the MMA's M (keys) and K (values)
 constexpr int AT_TILE = 128;                // slots of a tile, the grain in which work is shared out
+constexpr int AT_HEAD = 2;                  // what an item costs beside its tiles, in tiles
 constexpr int AT_COLS = 8;                  // query columns (token, head) of an item: the MMA's N
 constexpr int AT_GRID = 148;                // one CTA per SM
 constexpr int WT_WARPS = 8;                 // warps of the weight kernel: one tile
@@ -99,20 +100,22 @@ __device__ __forceinline__ void ldv(const uint8_t* p, uint32_t (&w)[N]) {
 // ------------------------------------------------------------------ work --
 // The work is the list of all (sequence, column block, kv head) items, each of
 // ceil(len / 128) tiles (one at least); a CTA takes an equal, contiguous share
-// of all tiles, so ragged batches and single long sequences spread alike.
+// of all tiles, so ragged batches and single long sequences spread alike. An
+// item counts AT_HEAD tiles more, in front of its own, for its beginning and
+// end (queries, first copies, combination of the warps).
 // Every warp finds its place from the lengths in device memory: nothing of the
 // split is known to the host.
 struct Place {
   int seq, item;   // item within the sequence: column block * kvh + kv head
-  int tile;        // first tile of this share within the item
-  int row0, n, len, tiles, items;
+  int tile;        // first tile of this share within the item, AT_HEAD tiles of overhead in front counted
+  int row0, n, len, tiles, items;  // tiles: with AT_HEAD
 };
 
 __device__ __forceinline__ void load_seq(const Kv4AttnArgs& a, int seq, Place& p) {
   p.seq = seq;
   p.n = kv4_new(a.b, seq, p.row0);
   p.len = kv4_len(a.b, seq);
-  p.tiles = max(1, (p.len + AT_TILE - 1) / AT_TILE);
+  p.tiles = AT_HEAD + max(1, (p.len + AT_TILE - 1) / AT_TILE);
   p.items = (int)(((int64_t)p.n * a.rep + AT_COLS - 1) / AT_COLS) * a.g.kvh;
 }
 
@@ -287,7 +290,7 @@ template <int HD, int GROUP, bool SPLIT>
 struct AttnShared {
   static constexpr int CODES = AT_UNIT * HD / 2, PARAMS = AT_UNIT * 4 * (HD / GROUP);  // bytes of a unit's keys (values)
   static constexpr int UNIT_BYTES = 2 * (CODES + PARAMS);
-  static constexpr int STAGES = HD == 256 ? 3 : HD == 128 ? 6 : 8;  // units in flight a warp: about 14 KB
+  static constexpr int STAGES = HD == 256 ? 4 : 8;                  // units in flight a warp (18 KB at 256 channels)
   static constexpr int SLICE = STAGES * UNIT_BYTES;                 // one warp's ring, its outputs at the end of an item
   static_assert(SLICE >= AT_COLS * HD * 4, "a warp's outputs fit its ring");
   alignas(128) uint8_t ring[AT_WARPS][SLICE];
@@ -332,8 +335,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
 
   for (int64_t f = r0; f < r1; next_item(a, p)) {
     const int h = p.item % g.kvh, cb = p.item / g.kvh;
-    const int tb = p.tile, t1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
-    f += t1 - tb;
+    const int v1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
+    // real tiles tb .. t1 - 1; the item's first part of several goes to slot 1, a later one (the share's first) to slot 0
+    const int tb = max(0, p.tile - AT_HEAD), t1 = v1 - AT_HEAD, slot = p.tile == 0 ? 1 : 0;
+    f += v1 - p.tile;
+    if (t1 <= 0) continue;  // only overhead of the next share's item
     // units u0, u0 + 16, ... < u1 are this warp's
     const int u0 = tb * (AT_TILE / AT_UNIT) + warp, u1 = min(t1 * (AT_TILE / AT_UNIT), (p.len + AT_UNIT - 1) / AT_UNIT);
     const int* tab = g.table + p.seq * g.tstride;
@@ -386,7 +392,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
     const int free_to = __reduce_min_sync(0xffffffffu, min(lim[0], lim[1]));  // every column sees slots up to here
     float o[NW * 4][4];
     float pb[NG][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int K = 0;             // p carries a factor 2^K (K = 14 - exponent of the largest value scale)
+    int K = 0;             // p carries a factor 2^K (K = 6 - exponent of the largest value scale)
     unsigned smax = 0u;    // that scale's bits
 #pragma unroll
     for (int i = 0; i < NW * 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -453,19 +459,20 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
 #pragma unroll
       for (int i = 0; i < NG; ++i) sb = max(sb, max(vp[0][i] & 0x7fffu, vp[1][i] & 0x7fffu));
       sb = __reduce_max_sync(0xffffffffu, min(sb, 0x7bffu));
-      const bool grow = sb > smax;
-      if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1]) || grow) {
+      // The reference point moves only when the maximum has outgrown it by
+      // 2^8 or the scales theirs: p then stays below 2^8, p s below 2^15.
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f) || sb > smax) {
         int dk = 0;
-        if (grow) {
-          smax = sb;
-          const int e = int(__float_as_uint(__half2float(__ushort_as_half((unsigned short)sb))) >> 23) - 127;
-          dk = 14 - e - K;
-          K = 14 - e;
+        if (sb > smax) {
+          smax = sb | 0x3ffu;  // the whole binade: K goes by the exponent (s < 2^(e + 1))
+          const int e = int(sb >> 10) - 15;
+          dk = 6 - e - K;
+          K = 6 - e;
         }
         const float up = ex2(float(dk));
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const float mn = fmaxf(m[q], mx[q]);
+          const float mn = mx[q] > m[q] + 8.f ? mx[q] : m[q];
           const float al = m[q] == -INFINITY ? 0.f : ex2(m[q] - mn) * up;
           m[q] = mn;
           l[q] *= al;
@@ -578,9 +585,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
           for (int k = 0; k < 8; ++k)
             red[((wi * 2 + q) * 8 + k) * 32 + lane] = fmaf(o[wi * 4 + k / 2][q + 2 * (k & 1)], k & 1 ? E1 : E0, pb[wi / (GROUP / 64)][q]);
     __syncthreads();
-    // four outputs a thread
-    const int e = threadIdx.x >> 7, q = (threadIdx.x >> 6) & 1, hf = (threadIdx.x >> 5) & 1;
-    if (e < NW) {
+    // four outputs of a column at a time
+    for (int i = warp; i < NW * 4; i += AT_WARPS) {
+      const int e = i >> 2, q = (i >> 1) & 1, hf = i & 1;
       const int col = 2 * c + q;
       float v[4] = {0.f, 0.f, 0.f, 0.f}, M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -596,7 +603,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
         for (int k = 0; k < 4; ++k) v[k] = fmaf(rw[((e * 2 + q) * 8 + hf * 4 + k) * 32 + lane], fw, v[k]);
       }
       const int ch = e * 64 + r * 8 + hf * 4;
-      if (tb == 0 && t1 == p.tiles) {
+      if (tb == 0 && v1 == p.tiles) {
         const int ci = cb * AT_COLS + col, tok = ci / a.rep, hq = h * a.rep + ci % a.rep;
         if (tok < p.n) {
           const float inv = M == -INFINITY ? 0.f : 1.f / L;
@@ -605,8 +612,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
           if (ch == 0) attn_lse(a)[int64_t(p.row0 + tok) * a.heads + hq] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * LN2;
         }
       } else {
-        // an item that goes on in another CTA: slot 0 if it began before this CTA, slot 1 if it begins here
-        float* part = attn_parts(a) + (int64_t(blockIdx.x) * 2 + (tb == 0 ? 1 : 0)) * part_floats(HD);
+        float* part = attn_parts(a) + (int64_t(blockIdx.x) * 2 + slot) * part_floats(HD);
         if (ch == 0) {
           part[col] = M;
           part[AT_COLS + col] = L;
@@ -636,14 +642,21 @@ __global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
   __shared__ float red[32];
   const float* parts = attn_parts(a);
   auto part = [&](int i) { return parts + (int64_t(i) * 2 + (i == x ? 1 : 0)) * part_floats(HD); };
-  // shares x .. last hold parts of the item (those without tiles none)
+  // shares x .. last hold parts of the item, those with no tile of it none
   int last = x;
   while (last + 1 < nc && total * (last + 1) / nc < end) ++last;
   const int np = last - x + 1;
+  auto has = [&](int i) {
+    const int64_t lo = max(begin + AT_HEAD, total * (x + i) / nc), hi = min(end, total * (x + i + 1) / nc);
+    return lo < hi;
+  };
+  // all its tiles in one share: written there
+  int one = x;
+  while (total * (one + 1) / nc <= begin + AT_HEAD) ++one;
+  if (one == last) return;
   float M = -INFINITY;
   for (int i = threadIdx.x; i < np; i += HD) {
-    const bool has = total * (x + i + 1) / nc > total * (x + i) / nc;
-    const float mi = has ? __ldcg(part(x + i) + col) : -INFINITY;
+    const float mi = has(i) ? __ldcg(part(x + i) + col) : -INFINITY;
     wt[i] = mi;
     M = fmaxf(M, mi);
   }
