@@ -82,6 +82,8 @@ void launch_kv4_read(const Kv4IoArgs& a, int dt, cudaStream_t st);
 void launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t st);
 int64_t kv4_attention_work(const Kv4Geo& g, const Kv4Batch& b, int heads);
 void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t st);
+int64_t kv4_prompt_work(const Kv4Geo& g, const Kv4Batch& b, int heads);
+void launch_kv4_prompt(const Kv4AttnArgs& a, cudaStream_t st);
 
 #ifdef __CUDACC__
 __device__ __forceinline__ int kv4_swz(int hd, int t) {
@@ -133,6 +135,19 @@ __device__ __forceinline__ void kv4_st(uint8_t* p, int dt, int64_t i, float v) {
   if (dt == DT_F32) reinterpret_cast<float*>(p)[i] = v;
   else if (dt == DT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+// N consecutive words of shared or global memory as one vector load.
+template <int N>
+__device__ __forceinline__ void kv4_ldv(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
 }
 // Scale and bias of a group from its word.
 __device__ __forceinline__ float2 kv4_param(uint32_t w) {

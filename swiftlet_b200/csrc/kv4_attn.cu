@@ -83,20 +83,6 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
   return r;
 }
-// N consecutive words of shared or global memory as one vector load.
-template <int N>
-__device__ __forceinline__ void ldv(const uint8_t* p, uint32_t (&w)[N]) {
-  if constexpr (N == 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
-}
-
 // ------------------------------------------------------------------ work --
 // The work is the list of all (sequence, column block, kv head) items, each of
 // ceil(len / 128) tiles (one at least); a CTA takes an equal, contiguous share
@@ -411,23 +397,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
       float x[4];
       {
         uint32_t kw[2][2][NW], kp[2][NG];
-        ldv(st + koff0, kw[0][0]);
-        ldv(st + koff0 + 8 * (HD / 2), kw[0][1]);
-        ldv(st + koff1, kw[1][0]);
-        ldv(st + koff1 + 8 * (HD / 2), kw[1][1]);
-        ldv(st + Sh::CODES + r * NG * 4, kp[0]);
-        ldv(st + Sh::CODES + (r + 8) * NG * 4, kp[1]);
+        kv4_ldv(st + koff0, kw[0][0]);
+        kv4_ldv(st + koff0 + 8 * (HD / 2), kw[0][1]);
+        kv4_ldv(st + koff1, kw[1][0]);
+        kv4_ldv(st + koff1 + 8 * (HD / 2), kw[1][1]);
+        kv4_ldv(st + Sh::CODES + r * NG * 4, kp[0]);
+        kv4_ldv(st + Sh::CODES + (r + 8) * NG * 4, kp[1]);
         scores<HD, GROUP, SPLIT>(kw, kp, qsum, [&](int k, uint32_t (&b)[SPLIT ? 4 : 2]) {
-          ldv(reinterpret_cast<const uint8_t*>(sh.q.frag + (k * 32 + lane) * QStage<HD, SPLIT>::W), b);
+          kv4_ldv(reinterpret_cast<const uint8_t*>(sh.q.frag + (k * 32 + lane) * QStage<HD, SPLIT>::W), b);
         }, x);
       }
       uint32_t vp[2][NG], vw[4][NW];
-      ldv(sv + Sh::CODES + r * NG * 4, vp[0]);
-      ldv(sv + Sh::CODES + (r + 8) * NG * 4, vp[1]);
-      ldv(sv + voff0, vw[0]);
-      ldv(sv + voff1, vw[1]);
-      ldv(sv + voff0 + 8 * (HD / 2), vw[2]);
-      ldv(sv + voff1 + 8 * (HD / 2), vw[3]);
+      kv4_ldv(sv + Sh::CODES + r * NG * 4, vp[0]);
+      kv4_ldv(sv + Sh::CODES + (r + 8) * NG * 4, vp[1]);
+      kv4_ldv(sv + voff0, vw[0]);
+      kv4_ldv(sv + voff1, vw[1]);
+      kv4_ldv(sv + voff0 + 8 * (HD / 2), vw[2]);
+      kv4_ldv(sv + voff1 + 8 * (HD / 2), vw[3]);
       unsigned see = 15u;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] *= mul[i & 1];
@@ -714,9 +700,9 @@ __global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs
 #pragma unroll
     for (int w = 0; w < NG; ++w) kp[i][w] = 0u;
     if (blk) {
-      ldv(blk + t * (HD / 2) + (c ^ kv4_swz(HD, t)) * (HD / 16), kw[0][i]);
-      ldv(blk + t * (HD / 2) + ((c + 4) ^ kv4_swz(HD, t)) * (HD / 16), kw[1][i]);
-      ldv(blk + g.seg * (HD / 2) + t * NG * 4, kp[i]);
+      kv4_ldv(blk + t * (HD / 2) + (c ^ kv4_swz(HD, t)) * (HD / 16), kw[0][i]);
+      kv4_ldv(blk + t * (HD / 2) + ((c + 4) ^ kv4_swz(HD, t)) * (HD / 16), kw[1][i]);
+      kv4_ldv(blk + g.seg * (HD / 2) + t * NG * 4, kp[i]);
     }
   }
   const float* lse = attn_lse(a);
@@ -742,7 +728,7 @@ __global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs
         for (int w = 0; w < GROUP / 64; ++w) qsum[k][i] += q.sum[2 * c + k][i * (GROUP / 64) + w];
       }
     scores<HD, GROUP, SPLIT>(kw, kp, qsum, [&](int k, uint32_t (&b)[SPLIT ? 4 : 2]) {
-      ldv(reinterpret_cast<const uint8_t*>(q.frag + (k * 32 + lane) * QStage<HD, SPLIT>::W), b);
+      kv4_ldv(reinterpret_cast<const uint8_t*>(q.frag + (k * 32 + lane) * QStage<HD, SPLIT>::W), b);
     }, x);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -764,10 +750,19 @@ __global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs
   }
 }
 
+// Query rows a kv head from which the tensor-core prompt kernel is used: a
+// tile there costs the same for 1 to 128 rows, here for every 8.
+constexpr int64_t AT_FEW = 16;
+bool few_rows(const Kv4Batch& b, int rep) { return int64_t(b.max_new) * rep <= AT_FEW; }
+
 template <int HD, int GROUP, bool SPLIT>
 void run(const Kv4AttnArgs& a, cudaStream_t st) {
-  launch(k_kv4_attn<HD, GROUP, SPLIT>, dim3(AT_GRID), dim3(AT_THREADS), sizeof(AttnShared<HD, GROUP, SPLIT>), st, false, a);
-  launch(k_kv4_attn_join<HD>, dim3(AT_GRID, AT_COLS), dim3(HD), 0, st, true, a);
+  if (few_rows(a.b, a.rep)) {
+    launch(k_kv4_attn<HD, GROUP, SPLIT>, dim3(AT_GRID), dim3(AT_THREADS), sizeof(AttnShared<HD, GROUP, SPLIT>), st, false, a);
+    launch(k_kv4_attn_join<HD>, dim3(AT_GRID, AT_COLS), dim3(HD), 0, st, true, a);
+  } else {
+    launch_kv4_prompt(a, st);
+  }
   if (a.weights && a.b.max_len > 0)
     launch(k_kv4_weights<HD, GROUP, SPLIT>, dim3((a.b.max_len + AT_TILE - 1) / AT_TILE, a.g.kvh, a.b.nseq), dim3(WT_WARPS * 32), 0, st,
            false, a);
@@ -782,6 +777,7 @@ void run_dt(const Kv4AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int64_t kv4_attention_work(const Kv4Geo& g, const Kv4Batch& b, int heads) {
+  if (!few_rows(b, heads / g.kvh)) return kv4_prompt_work(g, b, heads);
   return (int64_t(b.total) * heads * 4 + 15) / 16 * 16 + int64_t(AT_GRID) * 2 * part_floats(g.hd) * 4;
 }
 

@@ -1,0 +1,774 @@
+// Attention over the 4-bit KV cache for many query rows a sequence (prompts,
+// chunks of them, long turns) on the 5th-generation tensor cores.
+//
+// An item is 128 query rows (token-major, the heads of one kv head adjacent)
+// of one sequence and kv head; the context is walked in tiles of BN slots:
+//   S = Q K^T (tcgen05.mma, M 128, N BN, K head_dim; accumulator in TMEM),
+//   online softmax by one thread a row, P to TMEM as f16,
+//   O += P V (M 128, N head_dim, K BN; A from TMEM, V as an N-major operand).
+// Keys and values are unpacked to f16 on their way into shared memory, scaled
+// by a power of two so that the largest value of the sequence and head is
+// just below 2^14 (k_kv4_range reads the params for it). 16-bit inputs: one
+// product each, values rounded to 11 bits like the inputs themselves. f32
+// inputs: every operand as two f16 terms (22 bits) and three products each
+// (hi hi + lo hi + hi lo), f32 accumulators throughout.
+//
+// Warps: 0-3 softmax and output, 4-11 unpacking, 12 MMA issue and TMEM. S and
+// P are double-buffered, so Q K^T of the next tile runs during the softmax of
+// this one; the running maximum moves only when it has grown by 2^8, so O in
+// TMEM is rarely touched. Bound: the tensor cores (a tile of 64 slots at 256
+// channels is 1024 cycles of MMA for 16-bit inputs), next to the issue slots
+// of the unpacking (15 instructions per 8 values) and the softmax.
+//
+// The work is shared out like that of kv4_attn.cu: equal contiguous shares of
+// all tiles of all items over 148 CTAs, parts of an item that several CTAs
+// work on joined by a second kernel.
+#include <algorithm>
+
+#include "kcommon.cuh"
+#include "kv4.h"
+#include "launch.h"
+#include "tc.cuh"
+
+namespace swl {
+
+namespace {
+
+constexpr int PT_ROWS = 128;
+constexpr int PT_GRID = 148;
+constexpr int PT_SOFT = 128, PT_UNPACK = 256;           // threads of the softmax and unpack roles
+constexpr int PT_THREADS = PT_SOFT + PT_UNPACK + 32;
+constexpr int PT_HEAD = 4;                              // cost of an item beside its tiles, in tiles
+constexpr int RG_SPLIT = 16;                            // blocks a (sequence, head) of the range kernel
+constexpr float P_LOG2E = 1.4426950408889634f, P_LN2 = 0.6931471805599453f;
+
+template <int HD, bool SPLIT>
+struct PtShape {
+  static constexpr int BN = HD == 256 && SPLIT ? 32 : 64;  // slots of a tile (shared memory holds two terms of Q)
+  static constexpr int T = SPLIT ? 2 : 1;                  // f16 terms of an operand
+  static constexpr int ST = HD == 256 && SPLIT ? 1 : 2;    // buffers of unpacked keys, and of values
+  static constexpr int QB = PT_ROWS * HD * 2;              // bytes of one term of Q
+  static constexpr int KB = BN * HD * 2;                   // of one term of a tile's keys (values)
+  static constexpr int Q_OFF = 0, K_OFF = T * QB, V_OFF = K_OFF + ST * T * KB, M_OFF = V_OFF + ST * T * KB;
+  static constexpr int BAR_OFF = M_OFF + PT_ROWS * 8;      // after the rows' factors and limits
+  static constexpr int NBAR = 4 * ST + 2 + 2 + 2 + 1;      // k full / empty, v full / empty, s full, p full, o done, drain
+  static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 16 + 1024;  // 1024: base alignment
+  // TMEM columns
+  static constexpr int O_COL = 0, S_COL = HD, P_COL = HD + 2 * BN;
+  static_assert(P_COL + 2 * T * BN / 2 <= 512, "TMEM columns");
+};
+
+// D f32, A and B f16; N, transposed (N-major) B
+constexpr uint32_t pt_idesc(int n, bool bt) {
+  return (1u << 4) | (uint32_t(bt) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(PT_ROWS >> 4) << 24);
+}
+// N-major operand, 128-byte swizzle: rows of 64 elements (one K index each),
+// eight to an atom of 1024 bytes (SBO, along K); the next 64 elements of N lie
+// lbo bytes on.
+__device__ __forceinline__ uint64_t pt_desc_n(uint32_t saddr, uint32_t lbo) {
+  return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(lbo >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc))
+      : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc))
+      : "memory");
+}
+__device__ __forceinline__ void pt_ld32(uint32_t t, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(t));
+}
+__device__ __forceinline__ void pt_st32(uint32_t t, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void pt_st16(uint32_t t, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]),
+      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void pt_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float pt_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pt_h2(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 pt_u2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// ------------------------------------------------------------------ work --
+struct PtPlace {
+  int seq, qt, h;              // item: query tile qt, kv head h
+  int tile, tiles;             // first tile of the share and tiles of the item, PT_HEAD counted in front
+  int row0, n, len, nq;        // the sequence: first row, new tokens, slots, query tiles
+};
+
+// Tiles of query tile qt: up to the last slot its last row sees.
+__device__ __forceinline__ int pt_tiles(int n, int len, int rep, int bn, int qt) {
+  const int last = int(min(int64_t(n) - 1, (int64_t(qt + 1) * PT_ROWS - 1) / rep));
+  const int seen = max(0, min(len, len - n + last + 1));
+  return PT_HEAD + max(1, (seen + bn - 1) / bn);
+}
+__device__ __forceinline__ void pt_seq(const Kv4AttnArgs& a, int seq, PtPlace& p) {
+  p.seq = seq;
+  p.n = kv4_new(a.b, seq, p.row0);
+  p.len = kv4_len(a.b, seq);
+  p.nq = int((int64_t(p.n) * a.rep + PT_ROWS - 1) / PT_ROWS);
+}
+__device__ __forceinline__ int64_t pt_total(const Kv4AttnArgs& a, int bn) {
+  int64_t sum = 0;
+  PtPlace p;
+  for (int s = 0; s < a.b.nseq; ++s) {
+    pt_seq(a, s, p);
+    for (int q = threadIdx.x & 31; q < p.nq; q += 32) sum += pt_tiles(p.n, p.len, a.rep, bn, q);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum * a.g.kvh;
+}
+// Place of tile number `flat` (0 <= flat < total).
+__device__ __forceinline__ PtPlace pt_find(const Kv4AttnArgs& a, int bn, int64_t flat) {
+  const int lane = threadIdx.x & 31;
+  int64_t base = 0;
+  PtPlace p = {};
+  for (int s = 0; s < a.b.nseq; ++s) {
+    pt_seq(a, s, p);
+    for (int q0 = 0; q0 < p.nq; q0 += 32) {
+      const int64_t cnt = q0 + lane < p.nq ? int64_t(pt_tiles(p.n, p.len, a.rep, bn, q0 + lane)) * a.g.kvh : 0;
+      int64_t incl = cnt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, base + incl > flat);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        const int64_t rem = flat - base - __shfl_sync(0xffffffffu, incl - cnt, src);
+        p.qt = q0 + src;
+        p.tiles = pt_tiles(p.n, p.len, a.rep, bn, p.qt);
+        p.h = int(rem / p.tiles);
+        p.tile = int(rem % p.tiles);
+        return p;
+      }
+      base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  return p;
+}
+__device__ __forceinline__ void pt_next(const Kv4AttnArgs& a, int bn, PtPlace& p) {
+  p.tile = 0;
+  if (++p.h < a.g.kvh) return;
+  p.h = 0;
+  if (++p.qt < p.nq) {
+    p.tiles = pt_tiles(p.n, p.len, a.rep, bn, p.qt);
+    return;
+  }
+  p.qt = 0;
+  for (int s = p.seq + 1; s < a.b.nseq; ++s) {
+    pt_seq(a, s, p);
+    if (p.nq) {
+      p.tiles = pt_tiles(p.n, p.len, a.rep, bn, 0);
+      return;
+    }
+  }
+}
+
+// Workspace: lse rows, ranges, parts.
+__host__ __device__ inline int64_t pt_lse_bytes(int64_t total, int heads) { return (total * heads * 4 + 15) / 16 * 16; }
+__host__ __device__ inline int64_t pt_range_bytes(int64_t nseq, int kvh) { return nseq * kvh * RG_SPLIT * 16; }
+__host__ __device__ constexpr int pt_part_floats(int hd) { return PT_ROWS * (hd + 2); }
+__device__ __forceinline__ float* pt_lse(const Kv4AttnArgs& a) { return a.lse ? a.lse : reinterpret_cast<float*>(a.work); }
+__device__ __forceinline__ int4* pt_ranges(const Kv4AttnArgs& a) { return reinterpret_cast<int4*>(a.work + pt_lse_bytes(a.b.total, a.heads)); }
+__device__ __forceinline__ float* pt_parts(const Kv4AttnArgs& a) {
+  return reinterpret_cast<float*>(a.work + pt_lse_bytes(a.b.total, a.heads) + pt_range_bytes(a.b.nseq, a.g.kvh));
+}
+
+// Largest |value| of the keys and of the values of each (sequence, kv head),
+// as f32 bits, and flags (bit 0: a value group is NaN, bit 1: a page outside the
+// pool), over one of RG_SPLIT shares of the slots a block.
+__global__ void __launch_bounds__(256) k_kv4_range(const Kv4AttnArgs a) {
+  pdl_launch();
+  const int seq = blockIdx.y / a.g.kvh, h = blockIdx.y % a.g.kvh;
+  int row0;
+  const int n = kv4_new(a.b, seq, row0), len = n ? kv4_len(a.b, seq) : 0;
+  unsigned mk = 0u, mv = 0u, nan = 0u;
+  for (int s = blockIdx.x * 256 + threadIdx.x; s < len; s += 256 * RG_SPLIT) {
+    const uint8_t* blk = kv4_block(a.g, a.g.table, a.g.tstride, seq, h, s, a.b.status);
+    if (!blk) {
+      nan |= 2u;
+      continue;
+    }
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + a.g.seg * (a.g.hd / 2)) + (s & (a.g.seg - 1)) * a.g.ng;
+    const uint32_t* vp = kp + a.g.blk / 8;
+    for (int i = 0; i < a.g.ng; ++i) {
+      const float2 k = kv4_param(kp[i]), v = kv4_param(vp[i]);
+      const float ka = fmaxf(fabsf(k.y), fabsf(fmaf(15.f, k.x, k.y))), va = fmaxf(fabsf(v.y), fabsf(fmaf(15.f, v.x, v.y)));
+      if (ka < INFINITY) mk = max(mk, __float_as_uint(ka));
+      if (va < INFINITY) mv = max(mv, __float_as_uint(va));
+      nan |= unsigned(!(va < INFINITY));
+    }
+  }
+  __shared__ unsigned red[3][8];
+  mk = __reduce_max_sync(0xffffffffu, mk);
+  mv = __reduce_max_sync(0xffffffffu, mv);
+  nan = __reduce_or_sync(0xffffffffu, nan);
+  if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = mk, red[1][threadIdx.x >> 5] = mv, red[2][threadIdx.x >> 5] = nan;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) mk = max(mk, red[0][w]), mv = max(mv, red[1][w]), nan |= red[2][w];
+    pt_ranges(a)[int64_t(blockIdx.y) * RG_SPLIT + blockIdx.x] = make_int4(int(mk), int(mv), int(nan), 0);
+  }
+}
+
+// Exponent that takes a largest |value| (f32 bits) to [2^13, 2^14).
+__device__ __forceinline__ int pt_exp(unsigned bits) { return bits ? max(-14, min(60, 13 - (int(bits >> 23) - 127))) : 0; }
+__device__ __forceinline__ float pt_pow2(int e) { return __int_as_float((127 + e) << 23); }
+
+// Eight codes of a word as f16 pairs (0 4)(1 5)(2 6)(3 7): value 2^x (s c + b)
+// rounded once, or to two terms. f16 inputs of the arithmetic: the scaled
+// params (rounded where 2^x takes them below f16's normal range, 2^-28 of the
+// largest value).
+template <bool SPLIT>
+__device__ __forceinline__ void pt_unpack(uint32_t w, float2 sb, uint4& hi, uint4& lo) {
+  uint32_t* H = &hi.x;
+  uint32_t* L = &lo.x;
+  const __half2 m0 = pt_u2(0xe400e400u);                          // -1024
+  const __half2 r = pt_u2(0x2c002c00u), m1 = pt_u2(0xd400d400u);  // 1 / 16, -64
+  __half2 c[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = i ? w >> 8 : w;
+    c[2 * i] = __hadd2(pt_u2((x & 0x000f000fu) | 0x64006400u), m0);
+    c[2 * i + 1] = __hfma2(pt_u2((x & 0x00f000f0u) | 0x64006400u), r, m1);
+  }
+  if (!SPLIT) {
+    const __half2 s = __float2half2_rn(sb.x), b = __float2half2_rn(sb.y);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) H[i] = pt_h2(__hfma2(c[i], s, b));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 v = __half22float2(c[i]);
+      v.x = fmaf(sb.x, v.x, sb.y);
+      v.y = fmaf(sb.x, v.y, sb.y);
+      const __half2 h = __floats2half2_rn(v.x, v.y);
+      const float2 f = __half22float2(h);
+      H[i] = pt_h2(h);
+      L[i] = pt_h2(__floats2half2_rn(v.x - f.x, v.y - f.y));
+    }
+  }
+}
+
+template <int HD, int GROUP, bool SPLIT>
+__global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs a) {
+  using Sh = PtShape<HD, SPLIT>;
+  constexpr int BN = Sh::BN, T = Sh::T, ST = Sh::ST, NG = HD / GROUP, NW = HD / 64;
+  extern __shared__ __align__(1024) uint8_t pt_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
+  float* row_mul = reinterpret_cast<float*>(sm + Sh::M_OFF);
+  int* row_lim = reinterpret_cast<int*>(row_mul + PT_ROWS);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(sm + Sh::BAR_OFF);
+  uint64_t *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *s_full = v_empty + ST, *p_full = s_full + 2,
+           *o_done = p_full + 2, *drain = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Kv4Geo& g = a.g;
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&k_full[s], PT_UNPACK);
+      mbar_init(&v_full[s], PT_UNPACK);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], PT_SOFT);
+      mbar_init(&o_done[s], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tg_fence_before();
+  __syncthreads();
+  tg_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch();
+  const int64_t total = pt_total(a, BN);
+  const int64_t r0 = total * blockIdx.x / gridDim.x, r1 = total * (blockIdx.x + 1) / gridDim.x;
+  pdl_wait();  // the ranges
+  auto fail = [&]() {
+    if (a.b.status) atomicOr(a.b.status, 1);
+    *abort_flag = 1;
+  };
+  PtPlace p = {};
+  if (r0 < r1) p = pt_find(a, BN, r0);
+  int j = 0;  // tiles done by this CTA, the pipelines' counter
+  for (int64_t f = r0; f < r1; pt_next(a, BN, p)) {
+    const int v1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
+    const int tb = max(0, p.tile - PT_HEAD), nt = v1 - PT_HEAD - tb, slot_of_part = p.tile == 0 ? 1 : 0;
+    f += v1 - p.tile;
+    if (v1 <= PT_HEAD || nt <= 0) continue;
+    // ranges of the item
+    unsigned mk = 0u, mv = 0u, vnan = 0u;
+    if (lane < RG_SPLIT) {
+      const int4 q = __ldcg(pt_ranges(a) + (int64_t(p.seq) * g.kvh + p.h) * RG_SPLIT + lane);
+      mk = unsigned(q.x), mv = unsigned(q.y), vnan = unsigned(q.z);
+    }
+    mk = __reduce_max_sync(0xffffffffu, mk);
+    mv = __reduce_max_sync(0xffffffffu, mv);
+    vnan = __reduce_or_sync(0xffffffffu, vnan);
+    const int kx = pt_exp(mk), vx = pt_exp(mv);
+    const bool lost = (vnan & 2u) != 0u;
+    vnan &= 1u;
+
+    if (warp >= 4 && warp < 12) {
+      // ------------------------------------------------------ unpacking ----
+      // queries: a warp a row, eight channels a lane
+      for (int r = warp - 4; r < PT_ROWS; r += 8) {
+        const int64_t ci = int64_t(p.qt) * PT_ROWS + r;
+        const int t = int(ci / a.rep), hq = p.h * a.rep + int(ci % a.rep);
+        const bool on = t < p.n, act = lane < HD / 8;
+        float x[8], am = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = on && act ? kv4_ld(a.q.p, a.dt, (p.row0 + t) * a.q.ts + hq * a.q.hs + lane * 8 + e) : 0.f;
+          am = fmaxf(am, fabsf(x[e]));
+        }
+        am = warp_max(am);
+        int ex = am > 0.f && am < INFINITY ? 12 - (int(__float_as_uint(am) >> 23) - 127) : 0;
+        ex = max(-60, min(60, ex));
+        const float up = pt_pow2(ex);
+        if (act) {
+          uint4 hi, lo;
+          uint32_t *H = &hi.x, *L = &lo.x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // the order the codes come unpacked in
+            const float v0 = x[i] * up, v1f = x[i + 4] * up;
+            const __half2 hh = __floats2half2_rn(v0, v1f);
+            H[i] = pt_h2(hh);
+            if (SPLIT) {
+              const float2 ff = __half22float2(hh);
+              L[i] = pt_h2(__floats2half2_rn(v0 - ff.x, v1f - ff.y));
+            }
+          }
+          uint8_t* d = sm + Sh::Q_OFF + (lane >> 3) * (PT_ROWS * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(d) = hi;
+          if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::QB) = lo;
+        }
+        if (lane == 0) {
+          row_mul[r] = a.scale * P_LOG2E * pt_pow2(-ex) * pt_pow2(-kx);
+          row_lim[r] = on ? p.len - p.n + t : p.len - 1;
+        }
+      }
+      fence_proxy_async();
+    }
+    __syncthreads();  // queries staged (and TMEM and buffers of the last item free)
+
+    if (warp < 4) {
+      // -------------------------------------------------------- softmax ----
+      const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
+      const float mul = row_mul[tid];
+      const int lim = row_lim[tid];
+      const int lim_lo = __reduce_min_sync(0xffffffffu, lim);
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int i = 0; i < nt && ok; ++i) {
+        const int jj = j + i, b = jj & 1;
+        const unsigned ph = (jj >> 1) & 1;
+        if (!__all_sync(0xffffffffu, tg_wait(&s_full[b], ph) && !*abort_flag)) { fail(); break; }
+        tg_fence_after();
+        uint32_t s[BN];
+#pragma unroll
+        for (int q = 0; q < BN / 32; ++q) pt_ld32(lanes + Sh::S_COL + b * BN + q * 32, *reinterpret_cast<uint32_t(*)[32]>(s + q * 32));
+        tg_ld_wait();
+        const int s0 = (tb + i) * BN;
+#pragma unroll
+        for (int e = 0; e < BN; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * mul);
+        if (s0 + BN - 1 > lim_lo) {
+#pragma unroll
+          for (int e = 0; e < BN; ++e)
+            if (s0 + e > lim) s[e] = 0xff800000u;
+        }
+        if (lost) {  // slots of pages outside the pool
+#pragma unroll
+          for (int e = 0; e < BN; ++e)
+            if ((e & 15) == 0 && s0 + e < p.len && !kv4_block(g, g.table, g.tstride, p.seq, p.h, s0 + e, nullptr)) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) s[e + k] = 0xff800000u;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < BN; ++e) mx = fmaxf(mx, __uint_as_float(s[e]));
+        const bool grow = mx > m + 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float mn = grow ? mx : m;
+          const float al = m == -INFINITY ? (grow ? 0.f : 1.f) : pt_ex2(m - mn);
+          m = mn;
+          l *= al;
+          if (i > 0) {
+            // every earlier product has landed before O is scaled
+            if (!__all_sync(0xffffffffu, tg_wait(&o_done[b ^ 1], ((jj - 1) >> 1) & 1))) {
+              fail();
+              ok = false;
+            }
+            tg_fence_after();
+#pragma unroll 1
+            for (int q = 0; q < HD / 32; ++q) {
+              uint32_t o[32];
+              pt_ld32(lanes + Sh::O_COL + q * 32, o);
+              tg_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+              pt_st32(lanes + Sh::O_COL + q * 32, o);
+            }
+            pt_st_wait();
+          }
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+        // the product that read this P buffer two tiles ago
+        if (i >= 2 && !__all_sync(0xffffffffu, tg_wait(&o_done[b], ((jj - 2) >> 1) & 1))) { fail(); break; }
+        tg_fence_after();
+        const uint32_t pc = lanes + Sh::P_COL + b * (T * BN / 2);
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int q = 0; q < BN / 32; ++q) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = pt_ex2(__uint_as_float(s[q * 32 + 2 * e]) - mm), p1 = pt_ex2(__uint_as_float(s[q * 32 + 2 * e + 1]) - mm);
+            l0 += p0;
+            l1 += p1;
+            const __half2 hh = __floats2half2_rn(p0, p1);
+            hi[e] = pt_h2(hh);
+            if (SPLIT) {
+              const float2 ff = __half22float2(hh);
+              lo[e] = pt_h2(__floats2half2_rn(p0 - ff.x, p1 - ff.y));
+            }
+          }
+          pt_st16(pc + q * 16, hi);
+          if (SPLIT) pt_st16(pc + BN / 2 + q * 16, lo);
+        }
+        l += l0 + l1;
+        pt_st_wait();
+        tg_fence_before();
+        mbar_arrive(&p_full[b]);
+      }
+      // ---- output: the last product has landed ----
+      const int64_t ci = int64_t(p.qt) * PT_ROWS + tid;
+      const int tok = int(ci / a.rep), hq = p.h * a.rep + int(ci % a.rep);
+      const int64_t row = p.row0 + tok;
+      const bool whole = tb == 0 && v1 == p.tiles;
+      const int last = j + nt - 1;
+      const bool done = !*abort_flag && tg_wait(&o_done[last & 1], (last >> 1) & 1);
+      if (!done) fail();
+      tg_fence_after();
+      // value groups that are NaN went in as zeros: a row that sees one has NaN there
+      unsigned bad = 0u;
+      if (vnan)
+        for (int s = tb * BN; s < min(min((tb + nt) * BN, p.len), lim + 1); ++s) {
+          const uint8_t* blk = kv4_block(g, g.table, g.tstride, p.seq, p.h, s, nullptr);
+          if (!blk) continue;
+          const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + g.blk / 2 + g.seg * (HD / 2)) + (s & (g.seg - 1)) * NG;
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            const float2 v = kv4_param(vp[i]);
+            if (!(fabsf(v.x) < INFINITY) || !(fabsf(v.y) < INFINITY)) bad |= 1u << i;
+          }
+        }
+      __syncwarp();
+      const bool none = l == 0.f;
+      const float inv = none ? 0.f : pt_pow2(-vx) / l;
+      float* part = pt_parts(a) + (int64_t(blockIdx.x) * 2 + slot_of_part) * pt_part_floats(HD);
+#pragma unroll 1
+      for (int q = 0; q < HD / 32; ++q) {
+        uint32_t o[32];
+        pt_ld32(lanes + Sh::O_COL + q * 32, o);
+        tg_ld_wait();
+        const bool nan = (bad >> (q * 32 / GROUP)) & 1;
+#pragma unroll
+        for (int e0 = 0; e0 < 32; e0 += 8) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {  // column order 0 4 1 5 2 6 3 7
+            const float x = __uint_as_float(o[e0 + (e & 3) * 2 + (e >> 2)]);
+            v[e] = nan ? NAN : none ? 0.f : x * (whole ? inv : pt_pow2(-vx));
+          }
+          const int ch = q * 32 + e0;
+          if (!whole) {
+            float4* d = reinterpret_cast<float4*>(part + 2 * PT_ROWS + int64_t(tid) * HD + ch);
+            d[0] = make_float4(v[0], v[1], v[2], v[3]);
+            d[1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else if (tok < p.n) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (a.gate.p) v[e] *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch + e));
+              kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch + e, v[e]);
+            }
+          }
+        }
+      }
+      if (!whole) {
+        part[tid] = l != l ? INFINITY : m;  // a NaN sum stays NaN when parts are joined
+        part[PT_ROWS + tid] = l;
+      } else if (tok < p.n) {
+        pt_lse(a)[row * a.heads + hq] = none ? -INFINITY : (m + log2f(l)) * P_LN2;
+      }
+      tg_fence_before();
+    } else if (warp < 12) {
+      // ------------------------------------------------------ unpacking ----
+      // thread: unit r of slots t0 and t0 + 32 (of the tile), every 64-channel block
+      constexpr int NS = BN / 32;
+      const int ut = tid - PT_SOFT, r = ut & 7, t0 = ut >> 3;
+      const float ks = pt_pow2(kx), vs = pt_pow2(vx);
+      uint32_t kw[NS][NW], vw[NS][NW], kp[NS][NG], vp[NS][NG];
+      int pg[NS];
+      auto page_of = [&](int i, int q) {
+        const int s = (tb + i) * BN + t0 + 32 * q;
+        return i < nt && s < p.len ? __ldg(g.table + p.seq * g.tstride + (s >> g.pshift)) : -1;
+      };
+      const int nblk = g.page / g.seg;
+      auto load = [&](int i, uint32_t (&kwr)[NS][NW], uint32_t (&vwr)[NS][NW], uint32_t (&kpr)[NS][NG], uint32_t (&vpr)[NS][NG]) {
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+          const int s = (tb + i) * BN + t0 + 32 * q, t = s & (g.seg - 1);
+          if (unsigned(pg[q]) < unsigned(g.npages)) {
+            const uint8_t* blk = g.pages + pg[q] * g.page_bytes + int64_t(p.h * nblk + (s & (g.page - 1)) / g.seg) * g.blk;
+            const int off = t * (HD / 2) + ((r ^ kv4_swz(HD, t)) * (HD / 16)), po = g.seg * (HD / 2) + t * NG * 4;
+            kv4_ldv(blk + off, kwr[q]);
+            kv4_ldv(blk + g.blk / 2 + off, vwr[q]);
+            kv4_ldv(blk + po, kpr[q]);
+            kv4_ldv(blk + g.blk / 2 + po, vpr[q]);
+          } else {
+            // past the sequence, or a page outside the pool: zeros (the
+            // softmax gives such slots no weight)
+#pragma unroll
+            for (int w = 0; w < NW; ++w) kwr[q][w] = vwr[q][w] = 0u;
+#pragma unroll
+            for (int w = 0; w < NG; ++w) kpr[q][w] = vpr[q][w] = 0u;
+          }
+        }
+      };
+#pragma unroll
+      for (int q = 0; q < NS; ++q) pg[q] = page_of(0, q);
+      load(0, kw, vw, kp, vp);
+#pragma unroll
+      for (int q = 0; q < NS; ++q) pg[q] = page_of(1, q);
+      for (int i = 0; i < nt; ++i) {
+        const int jj = j + i, st = jj % ST;
+        const unsigned ph = (jj / ST) & 1;
+        uint32_t kw2[NS][NW], vw2[NS][NW], kp2[NS][NG], vp2[NS][NG];
+        if (i + 1 < nt) load(i + 1, kw2, vw2, kp2, vp2);
+#pragma unroll
+        for (int q = 0; q < NS; ++q) pg[q] = page_of(i + 2, q);
+        if (!tg_wait(&k_empty[st], ph ^ 1)) { fail(); break; }
+        if (*abort_flag) break;
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+          const int t = t0 + 32 * q;
+          uint8_t* d = sm + Sh::K_OFF + st * (T * Sh::KB) + t * 128 + ((r ^ (t & 7)) << 4);
+#pragma unroll
+          for (int w = 0; w < NW; ++w) {
+            float2 sb = kv4_param(kp[q][w * 64 / GROUP]);
+            sb.x *= ks;
+            sb.y *= ks;
+            uint4 hi, lo;
+            pt_unpack<SPLIT>(kw[q][w], sb, hi, lo);
+            *reinterpret_cast<uint4*>(d + w * (BN * 128)) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + w * (BN * 128)) = lo;
+          }
+        }
+        fence_proxy_async();
+        mbar_arrive(&k_full[st]);
+        if (!tg_wait(&v_empty[st], ph ^ 1)) { fail(); break; }
+        if (*abort_flag) break;
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+          const int t = t0 + 32 * q;
+          uint8_t* d = sm + Sh::V_OFF + st * (T * Sh::KB) + t * 128 + ((r ^ (t & 7)) << 4);
+#pragma unroll
+          for (int w = 0; w < NW; ++w) {
+            float2 sb = kv4_param(vp[q][w * 64 / GROUP]);
+            if (!(fabsf(sb.x) < INFINITY) || !(fabsf(sb.y) < INFINITY)) sb = make_float2(0.f, 0.f);
+            sb.x *= vs;
+            sb.y *= vs;
+            uint4 hi, lo;
+            pt_unpack<SPLIT>(vw[q][w], sb, hi, lo);
+            *reinterpret_cast<uint4*>(d + w * (BN * 128)) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + w * (BN * 128)) = lo;
+          }
+        }
+        fence_proxy_async();
+        mbar_arrive(&v_full[st]);
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+#pragma unroll
+          for (int w = 0; w < NW; ++w) kw[q][w] = kw2[q][w], vw[q][w] = vw2[q][w];
+#pragma unroll
+          for (int w = 0; w < NG; ++w) kp[q][w] = kp2[q][w], vp[q][w] = vp2[q][w];
+        }
+      }
+    } else if (lane == 0) {
+      // ------------------------------------------------------ MMA issue ----
+      const uint64_t qd = tg_desc(smem_u32(sm + Sh::Q_OFF));
+      constexpr uint32_t ids = pt_idesc(BN, false), idp = pt_idesc(HD, true);
+      bool ok = true;
+      auto qk = [&](int i) {
+        const int jj = j + i, st = jj % ST, b = jj & 1;
+        if (!tg_wait(&k_full[st], (jj / ST) & 1)) { fail(); return false; }
+        if (*abort_flag) return false;
+        tg_fence_after();
+        const uint64_t kd = tg_desc(smem_u32(sm + Sh::K_OFF + st * (T * Sh::KB)));
+        const uint32_t d = tmem + Sh::S_COL + b * BN;
+#pragma unroll
+        for (int tm = 0; tm < (SPLIT ? 3 : 1); ++tm)
+#pragma unroll
+          for (int w = 0; w < NW; ++w)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // 16 channels: 32 bytes of the 128-byte rows
+              const uint64_t ad = qd + (((tm == 1 ? Sh::QB : 0) + w * (PT_ROWS * 128) + k * 32) >> 4);
+              const uint64_t bd = kd + (((tm == 2 ? Sh::KB : 0) + w * (BN * 128) + k * 32) >> 4);
+              pt_mma_ss(d, ad, bd, ids, tm + w + k > 0);
+            }
+        tg_commit(&s_full[b]);
+        tg_commit(&k_empty[st]);
+        return true;
+      };
+      ok = qk(0);
+      for (int i = 0; i < nt && ok; ++i) {
+        if (i + 1 < nt) ok = qk(i + 1);
+        if (!ok) break;
+        const int jj = j + i, st = jj % ST, b = jj & 1;
+        if (!tg_wait(&v_full[st], (jj / ST) & 1) || !tg_wait(&p_full[b], (jj >> 1) & 1)) { fail(); break; }
+        if (*abort_flag) break;
+        tg_fence_after();
+        const uint64_t vd = pt_desc_n(smem_u32(sm + Sh::V_OFF + st * (T * Sh::KB)), BN * 128);
+        const uint32_t pc = tmem + Sh::P_COL + b * (T * BN / 2);
+#pragma unroll
+        for (int tm = 0; tm < (SPLIT ? 3 : 1); ++tm)
+#pragma unroll
+          for (int k = 0; k < BN / 16; ++k)
+            pt_mma_ts(tmem + Sh::O_COL, pc + (tm == 1 ? BN / 2 : 0) + k * 8, vd + (((tm == 2 ? Sh::KB : 0) + k * 2048) >> 4), idp,
+                      i + tm + k > 0);
+        tg_commit(&o_done[b]);
+        tg_commit(&v_empty[st]);
+      }
+    }
+    __syncwarp();
+    j += nt;
+    __syncthreads();
+    if (*abort_flag) break;
+    tg_fence_after();
+  }
+  __syncthreads();
+  if (warp == 12) {
+    if (lane == 0 && *abort_flag) {
+      tg_commit(drain);  // the products still in flight
+      tg_wait(drain, 0);
+    }
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Joins the parts of the item that begins in share x and goes on: one block per
+// (share, 16 rows), a thread a channel.
+template <int HD>
+__global__ void __launch_bounds__(HD) k_kv4_prompt_join(const Kv4AttnArgs a, int bn) {
+  const int nc = PT_GRID, x = blockIdx.x;
+  const int64_t total = pt_total(a, bn);
+  const int64_t r0 = total * x / nc, r1 = total * (x + 1) / nc;
+  PtPlace p = {};
+  if (r0 < r1) p = pt_find(a, bn, r1 - 1);
+  const int64_t begin = r1 - 1 - p.tile, end = begin + p.tiles;
+  pdl_wait();
+  if (r0 == r1 || begin < r0 || end <= r1) return;
+  int last = x, one = x;
+  while (last + 1 < nc && total * (last + 1) / nc < end) ++last;
+  while (total * (one + 1) / nc <= begin + PT_HEAD) ++one;
+  if (one == last) return;  // all its tiles in one share: written there
+  const float* parts = pt_parts(a);
+  auto has = [&](int i) {  // tiles of the item itself in share i
+    return max(begin + PT_HEAD, total * i / nc) < min(end, total * (i + 1) / nc);
+  };
+  for (int r = blockIdx.y * 16; r < blockIdx.y * 16 + 16; ++r) {
+    const int64_t ci = int64_t(p.qt) * PT_ROWS + r;
+    const int tok = int(ci / a.rep), hq = p.h * a.rep + int(ci % a.rep);
+    if (tok >= p.n) break;
+    float M = -INFINITY, L = 0.f, v = 0.f;
+    for (int i = one; i <= last; ++i) {
+      const float* q = parts + (int64_t(i) * 2 + (i == x ? 1 : 0)) * pt_part_floats(HD);
+      if (has(i)) M = fmaxf(M, __ldcg(q + r));
+    }
+    for (int i = one; i <= last; ++i) {
+      if (!has(i)) continue;
+      const float* q = parts + (int64_t(i) * 2 + (i == x ? 1 : 0)) * pt_part_floats(HD);
+      const float mi = __ldcg(q + r), f = mi == -INFINITY ? 0.f : pt_ex2(mi - M), o = __ldcg(q + 2 * PT_ROWS + int64_t(r) * HD + threadIdx.x);
+      L = fmaf(__ldcg(q + PT_ROWS + r), f, L);
+      v = fmaf(o, f, v);
+    }
+    v = L == 0.f ? v : v / L;  // an empty row: zeros, or NaN as its parts say
+    const int64_t row = p.row0 + tok;
+    if (a.gate.p) v *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + threadIdx.x));
+    kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + threadIdx.x, v);
+    if (threadIdx.x == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * P_LN2;
+  }
+}
+
+template <int HD, int GROUP, bool SPLIT>
+void run(const Kv4AttnArgs& a, cudaStream_t st) {
+  using Sh = PtShape<HD, SPLIT>;
+  launch(k_kv4_range, dim3(RG_SPLIT, a.b.nseq * a.g.kvh), dim3(256), 0, st, false, a);
+  launch(k_kv4_prompt<HD, GROUP, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS), Sh::TOTAL, st, true, a);
+  launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 16), dim3(HD), 0, st, true, a, int(Sh::BN));
+}
+
+template <int HD, int GROUP>
+void run_dt(const Kv4AttnArgs& a, cudaStream_t st) {
+  if (a.dt == DT_F32) run<HD, GROUP, true>(a, st);
+  else run<HD, GROUP, false>(a, st);
+}
+
+}  // namespace
+
+int64_t kv4_prompt_work(const Kv4Geo& g, const Kv4Batch& b, int heads) {
+  return pt_lse_bytes(b.total, heads) + pt_range_bytes(b.nseq, g.kvh) + int64_t(PT_GRID) * 2 * pt_part_floats(g.hd) * 4;
+}
+
+void launch_kv4_prompt(const Kv4AttnArgs& a, cudaStream_t st) {
+  if (int64_t(a.b.nseq) * a.g.kvh > 65535) throw Error(ERR_UNSUPPORTED, "kv4: more than 65535 sequences x kv heads with prompts");
+  if (a.g.hd == 64) run_dt<64, 64>(a, st);
+  else if (a.g.hd == 128) a.g.group == 64 ? run_dt<128, 64>(a, st) : run_dt<128, 128>(a, st);
+  else a.g.group == 64 ? run_dt<256, 64>(a, st) : run_dt<256, 128>(a, st);
+}
+
+}  // namespace swl

@@ -46,6 +46,7 @@
 #include "imma_impl.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "tc.cuh"
 
 namespace swl {
 
@@ -91,12 +92,6 @@ struct TgLayout {
 };
 
 // ---- tcgen05 / TMA primitives --------------------------------------------
-__device__ __forceinline__ uint64_t tg_desc(uint32_t saddr) {
-  // K-major operand, 128-byte swizzle: 8-row groups of 128-byte rows 1024
-  // bytes apart (SBO), descriptor version 1 (sm_100)
-  return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
-         (uint64_t(2) << 61);
-}
 __device__ __forceinline__ void tg_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -104,12 +99,6 @@ __device__ __forceinline__ void tg_mma(uint32_t d_tmem, uint64_t adesc, uint64_t
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(uint32_t(accumulate))
       : "memory");
 }
-__device__ __forceinline__ void tg_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void tg_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tg_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tg_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -117,7 +106,6 @@ __device__ __forceinline__ void tg_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tg_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tg_tma3(void* dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -137,18 +125,6 @@ __device__ __forceinline__ uint32_t tg_prmt(uint32_t a, uint32_t b, uint32_t sel
   uint32_t r;
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
   return r;
-}
-// Pipeline wait: polls without sleeping for the first ~4k tries (hand-offs
-// between the roles are short), then backs off; gives up after about 2 s.
-__device__ __forceinline__ bool tg_wait(uint64_t* b, unsigned parity) {
-  if (mbar_try(b, parity)) return true;
-  const unsigned long long t0 = gtimer();
-  for (int i = 0; i < (1 << 26); ++i) {
-    if (mbar_try(b, parity)) return true;
-    if (i >= 4096) __nanosleep(128);
-    if ((i & 255) == 0 && gtimer() - t0 > kWaitLimitNs) break;
-  }
-  return false;
 }
 // Exact float of an int32 partial sum (|v| < 2^22): magic-number conversion.
 __device__ __forceinline__ float tg_i2f(uint32_t v) {
