@@ -136,6 +136,52 @@ __device__ __forceinline__ void kv4_st(uint8_t* p, int dt, int64_t i, float v) {
   else if (dt == DT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
 }
+// Whether every 8 elements from a multiple of 8 on of r are 16-byte aligned.
+__device__ __forceinline__ bool kv4_vec(const Kv4Rows& r, int dt) {
+  const int64_t e = dt == DT_F32 ? 4 : 2;
+  return ((reinterpret_cast<uintptr_t>(r.p) | uintptr_t(r.ts * e) | uintptr_t(r.hs * e)) & 15) == 0;
+}
+// Eight consecutive elements; `vec`: 16-byte aligned.
+__device__ __forceinline__ void kv4_ld8(const uint8_t* p, int dt, int64_t i, bool vec, float (&x)[8]) {
+  if (!vec) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = kv4_ld(p, dt, i + e);
+  } else if (dt == DT_F32) {
+    const float4 a = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i)[0];
+    const float4 b = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i)[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[2 * e] = dt == DT_BF16 ? bf16_to_f32(uint16_t(w[e])) : f16_bits_to_f32(uint16_t(w[e]));
+      x[2 * e + 1] = dt == DT_BF16 ? bf16_to_f32(uint16_t(w[e] >> 16)) : f16_bits_to_f32(uint16_t(w[e] >> 16));
+    }
+  }
+}
+__device__ __forceinline__ void kv4_st8(uint8_t* p, int dt, int64_t i, bool vec, const float (&x)[8]) {
+  if (!vec) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) kv4_st(p, dt, i + e, x[e]);
+  } else if (dt == DT_F32) {
+    float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i);
+    d[0] = make_float4(x[0], x[1], x[2], x[3]);
+    d[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t lo = dt == DT_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x[2 * e])) : __half_as_ushort(__float2half_rn(x[2 * e]));
+      const uint32_t hi = dt == DT_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x[2 * e + 1])) : __half_as_ushort(__float2half_rn(x[2 * e + 1]));
+      w[e] = lo | hi << 16;
+    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+// Output gate: the fast exponential and divide are within a few ulp.
+__device__ __forceinline__ float kv4_sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+
 // N consecutive words of shared or global memory as one vector load.
 template <int N>
 __device__ __forceinline__ void kv4_ldv(const uint8_t* p, uint32_t (&w)[N]) {

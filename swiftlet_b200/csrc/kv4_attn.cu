@@ -294,7 +294,7 @@ __device__ __forceinline__ float* attn_parts(const Kv4AttnArgs& a) {
 
 // One output of a row, gated.
 __device__ __forceinline__ void write_out(const Kv4AttnArgs& a, int64_t row, int hq, int ch, float v) {
-  if (a.gate.p) v *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch));
+  if (a.gate.p) v *= kv4_sigmoid(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch));
   kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, v);
 }
 

@@ -37,7 +37,10 @@ namespace {
 constexpr int PT_ROWS = 128;
 constexpr int PT_GRID = 148;
 constexpr int PT_SOFT = 128, PT_UNPACK = 256;           // threads of the softmax and unpack roles
-constexpr int PT_THREADS = PT_SOFT + PT_UNPACK + 32;
+constexpr int PT_THREADS = PT_SOFT + PT_UNPACK + 128;   // and a warpgroup of which one thread issues the MMAs
+// Registers a thread: 128 at launch; the last warpgroup's go to the softmax
+// threads, which hold a row of S (128 + 128 + 88 + 168 = 4 x 128).
+constexpr int PT_REGS_SOFT = 168, PT_REGS_MMA = 88;
 constexpr int PT_HEAD = 4;                              // cost of an item beside its tiles, in tiles
 constexpr int RG_SPLIT = 16;                            // blocks a (sequence, head) of the range kernel
 constexpr float P_LOG2E = 1.4426950408889634f, P_LN2 = 0.6931471805599453f;
@@ -110,6 +113,16 @@ __device__ __forceinline__ void pt_st16(uint32_t t, const uint32_t* r) {
       : "memory");
 }
 __device__ __forceinline__ void pt_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// One lane of a converged warp.
+__device__ __forceinline__ bool pt_elect() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+template <int N>
+__device__ __forceinline__ void pt_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void pt_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ float pt_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -127,7 +140,7 @@ struct PtPlace {
 
 // Tiles of query tile qt: up to the last slot its last row sees.
 __device__ __forceinline__ int pt_tiles(int n, int len, int rep, int bn, int qt) {
-  const int last = int(min(int64_t(n) - 1, (int64_t(qt + 1) * PT_ROWS - 1) / rep));
+  const int last = int(min(unsigned(n) - 1u, (unsigned(qt + 1) * PT_ROWS - 1u) / unsigned(rep)));
   const int seen = max(0, min(len, len - n + last + 1));
   return PT_HEAD + max(1, (seen + bn - 1) / bn);
 }
@@ -135,7 +148,7 @@ __device__ __forceinline__ void pt_seq(const Kv4AttnArgs& a, int seq, PtPlace& p
   p.seq = seq;
   p.n = kv4_new(a.b, seq, p.row0);
   p.len = kv4_len(a.b, seq);
-  p.nq = int((int64_t(p.n) * a.rep + PT_ROWS - 1) / PT_ROWS);
+  p.nq = (p.n * a.rep + PT_ROWS - 1) / PT_ROWS;
 }
 __device__ __forceinline__ int64_t pt_total(const Kv4AttnArgs& a, int bn) {
   int64_t sum = 0;
@@ -244,15 +257,22 @@ __global__ void __launch_bounds__(256) k_kv4_range(const Kv4AttnArgs a) {
 }
 
 // Exponent that takes a largest |value| (f32 bits) to [2^13, 2^14).
-__device__ __forceinline__ int pt_exp(unsigned bits) { return bits ? max(-14, min(60, 13 - (int(bits >> 23) - 127))) : 0; }
+__device__ __forceinline__ int pt_exp(unsigned bits) { return bits ? max(-14, min(28, 13 - (int(bits >> 23) - 127))) : 0; }
 __device__ __forceinline__ float pt_pow2(int e) { return __int_as_float((127 + e) << 23); }
 
-// Eight codes of a word as f16 pairs (0 4)(1 5)(2 6)(3 7): value 2^x (s c + b)
-// rounded once, or to two terms. f16 inputs of the arithmetic: the scaled
-// params (rounded where 2^x takes them below f16's normal range, 2^-28 of the
-// largest value).
+// Params times 2^x as two f16 factors of at most 2^14 (exact, but where they
+// leave f16's normal range: below 2^-28 of the largest value).
+struct PtScale {
+  __half2 h0, h1;
+  __device__ explicit PtScale(int x) : h0(__float2half2_rn(pt_pow2(x / 2))), h1(__float2half2_rn(pt_pow2(x - x / 2))) {}
+  __device__ __half2 of(uint32_t param) const { return __hmul2(__hmul2(pt_u2(param), h0), h1); }
+};
+
+// Eight codes of a word as f16 pairs (0 4)(1 5)(2 6)(3 7): the scaled value s c
+// + b, rounded once, or as two terms. The codes themselves come out of the
+// bits exactly: 1024 + c (or 1024 + 16 c) less the constant.
 template <bool SPLIT>
-__device__ __forceinline__ void pt_unpack(uint32_t w, float2 sb, uint4& hi, uint4& lo) {
+__device__ __forceinline__ void pt_unpack(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
   uint32_t* H = &hi.x;
   uint32_t* L = &lo.x;
   const __half2 m0 = pt_u2(0xe400e400u);                          // -1024
@@ -265,15 +285,16 @@ __device__ __forceinline__ void pt_unpack(uint32_t w, float2 sb, uint4& hi, uint
     c[2 * i + 1] = __hfma2(pt_u2((x & 0x00f000f0u) | 0x64006400u), r, m1);
   }
   if (!SPLIT) {
-    const __half2 s = __float2half2_rn(sb.x), b = __float2half2_rn(sb.y);
+    const __half2 s = __low2half2(sb), b = __high2half2(sb);
 #pragma unroll
     for (int i = 0; i < 4; ++i) H[i] = pt_h2(__hfma2(c[i], s, b));
   } else {
+    const float2 f2 = __half22float2(sb);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float2 v = __half22float2(c[i]);
-      v.x = fmaf(sb.x, v.x, sb.y);
-      v.y = fmaf(sb.x, v.y, sb.y);
+      v.x = fmaf(f2.x, v.x, f2.y);
+      v.y = fmaf(f2.x, v.y, f2.y);
       const __half2 h = __floats2half2_rn(v.x, v.y);
       const float2 f = __half22float2(h);
       H[i] = pt_h2(h);
@@ -329,71 +350,43 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
     if (a.b.status) atomicOr(a.b.status, 1);
     *abort_flag = 1;
   };
-  PtPlace p = {};
-  if (r0 < r1) p = pt_find(a, BN, r0);
-  int j = 0;  // tiles done by this CTA, the pipelines' counter
-  for (int64_t f = r0; f < r1; pt_next(a, BN, p)) {
-    const int v1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
-    const int tb = max(0, p.tile - PT_HEAD), nt = v1 - PT_HEAD - tb, slot_of_part = p.tile == 0 ? 1 : 0;
-    f += v1 - p.tile;
-    if (v1 <= PT_HEAD || nt <= 0) continue;
-    // ranges of the item
-    unsigned mk = 0u, mv = 0u, vnan = 0u;
-    if (lane < RG_SPLIT) {
-      const int4 q = __ldcg(pt_ranges(a) + (int64_t(p.seq) * g.kvh + p.h) * RG_SPLIT + lane);
-      mk = unsigned(q.x), mv = unsigned(q.y), vnan = unsigned(q.z);
-    }
-    mk = __reduce_max_sync(0xffffffffu, mk);
-    mv = __reduce_max_sync(0xffffffffu, mv);
-    vnan = __reduce_or_sync(0xffffffffu, vnan);
-    const int kx = pt_exp(mk), vx = pt_exp(mv);
-    const bool lost = (vnan & 2u) != 0u;
-    vnan &= 1u;
-
-    if (warp >= 4 && warp < 12) {
-      // ------------------------------------------------------ unpacking ----
-      // queries: a warp a row, eight channels a lane
-      for (int r = warp - 4; r < PT_ROWS; r += 8) {
-        const int64_t ci = int64_t(p.qt) * PT_ROWS + r;
-        const int t = int(ci / a.rep), hq = p.h * a.rep + int(ci % a.rep);
-        const bool on = t < p.n, act = lane < HD / 8;
-        float x[8], am = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = on && act ? kv4_ld(a.q.p, a.dt, (p.row0 + t) * a.q.ts + hq * a.q.hs + lane * 8 + e) : 0.f;
-          am = fmaxf(am, fabsf(x[e]));
-        }
-        am = warp_max(am);
-        int ex = am > 0.f && am < INFINITY ? 12 - (int(__float_as_uint(am) >> 23) - 127) : 0;
-        ex = max(-60, min(60, ex));
-        const float up = pt_pow2(ex);
-        if (act) {
-          uint4 hi, lo;
-          uint32_t *H = &hi.x, *L = &lo.x;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {  // the order the codes come unpacked in
-            const float v0 = x[i] * up, v1f = x[i + 4] * up;
-            const __half2 hh = __floats2half2_rn(v0, v1f);
-            H[i] = pt_h2(hh);
-            if (SPLIT) {
-              const float2 ff = __half22float2(hh);
-              L[i] = pt_h2(__floats2half2_rn(v0 - ff.x, v1f - ff.y));
-            }
-          }
-          uint8_t* d = sm + Sh::Q_OFF + (lane >> 3) * (PT_ROWS * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
-          *reinterpret_cast<uint4*>(d) = hi;
-          if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::QB) = lo;
-        }
-        if (lane == 0) {
-          row_mul[r] = a.scale * P_LOG2E * pt_pow2(-ex) * pt_pow2(-kx);
-          row_lim[r] = on ? p.len - p.n + t : p.len - 1;
-        }
+  // One role's walk over the items of the share: body(p, tb, nt, v1, slot, kx,
+  // vx, flags) has one barrier of all roles in it (queries staged), and one
+  // follows it (everything of the item is over). j counts the tiles of this
+  // CTA, the pipelines' index.
+  int j = 0;
+  // barrier 1: the last three warps wait at the kernel's end, on barrier 0
+  auto bar = [] { asm volatile("bar.sync 1, %0;" ::"n"(PT_SOFT + PT_UNPACK + 32) : "memory"); };
+  auto for_items = [&](auto body) {
+    PtPlace p = {};
+    if (r0 < r1) p = pt_find(a, BN, r0);
+    for (int64_t f = r0; f < r1; pt_next(a, BN, p)) {
+      const int v1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
+      const int tb = max(0, p.tile - PT_HEAD), nt = v1 - PT_HEAD - tb, slot = p.tile == 0 ? 1 : 0;
+      f += v1 - p.tile;
+      if (v1 <= PT_HEAD || nt <= 0) continue;
+      unsigned mk = 0u, mv = 0u, flags = 0u;
+      if (lane < RG_SPLIT) {
+        const int4 q = __ldcg(pt_ranges(a) + (int64_t(p.seq) * g.kvh + p.h) * RG_SPLIT + lane);
+        mk = unsigned(q.x), mv = unsigned(q.y), flags = unsigned(q.z);
       }
-      fence_proxy_async();
+      mk = __reduce_max_sync(0xffffffffu, mk);
+      mv = __reduce_max_sync(0xffffffffu, mv);
+      flags = __reduce_or_sync(0xffffffffu, flags);
+      body(p, tb, nt, v1, slot, pt_exp(mk), pt_exp(mv), flags);
+      __syncwarp();
+      j += nt;
+      bar();
+      if (*abort_flag) break;
+      tg_fence_after();
     }
-    __syncthreads();  // queries staged (and TMEM and buffers of the last item free)
+  };
 
-    if (warp < 4) {
+  if (warp < 4) {
+    pt_regs_inc<PT_REGS_SOFT>();
+    for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part, int kx, int vx, unsigned flags) {
+      const bool lost = (flags & 2u) != 0u, vnan = (flags & 1u) != 0u;
+      bar();
       // -------------------------------------------------------- softmax ----
       const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
       const float mul = row_mul[tid];
@@ -484,9 +477,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         mbar_arrive(&p_full[b]);
       }
       // ---- output: the last product has landed ----
-      const int64_t ci = int64_t(p.qt) * PT_ROWS + tid;
-      const int tok = int(ci / a.rep), hq = p.h * a.rep + int(ci % a.rep);
+      const unsigned ci = unsigned(p.qt * PT_ROWS + tid);
+      const int tok = int(ci / unsigned(a.rep)), hq = p.h * a.rep + int(ci % unsigned(a.rep));
       const int64_t row = p.row0 + tok;
+      const bool vo = kv4_vec(a.out, a.dt), vg = kv4_vec(a.gate, a.dt);
       const bool whole = tb == 0 && v1 == p.tiles;
       const int last = j + nt - 1;
       const bool done = !*abort_flag && tg_wait(&o_done[last & 1], (last >> 1) & 1);
@@ -529,11 +523,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
             d[0] = make_float4(v[0], v[1], v[2], v[3]);
             d[1] = make_float4(v[4], v[5], v[6], v[7]);
           } else if (tok < p.n) {
+            if (a.gate.p) {
+              float gt[8];
+              kv4_ld8(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch, vg, gt);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (a.gate.p) v[e] *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch + e));
-              kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch + e, v[e]);
+              for (int e = 0; e < 8; ++e) v[e] *= kv4_sigmoid(gt[e]);
             }
+            kv4_st8(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, vo, v);
           }
         }
       }
@@ -544,12 +540,65 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         pt_lse(a)[row * a.heads + hq] = none ? -INFINITY : (m + log2f(l)) * P_LN2;
       }
       tg_fence_before();
-    } else if (warp < 12) {
+    });
+  } else if (warp < 12) {
+    for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part, int kx, int vx, unsigned flags) {
+      // ------------------------------------------------------ unpacking ----
+      // queries: a warp a row, eight channels a lane, four rows at a time
+      const bool vq = kv4_vec(a.q, a.dt), act = lane < HD / 8;
+      for (int rb = warp - 4; rb < PT_ROWS; rb += 32) {
+        float x[4][8];
+        int tok[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned ci = unsigned(p.qt * PT_ROWS + rb + 8 * k);
+          tok[k] = int(ci / unsigned(a.rep));
+          const int hq = p.h * a.rep + int(ci - unsigned(tok[k]) * unsigned(a.rep));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[k][e] = 0.f;
+          if (tok[k] < p.n && act) kv4_ld8(a.q.p, a.dt, int64_t(p.row0 + tok[k]) * a.q.ts + hq * a.q.hs + lane * 8, vq, x[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = rb + 8 * k;
+          float am = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[k][e]));
+          am = warp_max(am);
+          int ex = am > 0.f && am < INFINITY ? 12 - (int(__float_as_uint(am) >> 23) - 127) : 0;
+          ex = max(-60, min(60, ex));
+          const float up = pt_pow2(ex);
+          if (act) {
+            uint4 hi, lo;
+            uint32_t *H = &hi.x, *L = &lo.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // the order the codes come unpacked in
+              const float v0 = x[k][i] * up, v1f = x[k][i + 4] * up;
+              const __half2 hh = __floats2half2_rn(v0, v1f);
+              H[i] = pt_h2(hh);
+              if (SPLIT) {
+                const float2 ff = __half22float2(hh);
+                L[i] = pt_h2(__floats2half2_rn(v0 - ff.x, v1f - ff.y));
+              }
+            }
+            uint8_t* d = sm + Sh::Q_OFF + (lane >> 3) * (PT_ROWS * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+            *reinterpret_cast<uint4*>(d) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::QB) = lo;
+          }
+          if (lane == 0) {
+            row_mul[r] = a.scale * P_LOG2E * pt_pow2(-ex) * pt_pow2(-kx);
+            row_lim[r] = tok[k] < p.n ? p.len - p.n + tok[k] : p.len - 1;
+          }
+        }
+      }
+      fence_proxy_async();
+      bar();
       // ------------------------------------------------------ unpacking ----
       // thread: unit r of slots t0 and t0 + 32 (of the tile), every 64-channel block
       constexpr int NS = BN / 32;
       const int ut = tid - PT_SOFT, r = ut & 7, t0 = ut >> 3;
-      const float ks = pt_pow2(kx), vs = pt_pow2(vx);
+      const PtScale ks(kx), vs(vx);
+      const bool vnan = (flags & 1u) != 0u;
       uint32_t kw[NS][NW], vw[NS][NW], kp[NS][NG], vp[NS][NG];
       int pg[NS];
       auto page_of = [&](int i, int q) {
@@ -598,11 +647,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           uint8_t* d = sm + Sh::K_OFF + st * (T * Sh::KB) + t * 128 + ((r ^ (t & 7)) << 4);
 #pragma unroll
           for (int w = 0; w < NW; ++w) {
-            float2 sb = kv4_param(kp[q][w * 64 / GROUP]);
-            sb.x *= ks;
-            sb.y *= ks;
             uint4 hi, lo;
-            pt_unpack<SPLIT>(kw[q][w], sb, hi, lo);
+            pt_unpack<SPLIT>(kw[q][w], ks.of(kp[q][w * 64 / GROUP]), hi, lo);
             *reinterpret_cast<uint4*>(d + w * (BN * 128)) = hi;
             if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + w * (BN * 128)) = lo;
           }
@@ -617,12 +663,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           uint8_t* d = sm + Sh::V_OFF + st * (T * Sh::KB) + t * 128 + ((r ^ (t & 7)) << 4);
 #pragma unroll
           for (int w = 0; w < NW; ++w) {
-            float2 sb = kv4_param(vp[q][w * 64 / GROUP]);
-            if (!(fabsf(sb.x) < INFINITY) || !(fabsf(sb.y) < INFINITY)) sb = make_float2(0.f, 0.f);
-            sb.x *= vs;
-            sb.y *= vs;
+            uint32_t sb = vp[q][w * 64 / GROUP];
+            if (vnan && (!(fabsf(kv4_param(sb).x) < INFINITY) || !(fabsf(kv4_param(sb).y) < INFINITY))) sb = 0u;
             uint4 hi, lo;
-            pt_unpack<SPLIT>(vw[q][w], sb, hi, lo);
+            pt_unpack<SPLIT>(vw[q][w], vs.of(sb), hi, lo);
             *reinterpret_cast<uint4*>(d + w * (BN * 128)) = hi;
             if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + w * (BN * 128)) = lo;
           }
@@ -637,62 +681,69 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           for (int w = 0; w < NG; ++w) kp[q][w] = kp2[q][w], vp[q][w] = vp2[q][w];
         }
       }
-    } else if (lane == 0) {
-      // ------------------------------------------------------ MMA issue ----
-      const uint64_t qd = tg_desc(smem_u32(sm + Sh::Q_OFF));
-      constexpr uint32_t ids = pt_idesc(BN, false), idp = pt_idesc(HD, true);
-      bool ok = true;
-      auto qk = [&](int i) {
-        const int jj = j + i, st = jj % ST, b = jj & 1;
-        if (!tg_wait(&k_full[st], (jj / ST) & 1)) { fail(); return false; }
-        if (*abort_flag) return false;
-        tg_fence_after();
-        const uint64_t kd = tg_desc(smem_u32(sm + Sh::K_OFF + st * (T * Sh::KB)));
-        const uint32_t d = tmem + Sh::S_COL + b * BN;
+    });
+  } else {
+    pt_regs_dec<PT_REGS_MMA>();
+    if (warp == 12)
+      for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part, int kx, int vx, unsigned flags) {
+        bar();
+        // ---------------------------------------------------- MMA issue ----
+        // The warp stays together, so that descriptors live in uniform
+        // registers; one elected lane issues.
+        constexpr uint32_t ids = pt_idesc(BN, false), idp = pt_idesc(HD, true);
+        auto wait = [&](uint64_t* b, unsigned ph) {
+          if (__all_sync(0xffffffffu, tg_wait(b, ph) && !*abort_flag)) return true;
+          fail();
+          return false;
+        };
+        auto qk = [&](int i) {
+          const int jj = j + i, st = jj % ST, b = jj & 1;
+          if (!wait(&k_full[st], (jj / ST) & 1)) return false;
+          tg_fence_after();
+          const uint64_t qd = tg_desc(smem_u32(sm + Sh::Q_OFF)), kd = tg_desc(smem_u32(sm + Sh::K_OFF + st * (T * Sh::KB)));
+          const uint32_t d = tmem + Sh::S_COL + b * BN;
+          if (pt_elect()) {
+#pragma unroll 1
+            for (int tm = 0; tm < (SPLIT ? 3 : 1); ++tm)
 #pragma unroll
-        for (int tm = 0; tm < (SPLIT ? 3 : 1); ++tm)
+              for (int w = 0; w < NW; ++w)
 #pragma unroll
-          for (int w = 0; w < NW; ++w)
+                for (int k = 0; k < 4; ++k)  // 16 channels: 32 bytes of the 128-byte rows
+                  pt_mma_ss(d, qd + (((tm == 1 ? Sh::QB : 0) + w * (PT_ROWS * 128) + k * 32) >> 4),
+                            kd + (((tm == 2 ? Sh::KB : 0) + w * (BN * 128) + k * 32) >> 4), ids, tm + w + k > 0);
+            tg_commit(&s_full[b]);
+            tg_commit(&k_empty[st]);
+          }
+          __syncwarp();
+          return true;
+        };
+        bool ok = qk(0);
+        for (int i = 0; i < nt && ok; ++i) {
+          if (i + 1 < nt) ok = qk(i + 1);
+          const int jj = j + i, st = jj % ST, b = jj & 1;
+          if (!ok || !wait(&v_full[st], (jj / ST) & 1) || !wait(&p_full[b], (jj >> 1) & 1)) break;
+          tg_fence_after();
+          const uint64_t vd = pt_desc_n(smem_u32(sm + Sh::V_OFF + st * (T * Sh::KB)), BN * 128);
+          const uint32_t pc = tmem + Sh::P_COL + b * (T * BN / 2);
+          if (pt_elect()) {
+#pragma unroll 1
+            for (int tm = 0; tm < (SPLIT ? 3 : 1); ++tm)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {  // 16 channels: 32 bytes of the 128-byte rows
-              const uint64_t ad = qd + (((tm == 1 ? Sh::QB : 0) + w * (PT_ROWS * 128) + k * 32) >> 4);
-              const uint64_t bd = kd + (((tm == 2 ? Sh::KB : 0) + w * (BN * 128) + k * 32) >> 4);
-              pt_mma_ss(d, ad, bd, ids, tm + w + k > 0);
-            }
-        tg_commit(&s_full[b]);
-        tg_commit(&k_empty[st]);
-        return true;
-      };
-      ok = qk(0);
-      for (int i = 0; i < nt && ok; ++i) {
-        if (i + 1 < nt) ok = qk(i + 1);
-        if (!ok) break;
-        const int jj = j + i, st = jj % ST, b = jj & 1;
-        if (!tg_wait(&v_full[st], (jj / ST) & 1) || !tg_wait(&p_full[b], (jj >> 1) & 1)) { fail(); break; }
-        if (*abort_flag) break;
-        tg_fence_after();
-        const uint64_t vd = pt_desc_n(smem_u32(sm + Sh::V_OFF + st * (T * Sh::KB)), BN * 128);
-        const uint32_t pc = tmem + Sh::P_COL + b * (T * BN / 2);
-#pragma unroll
-        for (int tm = 0; tm < (SPLIT ? 3 : 1); ++tm)
-#pragma unroll
-          for (int k = 0; k < BN / 16; ++k)
-            pt_mma_ts(tmem + Sh::O_COL, pc + (tm == 1 ? BN / 2 : 0) + k * 8, vd + (((tm == 2 ? Sh::KB : 0) + k * 2048) >> 4), idp,
-                      i + tm + k > 0);
-        tg_commit(&o_done[b]);
-        tg_commit(&v_empty[st]);
-      }
-    }
-    __syncwarp();
-    j += nt;
-    __syncthreads();
-    if (*abort_flag) break;
-    tg_fence_after();
+              for (int k = 0; k < BN / 16; ++k)
+                pt_mma_ts(tmem + Sh::O_COL, pc + (tm == 1 ? BN / 2 : 0) + k * 8, vd + (((tm == 2 ? Sh::KB : 0) + k * 2048) >> 4), idp,
+                          tm + k > 0 || i > 0);
+            tg_commit(&o_done[b]);
+            tg_commit(&v_empty[st]);
+          }
+          __syncwarp();
+        }
+      });
   }
   __syncthreads();
   if (warp == 12) {
-    if (lane == 0 && *abort_flag) {
-      tg_commit(drain);  // the products still in flight
+    if (*abort_flag) {
+      if (pt_elect()) tg_commit(drain);  // the products still in flight
+      __syncwarp();
       tg_wait(drain, 0);
     }
     __syncwarp();
@@ -721,8 +772,8 @@ __global__ void __launch_bounds__(HD) k_kv4_prompt_join(const Kv4AttnArgs a, int
     return max(begin + PT_HEAD, total * i / nc) < min(end, total * (i + 1) / nc);
   };
   for (int r = blockIdx.y * 16; r < blockIdx.y * 16 + 16; ++r) {
-    const int64_t ci = int64_t(p.qt) * PT_ROWS + r;
-    const int tok = int(ci / a.rep), hq = p.h * a.rep + int(ci % a.rep);
+    const unsigned ci = unsigned(p.qt * PT_ROWS + r);
+    const int tok = int(ci / unsigned(a.rep)), hq = p.h * a.rep + int(ci % unsigned(a.rep));
     if (tok >= p.n) break;
     float M = -INFINITY, L = 0.f, v = 0.f;
     for (int i = one; i <= last; ++i) {
@@ -738,7 +789,7 @@ __global__ void __launch_bounds__(HD) k_kv4_prompt_join(const Kv4AttnArgs a, int
     }
     v = L == 0.f ? v : v / L;  // an empty row: zeros, or NaN as its parts say
     const int64_t row = p.row0 + tok;
-    if (a.gate.p) v *= sigmoid_ref(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + threadIdx.x));
+    if (a.gate.p) v *= kv4_sigmoid(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + threadIdx.x));
     kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + threadIdx.x, v);
     if (threadIdx.x == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * P_LN2;
   }
@@ -765,6 +816,7 @@ int64_t kv4_prompt_work(const Kv4Geo& g, const Kv4Batch& b, int heads) {
 }
 
 void launch_kv4_prompt(const Kv4AttnArgs& a, cudaStream_t st) {
+  if (int64_t(a.b.total) * a.rep > 0x7fffff00) throw Error(ERR_UNSUPPORTED, "kv4: more than 2^31 query rows a kv head");
   if (int64_t(a.b.nseq) * a.g.kvh > 65535) throw Error(ERR_UNSUPPORTED, "kv4: more than 65535 sequences x kv heads with prompts");
   if (a.g.hd == 64) run_dt<64, 64>(a, st);
   else if (a.g.hd == 128) a.g.group == 64 ? run_dt<128, 64>(a, st) : run_dt<128, 128>(a, st);
