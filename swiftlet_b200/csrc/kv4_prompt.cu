@@ -13,12 +13,15 @@
 // inputs: every operand as two f16 terms (22 bits) and three products each
 // (hi hi + lo hi + hi lo), f32 accumulators throughout.
 //
-// Warps: 0-3 softmax and output, 4-11 unpacking, 12 MMA issue and TMEM. S and
-// P are double-buffered, so Q K^T of the next tile runs during the softmax of
-// this one; the running maximum moves only when it has grown by 2^8, so O in
-// TMEM is rarely touched. Bound: the tensor cores (a tile of 64 slots at 256
-// channels is 1024 cycles of MMA for 16-bit inputs), next to the issue slots
-// of the unpacking (15 instructions per 8 values) and the softmax.
+// Warps: 0-7 softmax and output (two threads a row, half of the tile's slots
+// each), 8-15 unpacking, 16 MMA issue and TMEM, 17 bulk copies of the cache's
+// bytes into a ring of 32-slot stages. Q stands in TMEM (its low terms in shared
+// memory), S and P share columns and are double-buffered, so Q K^T of the next
+// tile runs during the softmax of this one; the running maximum moves only
+// when it has grown by 2^8, so O in TMEM is rarely touched. Bound: the tensor
+// cores (a tile of 64 slots at 256 channels is 1024 cycles of MMA for 16-bit
+// inputs), next to the issue slots of the unpacking (14 instructions per 8
+// values) and of the softmax.
 //
 // The work is shared out like that of kv4_attn.cu: equal contiguous shares of
 // all tiles of all items over 148 CTAs, parts of an item that several CTAs
@@ -35,30 +38,39 @@ namespace swl {
 namespace {
 
 constexpr int PT_ROWS = 128;
+constexpr int PT_BN = 64;                               // slots of a tile
+constexpr int PT_RAW = 32;                              // slots of a copied stage
 constexpr int PT_GRID = 148;
-constexpr int PT_SOFT = 128, PT_UNPACK = 256;           // threads of the softmax and unpack roles
-constexpr int PT_THREADS = PT_SOFT + PT_UNPACK + 128;   // and a warpgroup of which one thread issues the MMAs
-// Registers a thread: 128 at launch; the last warpgroup's go to the softmax
-// threads, which hold a row of S (128 + 128 + 88 + 168 = 4 x 128).
-constexpr int PT_REGS_SOFT = 168, PT_REGS_MMA = 88;
+constexpr int PT_SOFT = 256, PT_UNPACK = 256;           // threads of the softmax and unpack roles
+constexpr int PT_THREADS = PT_SOFT + PT_UNPACK + 128;   // and a warpgroup that issues MMAs and copies
+// Registers a thread: 96 at launch; the last warpgroup's spare ones go to the
+// softmax (256 x 104 + 256 x 96 + 128 x 80 = 640 x 96).
+constexpr int PT_REGS_SOFT = 104, PT_REGS_ISSUE = 80;
 constexpr int PT_HEAD = 4;                              // cost of an item beside its tiles, in tiles
 constexpr int RG_SPLIT = 16;                            // blocks a (sequence, head) of the range kernel
 constexpr float P_LOG2E = 1.4426950408889634f, P_LN2 = 0.6931471805599453f;
 
-template <int HD, bool SPLIT>
+template <int HD, int GROUP, bool SPLIT>
 struct PtShape {
-  static constexpr int BN = HD == 256 && SPLIT ? 32 : 64;  // slots of a tile (shared memory holds two terms of Q)
   static constexpr int T = SPLIT ? 2 : 1;                  // f16 terms of an operand
-  static constexpr int ST = HD == 256 && SPLIT ? 1 : 2;    // buffers of unpacked keys, and of values
+  static constexpr int KST = HD == 256 && SPLIT ? 1 : 2;   // buffers of unpacked keys, and of values
+  static constexpr int RST = HD == 256 && SPLIT ? 3 : 4;   // copied stages
   static constexpr int QB = PT_ROWS * HD * 2;              // bytes of one term of Q
-  static constexpr int KB = BN * HD * 2;                   // of one term of a tile's keys (values)
-  static constexpr int Q_OFF = 0, K_OFF = T * QB, V_OFF = K_OFF + ST * T * KB, M_OFF = V_OFF + ST * T * KB;
-  static constexpr int BAR_OFF = M_OFF + PT_ROWS * 8;      // after the rows' factors and limits
-  static constexpr int NBAR = 4 * ST + 2 + 2 + 2 + 1;      // k full / empty, v full / empty, s full, p full, o done, drain
-  static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 16 + 1024;  // 1024: base alignment
-  // TMEM columns
-  static constexpr int O_COL = 0, S_COL = HD, P_COL = HD + 2 * BN;
-  static_assert(P_COL + 2 * T * BN / 2 <= 512, "TMEM columns");
+  static constexpr int KB = PT_BN * HD * 2;                // of one term of a tile's keys (values)
+  static constexpr int CODES = PT_RAW * HD / 2, PARAMS = PT_RAW * 4 * (HD / GROUP), RAW = 2 * (CODES + PARAMS);
+  // low terms of Q, keys (first the high terms of Q, on their way to TMEM), values, copied stages
+  static constexpr int SCR = 8 * 32 * 33 * 4;              // the output's scratch, over the key buffers
+  static constexpr int KS = KST * T * KB > SCR ? KST * T * KB : (SCR + 1023) / 1024 * 1024;
+  static constexpr int Q_OFF = 0, K_OFF = SPLIT ? QB : 0, V_OFF = K_OFF + KS, R_OFF = V_OFF + KST * T * KB;
+  static constexpr int M_OFF = R_OFF + RST * RAW;          // the rows' factors and limits, exchange of the halves
+  static constexpr int BAR_OFF = M_OFF + PT_ROWS * 16;
+  static constexpr int NBAR = 4 * KST + 2 * RST + 7;       // k, v full / empty, raw full / empty, s full, p full, o done, drain
+  static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 16 + RST * 4 + 1024;  // 1024: base alignment
+  static_assert(KS >= QB, "Q fits the key buffers");
+  static_assert(TOTAL <= 232448, "shared memory");
+  // TMEM columns: O, S (two tiles; P over it), Q
+  static constexpr int O_COL = 0, S_COL = HD, Q_COL = HD + 2 * PT_BN;
+  static_assert(Q_COL + HD / 2 <= 512, "TMEM columns");
 };
 
 // D f32, A and B f16; N, transposed (N-major) B
@@ -118,6 +130,17 @@ __device__ __forceinline__ bool pt_elect() {
   uint32_t ok;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
   return ok != 0;
+}
+// Barrier `id` of N threads; true when `v` is true for any of them.
+template <int N = 64>
+__device__ __forceinline__ bool pt_bar_any(int id, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %2, 0;\n\tbarrier.cta.red.or.pred.aligned q, %1, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(uint32_t(v)), "n"(N)
+      : "memory");
+  return r != 0;
 }
 template <int N>
 __device__ __forceinline__ void pt_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -209,15 +232,22 @@ __device__ __forceinline__ void pt_next(const Kv4AttnArgs& a, int bn, PtPlace& p
   }
 }
 
-// Workspace: lse rows, ranges, parts.
+// The item that begins in a share and goes on: shares first .. last hold its
+// parts (first < 0: none).
+struct PtJoin {
+  int first, last, row0, n, qt, h, pad[2];
+};
+
+// Workspace: lse rows, ranges, joins, parts.
 __host__ __device__ inline int64_t pt_lse_bytes(int64_t total, int heads) { return (total * heads * 4 + 15) / 16 * 16; }
 __host__ __device__ inline int64_t pt_range_bytes(int64_t nseq, int kvh) { return nseq * kvh * RG_SPLIT * 16; }
 __host__ __device__ constexpr int pt_part_floats(int hd) { return PT_ROWS * (hd + 2); }
 __device__ __forceinline__ float* pt_lse(const Kv4AttnArgs& a) { return a.lse ? a.lse : reinterpret_cast<float*>(a.work); }
 __device__ __forceinline__ int4* pt_ranges(const Kv4AttnArgs& a) { return reinterpret_cast<int4*>(a.work + pt_lse_bytes(a.b.total, a.heads)); }
-__device__ __forceinline__ float* pt_parts(const Kv4AttnArgs& a) {
-  return reinterpret_cast<float*>(a.work + pt_lse_bytes(a.b.total, a.heads) + pt_range_bytes(a.b.nseq, a.g.kvh));
+__device__ __forceinline__ PtJoin* pt_joins(const Kv4AttnArgs& a) {
+  return reinterpret_cast<PtJoin*>(a.work + pt_lse_bytes(a.b.total, a.heads) + pt_range_bytes(a.b.nseq, a.g.kvh));
 }
+__device__ __forceinline__ float* pt_parts(const Kv4AttnArgs& a) { return reinterpret_cast<float*>(pt_joins(a) + PT_GRID); }
 
 // Largest |value| of the keys and of the values of each (sequence, kv head),
 // as f32 bits, and flags (bit 0: a value group is NaN, bit 1: a page outside the
@@ -305,25 +335,31 @@ __device__ __forceinline__ void pt_unpack(uint32_t w, __half2 sb, uint4& hi, uin
 
 template <int HD, int GROUP, bool SPLIT>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs a) {
-  using Sh = PtShape<HD, SPLIT>;
-  constexpr int BN = Sh::BN, T = Sh::T, ST = Sh::ST, NG = HD / GROUP, NW = HD / 64;
+  using Sh = PtShape<HD, GROUP, SPLIT>;
+  constexpr int BN = PT_BN, T = Sh::T, KST = Sh::KST, RST = Sh::RST, NG = HD / GROUP, NW = HD / 64;
   extern __shared__ __align__(1024) uint8_t pt_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
   float* row_mul = reinterpret_cast<float*>(sm + Sh::M_OFF);
   int* row_lim = reinterpret_cast<int*>(row_mul + PT_ROWS);
+  float* xch = reinterpret_cast<float*>(row_lim + PT_ROWS);  // [2][rows]
   uint64_t* k_full = reinterpret_cast<uint64_t*>(sm + Sh::BAR_OFF);
-  uint64_t *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *s_full = v_empty + ST, *p_full = s_full + 2,
-           *o_done = p_full + 2, *drain = o_done + 2;
+  uint64_t *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + KST, *r_full = v_empty + KST, *r_empty = r_full + RST,
+           *s_full = r_empty + RST, *p_full = s_full + 2, *o_done = p_full + 2, *drain = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* r_have = reinterpret_cast<int*>(tmem_slot + 4);  // per copied stage: 16-slot pieces that are there
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Kv4Geo& g = a.g;
   if (tid == 0) {
-    for (int s = 0; s < ST; ++s) {
+    for (int s = 0; s < KST; ++s) {
       mbar_init(&k_full[s], PT_UNPACK);
       mbar_init(&v_full[s], PT_UNPACK);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_empty[s], 1);
+    }
+    for (int s = 0; s < RST; ++s) {
+      mbar_init(&r_full[s], 1);
+      mbar_init(&r_empty[s], PT_UNPACK);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
@@ -334,7 +370,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
     *abort_flag = 0;
     mbar_init_fence();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -350,13 +386,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
     if (a.b.status) atomicOr(a.b.status, 1);
     *abort_flag = 1;
   };
-  // One role's walk over the items of the share: body(p, tb, nt, v1, slot, kx,
-  // vx, flags) has one barrier of all roles in it (queries staged), and one
-  // follows it (everything of the item is over). j counts the tiles of this
-  // CTA, the pipelines' index.
+  // A wait of a whole warp.
+  auto wait = [&](uint64_t* b, unsigned ph) {
+    if (__all_sync(0xffffffffu, tg_wait(b, ph) && !*abort_flag)) return true;
+    fail();
+    return false;
+  };
+  // One role's walk over the items of the share. j counts the tiles of this
+  // CTA, the pipelines' index. The softmax, unpack and MMA roles meet at
+  // barrier 1 three times an item: queries staged, queries in TMEM, all over.
   int j = 0;
-  // barrier 1: the last three warps wait at the kernel's end, on barrier 0
-  auto bar = [] { asm volatile("bar.sync 1, %0;" ::"n"(PT_SOFT + PT_UNPACK + 32) : "memory"); };
+  constexpr int PT_MEET = PT_SOFT + PT_UNPACK + 32;
+  auto bar = [] { asm volatile("bar.sync 1, %0;" ::"n"(PT_MEET) : "memory"); };
   auto for_items = [&](auto body) {
     PtPlace p = {};
     if (r0 < r1) p = pt_find(a, BN, r0);
@@ -365,127 +406,146 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       const int tb = max(0, p.tile - PT_HEAD), nt = v1 - PT_HEAD - tb, slot = p.tile == 0 ? 1 : 0;
       f += v1 - p.tile;
       if (v1 <= PT_HEAD || nt <= 0) continue;
-      unsigned mk = 0u, mv = 0u, flags = 0u;
-      if (lane < RG_SPLIT) {
-        const int4 q = __ldcg(pt_ranges(a) + (int64_t(p.seq) * g.kvh + p.h) * RG_SPLIT + lane);
-        mk = unsigned(q.x), mv = unsigned(q.y), flags = unsigned(q.z);
-      }
-      mk = __reduce_max_sync(0xffffffffu, mk);
-      mv = __reduce_max_sync(0xffffffffu, mv);
-      flags = __reduce_or_sync(0xffffffffu, flags);
-      body(p, tb, nt, v1, slot, pt_exp(mk), pt_exp(mv), flags);
-      __syncwarp();
+      body(p, tb, nt, v1, slot);
       j += nt;
-      bar();
-      if (*abort_flag) break;
-      tg_fence_after();
+      __syncwarp();
+      // every role takes the same decision to leave, or one would wait for another
+      bool over = *abort_flag != 0;
+      if (warp != 17) {
+        over = pt_bar_any<PT_MEET>(1, over);
+        tg_fence_after();
+      }
+      if (over) break;
     }
   };
+  // Ranges of an item: exponents of the keys' and values' scales, flags.
+  auto ranges = [&](const PtPlace& p, int& kx, int& vx) {
+    unsigned mk = 0u, mv = 0u, flags = 0u;
+    if (lane < RG_SPLIT) {
+      const int4 q = __ldcg(pt_ranges(a) + (int64_t(p.seq) * g.kvh + p.h) * RG_SPLIT + lane);
+      mk = unsigned(q.x), mv = unsigned(q.y), flags = unsigned(q.z);
+    }
+    kx = pt_exp(__reduce_max_sync(0xffffffffu, mk));
+    vx = pt_exp(__reduce_max_sync(0xffffffffu, mv));
+    return __reduce_or_sync(0xffffffffu, flags);
+  };
 
-  if (warp < 4) {
+  if (warp < 8) {
+    // ---------------------------------------------------------- softmax ----
     pt_regs_inc<PT_REGS_SOFT>();
-    for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part, int kx, int vx, unsigned flags) {
+    const int hf = warp >> 2, row = tid & (PT_ROWS - 1), pair = 2 + (warp & 3);
+    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+    constexpr int HB = BN / 2;
+    for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part) {
+      int kx, vx;
+      const unsigned flags = ranges(p, kx, vx);
       const bool lost = (flags & 2u) != 0u, vnan = (flags & 1u) != 0u;
       bar();
-      // -------------------------------------------------------- softmax ----
-      const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
-      const float mul = row_mul[tid];
-      const int lim = row_lim[tid];
+      // the row's queries (this half's channels) from the key buffers to TMEM
+#pragma unroll
+      for (int c4 = 0; c4 < HD / 64; ++c4) {
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int ck = hf * (HD / 16) + c4 * 4 + k;  // 16-byte chunk of the row
+          kv4_ldv(sm + Sh::K_OFF + (ck >> 3) * (PT_ROWS * 128) + row * 128 + (((ck & 7) ^ (row & 7)) << 4),
+                  *reinterpret_cast<uint32_t(*)[4]>(w + 4 * k));
+        }
+        pt_st16(lanes + Sh::Q_COL + hf * (HD / 4) + c4 * 16, w);
+      }
+      pt_st_wait();
+      tg_fence_before();
+      const float mul = row_mul[row];
+      const int lim = row_lim[row];
       const int lim_lo = __reduce_min_sync(0xffffffffu, lim);
+      bar();
       float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int i = 0; i < nt && ok; ++i) {
+      for (int i = 0; i < nt; ++i) {
         const int jj = j + i, b = jj & 1;
-        const unsigned ph = (jj >> 1) & 1;
-        if (!__all_sync(0xffffffffu, tg_wait(&s_full[b], ph) && !*abort_flag)) { fail(); break; }
+        // the halves of a row leave together, or one would wait for the other
+        const bool dead = !wait(&s_full[b], (jj >> 1) & 1);
         tg_fence_after();
-        uint32_t s[BN];
-#pragma unroll
-        for (int q = 0; q < BN / 32; ++q) pt_ld32(lanes + Sh::S_COL + b * BN + q * 32, *reinterpret_cast<uint32_t(*)[32]>(s + q * 32));
+        uint32_t s[HB];
+        pt_ld32(lanes + Sh::S_COL + b * BN + hf * HB, s);
         tg_ld_wait();
-        const int s0 = (tb + i) * BN;
+        const int s0 = (tb + i) * BN + hf * HB;
 #pragma unroll
-        for (int e = 0; e < BN; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * mul);
-        if (s0 + BN - 1 > lim_lo) {
+        for (int e = 0; e < HB; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * mul);
+        if (s0 + HB - 1 > lim_lo) {
 #pragma unroll
-          for (int e = 0; e < BN; ++e)
+          for (int e = 0; e < HB; ++e)
             if (s0 + e > lim) s[e] = 0xff800000u;
         }
         if (lost) {  // slots of pages outside the pool
 #pragma unroll
-          for (int e = 0; e < BN; ++e)
+          for (int e = 0; e < HB; ++e)
             if ((e & 15) == 0 && s0 + e < p.len && !kv4_block(g, g.table, g.tstride, p.seq, p.h, s0 + e, nullptr)) {
 #pragma unroll
               for (int k = 0; k < 16; ++k) s[e + k] = 0xff800000u;
             }
         }
-        float mx = -INFINITY;
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < BN; ++e) mx = fmaxf(mx, __uint_as_float(s[e]));
-        const bool grow = mx > m + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
+        for (int e = 0; e < HB; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(s[e]));
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        // both halves have read S when the pair has met: P may take its place
+        tg_fence_before();
+        if (pt_bar_any(pair, mx > m + 8.f || dead)) {
+          xch[hf * PT_ROWS + row] = mx;
+          if (pt_bar_any(pair, dead)) break;
+          mx = fmaxf(mx, xch[(hf ^ 1) * PT_ROWS + row]);
+          const bool grow = mx > m + 8.f;
           const float mn = grow ? mx : m;
           const float al = m == -INFINITY ? (grow ? 0.f : 1.f) : pt_ex2(m - mn);
           m = mn;
           l *= al;
+          bool late = false;
           if (i > 0) {
             // every earlier product has landed before O is scaled
-            if (!__all_sync(0xffffffffu, tg_wait(&o_done[b ^ 1], ((jj - 1) >> 1) & 1))) {
-              fail();
-              ok = false;
-            }
+            late = !wait(&o_done[b ^ 1], ((jj - 1) >> 1) & 1);
             tg_fence_after();
 #pragma unroll 1
-            for (int q = 0; q < HD / 32; ++q) {
+            for (int q = 0; q < HD / 64; ++q) {
               uint32_t o[32];
-              pt_ld32(lanes + Sh::O_COL + q * 32, o);
+              pt_ld32(lanes + Sh::O_COL + hf * (HD / 2) + q * 32, o);
               tg_ld_wait();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
-              pt_st32(lanes + Sh::O_COL + q * 32, o);
+              pt_st32(lanes + Sh::O_COL + hf * (HD / 2) + q * 32, o);
             }
             pt_st_wait();
           }
+          if (pt_bar_any(pair, late)) break;  // and xch is free again
         }
-        const float mm = m == -INFINITY ? 0.f : m;
-        // the product that read this P buffer two tiles ago
-        if (i >= 2 && !__all_sync(0xffffffffu, tg_wait(&o_done[b], ((jj - 2) >> 1) & 1))) { fail(); break; }
         tg_fence_after();
-        const uint32_t pc = lanes + Sh::P_COL + b * (T * BN / 2);
-        float l0 = 0.f, l1 = 0.f;
+        const float mm = m == -INFINITY ? 0.f : m;
+        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t hi[HB / 2], lo[SPLIT ? HB / 2 : 1];
 #pragma unroll
-        for (int q = 0; q < BN / 32; ++q) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p0 = pt_ex2(__uint_as_float(s[q * 32 + 2 * e]) - mm), p1 = pt_ex2(__uint_as_float(s[q * 32 + 2 * e + 1]) - mm);
-            l0 += p0;
-            l1 += p1;
-            const __half2 hh = __floats2half2_rn(p0, p1);
-            hi[e] = pt_h2(hh);
-            if (SPLIT) {
-              const float2 ff = __half22float2(hh);
-              lo[e] = pt_h2(__floats2half2_rn(p0 - ff.x, p1 - ff.y));
-            }
+        for (int e = 0; e < HB / 2; ++e) {
+          const float p0 = pt_ex2(__uint_as_float(s[2 * e]) - mm), p1 = pt_ex2(__uint_as_float(s[2 * e + 1]) - mm);
+          l4[2 * (e & 1)] += p0;
+          l4[2 * (e & 1) + 1] += p1;
+          const __half2 hh = __floats2half2_rn(p0, p1);
+          hi[e] = pt_h2(hh);
+          if (SPLIT) {
+            const float2 ff = __half22float2(hh);
+            lo[e] = pt_h2(__floats2half2_rn(p0 - ff.x, p1 - ff.y));
           }
-          pt_st16(pc + q * 16, hi);
-          if (SPLIT) pt_st16(pc + BN / 2 + q * 16, lo);
         }
-        l += l0 + l1;
+        pt_st16(lanes + Sh::S_COL + b * BN + hf * 16, hi);
+        if (SPLIT) pt_st16(lanes + Sh::S_COL + b * BN + 32 + hf * 16, lo);
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
         pt_st_wait();
         tg_fence_before();
         mbar_arrive(&p_full[b]);
       }
       // ---- output: the last product has landed ----
-      const unsigned ci = unsigned(p.qt * PT_ROWS + tid);
-      const int tok = int(ci / unsigned(a.rep)), hq = p.h * a.rep + int(ci % unsigned(a.rep));
-      const int64_t row = p.row0 + tok;
-      const bool vo = kv4_vec(a.out, a.dt), vg = kv4_vec(a.gate, a.dt);
       const bool whole = tb == 0 && v1 == p.tiles;
       const int last = j + nt - 1;
-      const bool done = !*abort_flag && tg_wait(&o_done[last & 1], (last >> 1) & 1);
-      if (!done) fail();
+      wait(&o_done[last & 1], (last >> 1) & 1);
       tg_fence_after();
+      xch[hf * PT_ROWS + row] = l;
       // value groups that are NaN went in as zeros: a row that sees one has NaN there
       unsigned bad = 0u;
       if (vnan)
@@ -500,53 +560,93 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           }
         }
       __syncwarp();
+      pt_bar_any(pair, false);
+      l += xch[(hf ^ 1) * PT_ROWS + row];
       const bool none = l == 0.f;
-      const float inv = none ? 0.f : pt_pow2(-vx) / l;
-      float* part = pt_parts(a) + (int64_t(blockIdx.x) * 2 + slot_of_part) * pt_part_floats(HD);
-#pragma unroll 1
-      for (int q = 0; q < HD / 32; ++q) {
-        uint32_t o[32];
-        pt_ld32(lanes + Sh::O_COL + q * 32, o);
-        tg_ld_wait();
-        const bool nan = (bad >> (q * 32 / GROUP)) & 1;
-#pragma unroll
-        for (int e0 = 0; e0 < 32; e0 += 8) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {  // column order 0 4 1 5 2 6 3 7
-            const float x = __uint_as_float(o[e0 + (e & 3) * 2 + (e >> 2)]);
-            v[e] = nan ? NAN : none ? 0.f : x * (whole ? inv : pt_pow2(-vx));
-          }
-          const int ch = q * 32 + e0;
-          if (!whole) {
-            float4* d = reinterpret_cast<float4*>(part + 2 * PT_ROWS + int64_t(tid) * HD + ch);
-            d[0] = make_float4(v[0], v[1], v[2], v[3]);
-            d[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else if (tok < p.n) {
-            if (a.gate.p) {
-              float gt[8];
-              kv4_ld8(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch, vg, gt);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] *= kv4_sigmoid(gt[e]);
-            }
-            kv4_st8(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, vo, v);
-          }
+      const float fac = none ? 0.f : whole ? pt_pow2(-vx) / l : pt_pow2(-vx);
+      const unsigned ci0 = unsigned(p.qt * PT_ROWS + (warp & 3) * 32);
+      if (hf == 0) {
+        const unsigned ci = ci0 + lane;
+        const int tok = int(ci / unsigned(a.rep)), hq = p.h * a.rep + int(ci % unsigned(a.rep));
+        if (!whole) {
+          float* part = pt_parts(a) + (int64_t(blockIdx.x) * 2 + slot_of_part) * pt_part_floats(HD);
+          part[row] = l != l ? INFINITY : m;  // a NaN sum stays NaN when parts are joined
+          part[PT_ROWS + row] = l;
+        } else if (tok < p.n) {
+          pt_lse(a)[int64_t(p.row0 + tok) * a.heads + hq] = none ? -INFINITY : (m + log2f(l)) * P_LN2;
         }
       }
-      if (!whole) {
-        part[tid] = l != l ? INFINITY : m;  // a NaN sum stays NaN when parts are joined
-        part[PT_ROWS + tid] = l;
-      } else if (tok < p.n) {
-        pt_lse(a)[row * a.heads + hq] = none ? -INFINITY : (m + log2f(l)) * P_LN2;
+      // through shared memory (the key buffers: nothing reads them any more),
+      // 32 rows x 32 channels a warp, so that a row's channels are written together
+      float* scr = reinterpret_cast<float*>(sm + Sh::K_OFF) + warp * (32 * 33);
+      const bool vo = kv4_vec(a.out, a.dt), vg = kv4_vec(a.gate, a.dt);
+#pragma unroll 1
+      for (int q = 0; q < HD / 64; ++q) {
+        const int c0 = hf * (HD / 2) + q * 32;
+        uint32_t o[32];
+        pt_ld32(lanes + Sh::O_COL + c0, o);
+        tg_ld_wait();
+        const bool nan = (bad >> (c0 / GROUP)) & 1;
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {  // column order within eight: 0 4 1 5 2 6 3 7
+          const int ch = (e & ~7) + ((e & 7) >> 1) + 4 * (e & 1);
+          scr[lane * 33 + ch] = nan ? NAN : none ? 0.f : __uint_as_float(o[e]) * fac;
+        }
+        __syncwarp();
+        const int ch = (lane & 3) * 8;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int rr = k * 8 + (lane >> 2);
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = scr[rr * 33 + ch + e];
+          if (!whole) {
+            float* part = pt_parts(a) + (int64_t(blockIdx.x) * 2 + slot_of_part) * pt_part_floats(HD);
+            float4* d = reinterpret_cast<float4*>(part + 2 * PT_ROWS + ((warp & 3) * 32 + rr) * HD + c0 + ch);
+            d[0] = make_float4(v[0], v[1], v[2], v[3]);
+            d[1] = make_float4(v[4], v[5], v[6], v[7]);
+            continue;
+          }
+          const unsigned ci = ci0 + rr;
+          const int tok = int(ci / unsigned(a.rep)), hq = p.h * a.rep + int(ci % unsigned(a.rep));
+          if (tok >= p.n) continue;
+          const int64_t at = int64_t(p.row0 + tok);
+          if (a.gate.p) {
+            float gt[8];
+            kv4_ld8(a.gate.p, a.dt, at * a.gate.ts + hq * a.gate.hs + c0 + ch, vg, gt);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= kv4_sigmoid(gt[e]);
+          }
+          kv4_st8(a.out.p, a.dt, at * a.out.ts + hq * a.out.hs + c0 + ch, vo, v);
+        }
       }
       tg_fence_before();
     });
-  } else if (warp < 12) {
-    for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part, int kx, int vx, unsigned flags) {
-      // ------------------------------------------------------ unpacking ----
+    if (warp == 0) {  // what the join kernel has to do for this share
+      PtJoin d = {-1, -1, 0, 0, 0, 0, {0, 0}};
+      if (r0 < r1) {
+        const PtPlace p = pt_find(a, BN, r1 - 1);
+        const int64_t begin = r1 - 1 - p.tile, end = begin + p.tiles;
+        if (begin >= r0 && end > r1) {
+          const int nc = gridDim.x;
+          int first = blockIdx.x, last = blockIdx.x;
+          while (total * (first + 1) / nc <= begin + PT_HEAD) ++first;
+          while (last + 1 < nc && total * (last + 1) / nc < end) ++last;
+          if (first < last) d = PtJoin{first, last, p.row0, p.n, p.qt, p.h, {0, 0}};
+        }
+      }
+      if (lane == 0) pt_joins(a)[blockIdx.x] = d;
+    }
+  } else if (warp < 16) {
+    // -------------------------------------------------------- unpacking ----
+    const int ut = tid - PT_SOFT, r = ut & 7, t = ut >> 3;
+    for_items([&](const PtPlace& p, int tb, int nt, int v1, int) {
+      int kx, vx;
+      const unsigned flags = ranges(p, kx, vx);
       // queries: a warp a row, eight channels a lane, four rows at a time
       const bool vq = kv4_vec(a.q, a.dt), act = lane < HD / 8;
-      for (int rb = warp - 4; rb < PT_ROWS; rb += 32) {
+      for (int rb = warp - 8; rb < PT_ROWS; rb += 32) {
         float x[4][8];
         int tok[4];
 #pragma unroll
@@ -560,7 +660,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int r = rb + 8 * k;
+          const int qr = rb + 8 * k;
           float am = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[k][e]));
@@ -573,144 +673,116 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
             uint32_t *H = &hi.x, *L = &lo.x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // the order the codes come unpacked in
-              const float v0 = x[k][i] * up, v1f = x[k][i + 4] * up;
-              const __half2 hh = __floats2half2_rn(v0, v1f);
+              const float v0 = x[k][i] * up, v4 = x[k][i + 4] * up;
+              const __half2 hh = __floats2half2_rn(v0, v4);
               H[i] = pt_h2(hh);
               if (SPLIT) {
                 const float2 ff = __half22float2(hh);
-                L[i] = pt_h2(__floats2half2_rn(v0 - ff.x, v1f - ff.y));
+                L[i] = pt_h2(__floats2half2_rn(v0 - ff.x, v4 - ff.y));
               }
             }
-            uint8_t* d = sm + Sh::Q_OFF + (lane >> 3) * (PT_ROWS * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
-            *reinterpret_cast<uint4*>(d) = hi;
-            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::QB) = lo;
+            const int off = (lane >> 3) * (PT_ROWS * 128) + qr * 128 + (((lane & 7) ^ (qr & 7)) << 4);
+            *reinterpret_cast<uint4*>(sm + Sh::K_OFF + off) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(sm + Sh::Q_OFF + off) = lo;
           }
           if (lane == 0) {
-            row_mul[r] = a.scale * P_LOG2E * pt_pow2(-ex) * pt_pow2(-kx);
-            row_lim[r] = tok[k] < p.n ? p.len - p.n + tok[k] : p.len - 1;
+            row_mul[qr] = a.scale * P_LOG2E * pt_pow2(-ex) * pt_pow2(-kx);
+            row_lim[qr] = tok[k] < p.n ? p.len - p.n + tok[k] : p.len - 1;
           }
         }
       }
       fence_proxy_async();
       bar();
-      // ------------------------------------------------------ unpacking ----
-      // thread: unit r of slots t0 and t0 + 32 (of the tile), every 64-channel block
-      constexpr int NS = BN / 32;
-      const int ut = tid - PT_SOFT, r = ut & 7, t0 = ut >> 3;
+      bar();
+      // a thread: unit r of slots t and t + 32 of the tile, every 64-channel block
       const PtScale ks(kx), vs(vx);
       const bool vnan = (flags & 1u) != 0u;
-      uint32_t kw[NS][NW], vw[NS][NW], kp[NS][NG], vp[NS][NG];
-      int pg[NS];
-      auto page_of = [&](int i, int q) {
-        const int s = (tb + i) * BN + t0 + 32 * q;
-        return i < nt && s < p.len ? __ldg(g.table + p.seq * g.tstride + (s >> g.pshift)) : -1;
-      };
-      const int nblk = g.page / g.seg;
-      auto load = [&](int i, uint32_t (&kwr)[NS][NW], uint32_t (&vwr)[NS][NW], uint32_t (&kpr)[NS][NG], uint32_t (&vpr)[NS][NG]) {
-#pragma unroll
-        for (int q = 0; q < NS; ++q) {
-          const int s = (tb + i) * BN + t0 + 32 * q, t = s & (g.seg - 1);
-          if (unsigned(pg[q]) < unsigned(g.npages)) {
-            const uint8_t* blk = g.pages + pg[q] * g.page_bytes + int64_t(p.h * nblk + (s & (g.page - 1)) / g.seg) * g.blk;
-            const int off = t * (HD / 2) + ((r ^ kv4_swz(HD, t)) * (HD / 16)), po = g.seg * (HD / 2) + t * NG * 4;
-            kv4_ldv(blk + off, kwr[q]);
-            kv4_ldv(blk + g.blk / 2 + off, vwr[q]);
-            kv4_ldv(blk + po, kpr[q]);
-            kv4_ldv(blk + g.blk / 2 + po, vpr[q]);
-          } else {
-            // past the sequence, or a page outside the pool: zeros (the
-            // softmax gives such slots no weight)
-#pragma unroll
-            for (int w = 0; w < NW; ++w) kwr[q][w] = vwr[q][w] = 0u;
-#pragma unroll
-            for (int w = 0; w < NG; ++w) kpr[q][w] = vpr[q][w] = 0u;
-          }
-        }
-      };
-#pragma unroll
-      for (int q = 0; q < NS; ++q) pg[q] = page_of(0, q);
-      load(0, kw, vw, kp, vp);
-#pragma unroll
-      for (int q = 0; q < NS; ++q) pg[q] = page_of(1, q);
+      const int uo = t * (HD / 2) + ((r ^ kv4_swz(HD, t)) * (HD / 16)), po = Sh::CODES + t * NG * 4;
+      const int d0 = t * 128 + ((r ^ (t & 7)) << 4);
       for (int i = 0; i < nt; ++i) {
-        const int jj = j + i, st = jj % ST;
-        const unsigned ph = (jj / ST) & 1;
-        uint32_t kw2[NS][NW], vw2[NS][NW], kp2[NS][NG], vp2[NS][NG];
-        if (i + 1 < nt) load(i + 1, kw2, vw2, kp2, vp2);
+        const int jj = j + i, st = jj % KST;
+        const unsigned ph = (jj / KST) & 1;
+        const uint8_t* raw[2];
+        bool there[2];
+        if (!wait(&k_empty[st], ph ^ 1)) break;
 #pragma unroll
-        for (int q = 0; q < NS; ++q) pg[q] = page_of(i + 2, q);
-        if (!tg_wait(&k_empty[st], ph ^ 1)) { fail(); break; }
-        if (*abort_flag) break;
+        for (int q = 0; q < 2; ++q) {
+          const int rs = (2 * jj + q) % RST;
+          if (!wait(&r_full[rs], ((2 * jj + q) / RST) & 1)) break;
+          raw[q] = sm + Sh::R_OFF + rs * Sh::RAW;
+          there[q] = (tb + i) * BN + q * 32 + t < p.len && ((r_have[rs] >> (t >> 4)) & 1);
+          uint32_t w[NW], pr[NG];
+          kv4_ldv(raw[q] + uo, w);
+          kv4_ldv(raw[q] + po, pr);
+          uint8_t* d = sm + Sh::K_OFF + st * (T * Sh::KB) + q * (32 * 128) + d0;
 #pragma unroll
-        for (int q = 0; q < NS; ++q) {
-          const int t = t0 + 32 * q;
-          uint8_t* d = sm + Sh::K_OFF + st * (T * Sh::KB) + t * 128 + ((r ^ (t & 7)) << 4);
-#pragma unroll
-          for (int w = 0; w < NW; ++w) {
+          for (int k = 0; k < NW; ++k) {
+            // past the sequence, or a page outside the pool: zeros (the softmax gives such slots no weight)
+            const uint32_t sb = there[q] ? pr[k * 64 / GROUP] : 0u;
             uint4 hi, lo;
-            pt_unpack<SPLIT>(kw[q][w], ks.of(kp[q][w * 64 / GROUP]), hi, lo);
-            *reinterpret_cast<uint4*>(d + w * (BN * 128)) = hi;
-            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + w * (BN * 128)) = lo;
+            pt_unpack<SPLIT>(w[k], ks.of(sb), hi, lo);
+            *reinterpret_cast<uint4*>(d + k * (BN * 128)) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + k * (BN * 128)) = lo;
           }
         }
+        if (*abort_flag) break;
         fence_proxy_async();
         mbar_arrive(&k_full[st]);
-        if (!tg_wait(&v_empty[st], ph ^ 1)) { fail(); break; }
-        if (*abort_flag) break;
+        if (!wait(&v_empty[st], ph ^ 1)) break;
 #pragma unroll
-        for (int q = 0; q < NS; ++q) {
-          const int t = t0 + 32 * q;
-          uint8_t* d = sm + Sh::V_OFF + st * (T * Sh::KB) + t * 128 + ((r ^ (t & 7)) << 4);
+        for (int q = 0; q < 2; ++q) {
+          uint32_t w[NW], pr[NG];
+          kv4_ldv(raw[q] + Sh::CODES + Sh::PARAMS + uo, w);
+          kv4_ldv(raw[q] + Sh::CODES + Sh::PARAMS + po, pr);
+          mbar_arrive(&r_empty[(2 * jj + q) % RST]);
+          uint8_t* d = sm + Sh::V_OFF + st * (T * Sh::KB) + q * (32 * 128) + d0;
 #pragma unroll
-          for (int w = 0; w < NW; ++w) {
-            uint32_t sb = vp[q][w * 64 / GROUP];
+          for (int k = 0; k < NW; ++k) {
+            uint32_t sb = there[q] ? pr[k * 64 / GROUP] : 0u;
             if (vnan && (!(fabsf(kv4_param(sb).x) < INFINITY) || !(fabsf(kv4_param(sb).y) < INFINITY))) sb = 0u;
             uint4 hi, lo;
-            pt_unpack<SPLIT>(vw[q][w], vs.of(sb), hi, lo);
-            *reinterpret_cast<uint4*>(d + w * (BN * 128)) = hi;
-            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + w * (BN * 128)) = lo;
+            pt_unpack<SPLIT>(w[k], vs.of(sb), hi, lo);
+            *reinterpret_cast<uint4*>(d + k * (BN * 128)) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + k * (BN * 128)) = lo;
           }
         }
         fence_proxy_async();
         mbar_arrive(&v_full[st]);
-#pragma unroll
-        for (int q = 0; q < NS; ++q) {
-#pragma unroll
-          for (int w = 0; w < NW; ++w) kw[q][w] = kw2[q][w], vw[q][w] = vw2[q][w];
-#pragma unroll
-          for (int w = 0; w < NG; ++w) kp[q][w] = kp2[q][w], vp[q][w] = vp2[q][w];
-        }
       }
     });
   } else {
-    pt_regs_dec<PT_REGS_MMA>();
-    if (warp == 12)
-      for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part, int kx, int vx, unsigned flags) {
+    pt_regs_dec<PT_REGS_ISSUE>();
+    if (warp == 16) {
+      // ------------------------------------------------------ MMA issue ----
+      // The warp stays together, so that descriptors live in uniform
+      // registers; one elected lane issues.
+      constexpr uint32_t ids = pt_idesc(BN, false), idp = pt_idesc(HD, true);
+      for_items([&](const PtPlace&, int, int nt, int, int) {
         bar();
-        // ---------------------------------------------------- MMA issue ----
-        // The warp stays together, so that descriptors live in uniform
-        // registers; one elected lane issues.
-        constexpr uint32_t ids = pt_idesc(BN, false), idp = pt_idesc(HD, true);
-        auto wait = [&](uint64_t* b, unsigned ph) {
-          if (__all_sync(0xffffffffu, tg_wait(b, ph) && !*abort_flag)) return true;
-          fail();
-          return false;
-        };
+        bar();
+        tg_fence_after();
         auto qk = [&](int i) {
-          const int jj = j + i, st = jj % ST, b = jj & 1;
-          if (!wait(&k_full[st], (jj / ST) & 1)) return false;
+          const int jj = j + i, st = jj % KST, b = jj & 1;
+          if (!wait(&k_full[st], (jj / KST) & 1)) return false;
           tg_fence_after();
-          const uint64_t qd = tg_desc(smem_u32(sm + Sh::Q_OFF)), kd = tg_desc(smem_u32(sm + Sh::K_OFF + st * (T * Sh::KB)));
+          const uint64_t kd = tg_desc(smem_u32(sm + Sh::K_OFF + st * (T * Sh::KB)));
           const uint32_t d = tmem + Sh::S_COL + b * BN;
           if (pt_elect()) {
-#pragma unroll 1
-            for (int tm = 0; tm < (SPLIT ? 3 : 1); ++tm)
+#pragma unroll
+            for (int w = 0; w < NW; ++w)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)  // 16 channels: 32 bytes of the 128-byte rows
+                pt_mma_ts(d, tmem + Sh::Q_COL + w * 32 + k * 8, kd + ((w * (BN * 128) + k * 32) >> 4), ids, w + k > 0);
+            if (SPLIT) {
+              const uint64_t qd = tg_desc(smem_u32(sm + Sh::Q_OFF));
 #pragma unroll
               for (int w = 0; w < NW; ++w)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)  // 16 channels: 32 bytes of the 128-byte rows
-                  pt_mma_ss(d, qd + (((tm == 1 ? Sh::QB : 0) + w * (PT_ROWS * 128) + k * 32) >> 4),
-                            kd + (((tm == 2 ? Sh::KB : 0) + w * (BN * 128) + k * 32) >> 4), ids, tm + w + k > 0);
+                for (int k = 0; k < 4; ++k) {
+                  pt_mma_ts(d, tmem + Sh::Q_COL + w * 32 + k * 8, kd + ((Sh::KB + w * (BN * 128) + k * 32) >> 4), ids, true);
+                  pt_mma_ss(d, qd + ((w * (PT_ROWS * 128) + k * 32) >> 4), kd + ((w * (BN * 128) + k * 32) >> 4), ids, true);
+                }
+            }
             tg_commit(&s_full[b]);
             tg_commit(&k_empty[st]);
           }
@@ -719,28 +791,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         };
         bool ok = qk(0);
         for (int i = 0; i < nt && ok; ++i) {
+          // S of tile i + 1 takes the columns P of tile i - 1 was read from: products complete in order
           if (i + 1 < nt) ok = qk(i + 1);
-          const int jj = j + i, st = jj % ST, b = jj & 1;
-          if (!ok || !wait(&v_full[st], (jj / ST) & 1) || !wait(&p_full[b], (jj >> 1) & 1)) break;
+          const int jj = j + i, st = jj % KST, b = jj & 1;
+          if (!ok || !wait(&v_full[st], (jj / KST) & 1) || !wait(&p_full[b], (jj >> 1) & 1)) break;
           tg_fence_after();
           const uint64_t vd = pt_desc_n(smem_u32(sm + Sh::V_OFF + st * (T * Sh::KB)), BN * 128);
-          const uint32_t pc = tmem + Sh::P_COL + b * (T * BN / 2);
+          const uint32_t pc = tmem + Sh::S_COL + b * BN;
           if (pt_elect()) {
-#pragma unroll 1
-            for (int tm = 0; tm < (SPLIT ? 3 : 1); ++tm)
 #pragma unroll
-              for (int k = 0; k < BN / 16; ++k)
-                pt_mma_ts(tmem + Sh::O_COL, pc + (tm == 1 ? BN / 2 : 0) + k * 8, vd + (((tm == 2 ? Sh::KB : 0) + k * 2048) >> 4), idp,
-                          tm + k > 0 || i > 0);
+            for (int k = 0; k < BN / 16; ++k) {
+              pt_mma_ts(tmem + Sh::O_COL, pc + k * 8, vd + ((k * 2048) >> 4), idp, k > 0 || i > 0);
+              if (SPLIT) {
+                pt_mma_ts(tmem + Sh::O_COL, pc + 32 + k * 8, vd + ((k * 2048) >> 4), idp, true);
+                pt_mma_ts(tmem + Sh::O_COL, pc + k * 8, vd + ((Sh::KB + k * 2048) >> 4), idp, true);
+              }
+            }
             tg_commit(&o_done[b]);
             tg_commit(&v_empty[st]);
           }
           __syncwarp();
         }
       });
+    } else if (warp == 17) {
+      // --------------------------------------------------- bulk copies ----
+      // A stage is 32 slots: keys, their params, values and theirs of each
+      // block piece by a lane of its own.
+      const int nblk = g.page / g.seg, pc = min(g.seg, PT_RAW), np = PT_RAW / pc;  // slots of a piece, pieces
+      int issued = 0;
+      for_items([&](const PtPlace& p, int tb, int nt, int, int) {
+        const int piece = lane >> 2, part = lane & 3;
+        const int bytes = part & 1 ? pc * NG * 4 : pc * (HD / 2);
+        for (int i = 0; i < 2 * nt; ++i, ++issued) {
+          const int jj = 2 * j + i, rs = jj % RST;
+          if (!wait(&r_empty[rs], ((jj / RST) & 1) ^ 1)) break;
+          const int s = tb * BN + i * PT_RAW + piece * pc;
+          const bool want = piece < np && s < p.len;
+          const int pg = want ? __ldg(g.table + p.seq * g.tstride + (s >> g.pshift)) : -1;
+          const bool on = unsigned(pg) < unsigned(g.npages);
+          if (want && !on && a.b.status) atomicOr(a.b.status, KV4_BAD);
+          const unsigned have = __ballot_sync(0xffffffffu, on);
+          int bits = 0;  // by 16 slots
+          for (int k = 0; k < np; ++k)
+            if ((have >> (4 * k)) & 1) bits |= (pc == 16 ? 1 : 3) << k;
+          if (lane == 0) {
+            r_have[rs] = bits;
+            mbar_expect_tx(&r_full[rs], unsigned(__popc(have)) / 4 * unsigned(2 * pc * (HD / 2 + NG * 4)));
+          }
+          __syncwarp();
+          if (on) {
+            const uint8_t* blk = g.pages + pg * g.page_bytes + int64_t(p.h * nblk + (s & (g.page - 1)) / g.seg) * g.blk +
+                                 (part >> 1) * (g.blk / 2) + (part & 1) * (g.seg * (HD / 2));
+            uint8_t* d = sm + Sh::R_OFF + rs * Sh::RAW + (part >> 1) * (Sh::CODES + Sh::PARAMS) + (part & 1) * Sh::CODES;
+            bulk_g2s_keep(d + piece * bytes, blk + ((s & (g.seg - 1)) / pc) * bytes, unsigned(bytes), &r_full[rs]);
+          }
+        }
+      });
+      if (*abort_flag)  // copies in flight land before the CTA may end
+        for (int i = max(0, issued - RST); i < issued; ++i) tg_wait(&r_full[i % RST], (i / RST) & 1);
+    }
   }
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     if (*abort_flag) {
       if (pt_elect()) tg_commit(drain);  // the products still in flight
       __syncwarp();
@@ -751,56 +863,54 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
   }
 }
 
-// Joins the parts of the item that begins in share x and goes on: one block per
-// (share, 16 rows), a thread a channel.
+// Joins the parts of the item that begins in share x and goes on: a warp a row.
 template <int HD>
-__global__ void __launch_bounds__(HD) k_kv4_prompt_join(const Kv4AttnArgs a, int bn) {
-  const int nc = PT_GRID, x = blockIdx.x;
-  const int64_t total = pt_total(a, bn);
-  const int64_t r0 = total * x / nc, r1 = total * (x + 1) / nc;
-  PtPlace p = {};
-  if (r0 < r1) p = pt_find(a, bn, r1 - 1);
-  const int64_t begin = r1 - 1 - p.tile, end = begin + p.tiles;
+__global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4AttnArgs a) {
   pdl_wait();
-  if (r0 == r1 || begin < r0 || end <= r1) return;
-  int last = x, one = x;
-  while (last + 1 < nc && total * (last + 1) / nc < end) ++last;
-  while (total * (one + 1) / nc <= begin + PT_HEAD) ++one;
-  if (one == last) return;  // all its tiles in one share: written there
-  const float* parts = pt_parts(a);
-  auto has = [&](int i) {  // tiles of the item itself in share i
-    return max(begin + PT_HEAD, total * i / nc) < min(end, total * (i + 1) / nc);
-  };
-  for (int r = blockIdx.y * 16; r < blockIdx.y * 16 + 16; ++r) {
-    const unsigned ci = unsigned(p.qt * PT_ROWS + r);
-    const int tok = int(ci / unsigned(a.rep)), hq = p.h * a.rep + int(ci % unsigned(a.rep));
-    if (tok >= p.n) break;
-    float M = -INFINITY, L = 0.f, v = 0.f;
-    for (int i = one; i <= last; ++i) {
-      const float* q = parts + (int64_t(i) * 2 + (i == x ? 1 : 0)) * pt_part_floats(HD);
-      if (has(i)) M = fmaxf(M, __ldcg(q + r));
-    }
-    for (int i = one; i <= last; ++i) {
-      if (!has(i)) continue;
-      const float* q = parts + (int64_t(i) * 2 + (i == x ? 1 : 0)) * pt_part_floats(HD);
-      const float mi = __ldcg(q + r), f = mi == -INFINITY ? 0.f : pt_ex2(mi - M), o = __ldcg(q + 2 * PT_ROWS + int64_t(r) * HD + threadIdx.x);
-      L = fmaf(__ldcg(q + PT_ROWS + r), f, L);
-      v = fmaf(o, f, v);
-    }
-    v = L == 0.f ? v : v / L;  // an empty row: zeros, or NaN as its parts say
-    const int64_t row = p.row0 + tok;
-    if (a.gate.p) v *= kv4_sigmoid(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + threadIdx.x));
-    kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + threadIdx.x, v);
-    if (threadIdx.x == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * P_LN2;
+  const int x = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const PtJoin d = pt_joins(a)[x];
+  if (d.first < 0) return;
+  const unsigned ci = unsigned(d.qt * PT_ROWS + r);
+  const int tok = int(ci / unsigned(a.rep)), hq = d.h * a.rep + int(ci % unsigned(a.rep));
+  if (tok >= d.n) return;
+  const int64_t total = pt_total(a, PT_BN), step = pt_part_floats(HD);
+  auto part = [&](int i) { return pt_parts(a) + (int64_t(i) * 2 + (i == x ? 1 : 0)) * step; };
+  // shares without tiles (fewer tiles than CTAs) have no part
+  auto has = [&](int i) { return i == d.first || total * i / PT_GRID < total * (i + 1) / PT_GRID; };
+  float M = -INFINITY, L = 0.f;
+  for (int i = d.first + lane; i <= d.last; i += 32)
+    if (has(i)) M = fmaxf(M, __ldcg(part(i) + r));
+  M = warp_max(M);
+  constexpr int E = HD / 32;
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll 4
+  for (int i = d.first; i <= d.last; ++i) {
+    if (!has(i)) continue;
+    const float* q = part(i);
+    const float mi = __ldcg(q + r), f = mi == -INFINITY ? 0.f : pt_ex2(mi - M);
+    L = fmaf(__ldcg(q + PT_ROWS + r), f, L);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = fmaf(__ldcg(q + 2 * PT_ROWS + int64_t(r) * HD + e * 32 + lane), f, v[e]);
   }
+  const int64_t row = d.row0 + tok;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int ch = e * 32 + lane;
+    float o = L == 0.f ? v[e] : v[e] / L;  // an empty row: zeros
+    if (a.gate.p) o *= kv4_sigmoid(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch));
+    kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, o);
+  }
+  if (lane == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * P_LN2;
 }
 
 template <int HD, int GROUP, bool SPLIT>
 void run(const Kv4AttnArgs& a, cudaStream_t st) {
-  using Sh = PtShape<HD, SPLIT>;
+  using Sh = PtShape<HD, GROUP, SPLIT>;
   launch(k_kv4_range, dim3(RG_SPLIT, a.b.nseq * a.g.kvh), dim3(256), 0, st, false, a);
   launch(k_kv4_prompt<HD, GROUP, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS), Sh::TOTAL, st, true, a);
-  launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 16), dim3(HD), 0, st, true, a, int(Sh::BN));
+  launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(256), 0, st, true, a);
 }
 
 template <int HD, int GROUP>
@@ -812,7 +922,7 @@ void run_dt(const Kv4AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int64_t kv4_prompt_work(const Kv4Geo& g, const Kv4Batch& b, int heads) {
-  return pt_lse_bytes(b.total, heads) + pt_range_bytes(b.nseq, g.kvh) + int64_t(PT_GRID) * 2 * pt_part_floats(g.hd) * 4;
+  return pt_lse_bytes(b.total, heads) + pt_range_bytes(b.nseq, g.kvh) + PT_GRID * int64_t(sizeof(PtJoin)) + int64_t(PT_GRID) * 2 * pt_part_floats(g.hd) * 4;
 }
 
 void launch_kv4_prompt(const Kv4AttnArgs& a, cudaStream_t st) {
