@@ -14,8 +14,8 @@
 // (hi hi + lo hi + hi lo), f32 accumulators throughout.
 //
 // Warps: 0-7 softmax and output (two threads a row, half of the tile's slots
-// each), 8-15 unpacking, 16 MMA issue and TMEM, 17 bulk copies of the cache's
-// bytes into a ring of 32-slot stages. Q stands in TMEM (its low terms in shared
+// each), 8-23 unpacking, 24 MMA issue and TMEM, 25 bulk copies of the cache's
+// bytes into a ring of stages (a tile's keys, then its values). Q stands in TMEM (its low terms in shared
 // memory), S and P share columns and are double-buffered, so Q K^T of the next
 // tile runs during the softmax of this one; the running maximum moves only
 // when it has grown by 2^8, so O in TMEM is rarely touched. Bound: the tensor
@@ -39,14 +39,13 @@ namespace {
 
 constexpr int PT_ROWS = 128;
 constexpr int PT_BN = 64;                               // slots of a tile
-constexpr int PT_RAW = 32;                              // slots of a copied stage
 constexpr int PT_GRID = 148;
-constexpr int PT_SOFT = 256, PT_UNPACK = 256;           // threads of the softmax and unpack roles
+constexpr int PT_SOFT = 256, PT_UNPACK = 512;           // threads of the softmax and unpack roles
 constexpr int PT_THREADS = PT_SOFT + PT_UNPACK + 128;   // and a warpgroup that issues MMAs and copies
-// Registers a thread: 96 at launch; the last warpgroup's spare ones go to the
-// softmax (256 x 104 + 256 x 96 + 128 x 80 = 640 x 96).
-constexpr int PT_REGS_SOFT = 104, PT_REGS_ISSUE = 80;
-constexpr int PT_HEAD = 4;                              // cost of an item beside its tiles, in tiles
+constexpr int PT_MMA = (PT_SOFT + PT_UNPACK) / 32, PT_COPY = PT_MMA + 1;  // warps
+// Registers a thread: 72 at launch, then 256 x 96 + 512 x 64 + 128 x 56 (= 896 x 72).
+constexpr int PT_REGS_SOFT = 96, PT_REGS_UNPACK = 64, PT_REGS_ISSUE = 56;
+constexpr int PT_HEAD = 12;                             // cost of an item beside its tiles, in tiles
 constexpr int RG_SPLIT = 16;                            // blocks a (sequence, head) of the range kernel
 constexpr float P_LOG2E = 1.4426950408889634f, P_LN2 = 0.6931471805599453f;
 
@@ -57,7 +56,7 @@ struct PtShape {
   static constexpr int RST = HD == 256 && SPLIT ? 3 : 4;   // copied stages
   static constexpr int QB = PT_ROWS * HD * 2;              // bytes of one term of Q
   static constexpr int KB = PT_BN * HD * 2;                // of one term of a tile's keys (values)
-  static constexpr int CODES = PT_RAW * HD / 2, PARAMS = PT_RAW * 4 * (HD / GROUP), RAW = 2 * (CODES + PARAMS);
+  static constexpr int RAW = PT_BN * (HD / 2 + 4 * (HD / GROUP));  // bytes of a tile's keys (values) as they are held
   // low terms of Q, keys (first the high terms of Q, on their way to TMEM), values, copied stages
   static constexpr int SCR = 8 * 32 * 33 * 4;              // the output's scratch, over the key buffers
   static constexpr int KS = KST * T * KB > SCR ? KST * T * KB : (SCR + 1023) / 1024 * 1024;
@@ -125,6 +124,18 @@ __device__ __forceinline__ void pt_st16(uint32_t t, const uint32_t* r) {
       : "memory");
 }
 __device__ __forceinline__ void pt_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Pipeline wait: polls (hand-offs come within a tile's time), and gives up
+// after 2^32 cycles, over two seconds. The bound goes by the SM's clock: a read
+// of the global timer costs more than most waits.
+__device__ __forceinline__ bool pt_wait(uint64_t* b, unsigned parity) {
+  if (mbar_try(b, parity)) return true;
+  const long long t0 = clock64();
+  do {
+    for (int i = 0; i < 256; ++i)
+      if (mbar_try(b, parity)) return true;
+  } while (clock64() - t0 < (1ll << 32));
+  return false;
+}
 // One lane of a converged warp.
 __device__ __forceinline__ bool pt_elect() {
   uint32_t ok;
@@ -370,7 +381,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
     *abort_flag = 0;
     mbar_init_fence();
   }
-  if (warp == 16) {
+  if (warp == PT_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -388,7 +399,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
   };
   // A wait of a whole warp.
   auto wait = [&](uint64_t* b, unsigned ph) {
-    if (__all_sync(0xffffffffu, tg_wait(b, ph) && !*abort_flag)) return true;
+    if (__all_sync(0xffffffffu, pt_wait(b, ph) && !*abort_flag)) return true;
     fail();
     return false;
   };
@@ -411,7 +422,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       __syncwarp();
       // every role takes the same decision to leave, or one would wait for another
       bool over = *abort_flag != 0;
-      if (warp != 17) {
+      if (warp != PT_COPY) {
         over = pt_bar_any<PT_MEET>(1, over);
         tg_fence_after();
       }
@@ -469,8 +480,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         pt_ld32(lanes + Sh::S_COL + b * BN + hf * HB, s);
         tg_ld_wait();
         const int s0 = (tb + i) * BN + hf * HB;
-#pragma unroll
-        for (int e = 0; e < HB; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * mul);
         if (s0 + HB - 1 > lim_lo) {
 #pragma unroll
           for (int e = 0; e < HB; ++e)
@@ -487,7 +496,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int e = 0; e < HB; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(s[e]));
-        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
         // both halves have read S when the pair has met: P may take its place
         tg_fence_before();
         if (pt_bar_any(pair, mx > m + 8.f || dead)) {
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         uint32_t hi[HB / 2], lo[SPLIT ? HB / 2 : 1];
 #pragma unroll
         for (int e = 0; e < HB / 2; ++e) {
-          const float p0 = pt_ex2(__uint_as_float(s[2 * e]) - mm), p1 = pt_ex2(__uint_as_float(s[2 * e + 1]) - mm);
+          const float p0 = pt_ex2(fmaf(__uint_as_float(s[2 * e]), mul, -mm)), p1 = pt_ex2(fmaf(__uint_as_float(s[2 * e + 1]), mul, -mm));
           l4[2 * (e & 1)] += p0;
           l4[2 * (e & 1) + 1] += p1;
           const __half2 hh = __floats2half2_rn(p0, p1);
@@ -638,20 +647,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       }
       if (lane == 0) pt_joins(a)[blockIdx.x] = d;
     }
-  } else if (warp < 16) {
+  } else if (warp < PT_MMA) {
     // -------------------------------------------------------- unpacking ----
+    pt_regs_dec<PT_REGS_UNPACK>();
     const int ut = tid - PT_SOFT, r = ut & 7, t = ut >> 3;
     for_items([&](const PtPlace& p, int tb, int nt, int v1, int) {
       int kx, vx;
       const unsigned flags = ranges(p, kx, vx);
-      // queries: a warp a row, eight channels a lane, four rows at a time
+      // queries: a warp a row, eight channels a lane, two rows at a time; a
+      // negative scale goes into them, so that the rows' factors are positive
       const bool vq = kv4_vec(a.q, a.dt), act = lane < HD / 8;
-      for (int rb = warp - 8; rb < PT_ROWS; rb += 32) {
-        float x[4][8];
-        int tok[4];
+      const float sgn = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+      for (int rb = warp - PT_SOFT / 32; rb < PT_ROWS; rb += 2 * PT_UNPACK / 32) {
+        float x[2][8];
+        int tok[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const unsigned ci = unsigned(p.qt * PT_ROWS + rb + 8 * k);
+        for (int k = 0; k < 2; ++k) {
+          const unsigned ci = unsigned(p.qt * PT_ROWS + rb + PT_UNPACK / 32 * k);
           tok[k] = int(ci / unsigned(a.rep));
           const int hq = p.h * a.rep + int(ci - unsigned(tok[k]) * unsigned(a.rep));
 #pragma unroll
@@ -659,15 +671,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           if (tok[k] < p.n && act) kv4_ld8(a.q.p, a.dt, int64_t(p.row0 + tok[k]) * a.q.ts + hq * a.q.hs + lane * 8, vq, x[k]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int qr = rb + 8 * k;
+        for (int k = 0; k < 2; ++k) {
+          const int qr = rb + PT_UNPACK / 32 * k;
           float am = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[k][e]));
           am = warp_max(am);
           int ex = am > 0.f && am < INFINITY ? 12 - (int(__float_as_uint(am) >> 23) - 127) : 0;
           ex = max(-60, min(60, ex));
-          const float up = pt_pow2(ex);
+          const float up = pt_pow2(ex) * sgn;
           if (act) {
             uint4 hi, lo;
             uint32_t *H = &hi.x, *L = &lo.x;
@@ -686,7 +698,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
             if (SPLIT) *reinterpret_cast<uint4*>(sm + Sh::Q_OFF + off) = lo;
           }
           if (lane == 0) {
-            row_mul[qr] = a.scale * P_LOG2E * pt_pow2(-ex) * pt_pow2(-kx);
+            row_mul[qr] = sgn == 0.f ? 1.f : fabsf(a.scale) * P_LOG2E * pt_pow2(-ex) * pt_pow2(-kx);
             row_lim[qr] = tok[k] < p.n ? p.len - p.n + tok[k] : p.len - 1;
           }
         }
@@ -694,65 +706,46 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       fence_proxy_async();
       bar();
       bar();
-      // a thread: unit r of slots t and t + 32 of the tile, every 64-channel block
-      const PtScale ks(kx), vs(vx);
+      // a thread: unit r of slot t of the tile, every 64-channel block; the
+      // keys, then the values, by the same code (the instruction cache holds
+      // it beside the softmax's)
       const bool vnan = (flags & 1u) != 0u;
-      const int uo = t * (HD / 2) + ((r ^ kv4_swz(HD, t)) * (HD / 16)), po = Sh::CODES + t * NG * 4;
+      const int half = g.blk / 2, lseg = g.seg == 16 ? 4 : g.seg == 32 ? 5 : 6, in = t & (g.seg - 1), base = (t >> lseg) * half;
+      const int uo = base + in * (HD / 2) + ((r ^ kv4_swz(HD, t)) * (HD / 16)), po = base + g.seg * (HD / 2) + in * NG * 4;
       const int d0 = t * 128 + ((r ^ (t & 7)) << 4);
-      for (int i = 0; i < nt; ++i) {
-        const int jj = j + i, st = jj % KST;
-        const unsigned ph = (jj / KST) & 1;
-        const uint8_t* raw[2];
-        bool there[2];
-        if (!wait(&k_empty[st], ph ^ 1)) break;
+#pragma unroll 1
+      for (int i = 0; i < 2 * nt; ++i) {
+        const int jj = j + (i >> 1), st = jj % KST, kv = i & 1, ss = 2 * j + i, rs = ss % RST;
+        if (!wait((kv ? v_empty : k_empty) + st, ((jj / KST) & 1) ^ 1) || !wait(&r_full[rs], (ss / RST) & 1)) break;
+        const uint8_t* raw = sm + Sh::R_OFF + rs * Sh::RAW;
+        uint8_t* d = sm + (kv ? Sh::V_OFF : Sh::K_OFF) + st * (T * Sh::KB) + d0;
+        const PtScale sc(kv ? vx : kx);
+        uint32_t w[NW], pr[NG];
+        kv4_ldv(raw + uo, w);
+        kv4_ldv(raw + po, pr);
+        // past the sequence, or a page outside the pool: zeros (the softmax gives such slots no weight)
+        if ((tb + (i >> 1)) * BN + t >= p.len || !((r_have[rs] >> (t >> lseg)) & 1))
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int rs = (2 * jj + q) % RST;
-          if (!wait(&r_full[rs], ((2 * jj + q) / RST) & 1)) break;
-          raw[q] = sm + Sh::R_OFF + rs * Sh::RAW;
-          there[q] = (tb + i) * BN + q * 32 + t < p.len && ((r_have[rs] >> (t >> 4)) & 1);
-          uint32_t w[NW], pr[NG];
-          kv4_ldv(raw[q] + uo, w);
-          kv4_ldv(raw[q] + po, pr);
-          uint8_t* d = sm + Sh::K_OFF + st * (T * Sh::KB) + q * (32 * 128) + d0;
+          for (int k = 0; k < NG; ++k) pr[k] = 0u;
+        if (vnan && kv)
 #pragma unroll
-          for (int k = 0; k < NW; ++k) {
-            // past the sequence, or a page outside the pool: zeros (the softmax gives such slots no weight)
-            const uint32_t sb = there[q] ? pr[k * 64 / GROUP] : 0u;
-            uint4 hi, lo;
-            pt_unpack<SPLIT>(w[k], ks.of(sb), hi, lo);
-            *reinterpret_cast<uint4*>(d + k * (BN * 128)) = hi;
-            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + k * (BN * 128)) = lo;
-          }
-        }
-        if (*abort_flag) break;
-        fence_proxy_async();
-        mbar_arrive(&k_full[st]);
-        if (!wait(&v_empty[st], ph ^ 1)) break;
+          for (int k = 0; k < NG; ++k)
+            if (!(fabsf(kv4_param(pr[k]).x) < INFINITY) || !(fabsf(kv4_param(pr[k]).y) < INFINITY)) pr[k] = 0u;
+        mbar_arrive(&r_empty[rs]);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t w[NW], pr[NG];
-          kv4_ldv(raw[q] + Sh::CODES + Sh::PARAMS + uo, w);
-          kv4_ldv(raw[q] + Sh::CODES + Sh::PARAMS + po, pr);
-          mbar_arrive(&r_empty[(2 * jj + q) % RST]);
-          uint8_t* d = sm + Sh::V_OFF + st * (T * Sh::KB) + q * (32 * 128) + d0;
-#pragma unroll
-          for (int k = 0; k < NW; ++k) {
-            uint32_t sb = there[q] ? pr[k * 64 / GROUP] : 0u;
-            if (vnan && (!(fabsf(kv4_param(sb).x) < INFINITY) || !(fabsf(kv4_param(sb).y) < INFINITY))) sb = 0u;
-            uint4 hi, lo;
-            pt_unpack<SPLIT>(w[k], vs.of(sb), hi, lo);
-            *reinterpret_cast<uint4*>(d + k * (BN * 128)) = hi;
-            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + k * (BN * 128)) = lo;
-          }
+        for (int k = 0; k < NW; ++k) {
+          uint4 hi, lo;
+          pt_unpack<SPLIT>(w[k], sc.of(pr[k * 64 / GROUP]), hi, lo);
+          *reinterpret_cast<uint4*>(d + k * (BN * 128)) = hi;
+          if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + k * (BN * 128)) = lo;
         }
         fence_proxy_async();
-        mbar_arrive(&v_full[st]);
+        mbar_arrive((kv ? v_full : k_full) + st);
       }
     });
   } else {
     pt_regs_dec<PT_REGS_ISSUE>();
-    if (warp == 16) {
+    if (warp == PT_MMA) {
       // ------------------------------------------------------ MMA issue ----
       // The warp stays together, so that descriptors live in uniform
       // registers; one elected lane issues.
@@ -813,50 +806,51 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           __syncwarp();
         }
       });
-    } else if (warp == 17) {
+    } else if (warp == PT_COPY) {
       // --------------------------------------------------- bulk copies ----
-      // A stage is 32 slots: keys, their params, values and theirs of each
-      // block piece by a lane of its own.
-      const int nblk = g.page / g.seg, pc = min(g.seg, PT_RAW), np = PT_RAW / pc;  // slots of a piece, pieces
+      // A stage is a tile's keys with their params, or its values with theirs:
+      // one copy a block (one in all from pages of 64 slots on), a lane each.
+      const int nblk = g.page / g.seg, np = BN / g.seg, half = g.blk / 2;
       int issued = 0;
       for_items([&](const PtPlace& p, int tb, int nt, int, int) {
-        const int piece = lane >> 2, part = lane & 3;
-        const int bytes = part & 1 ? pc * NG * 4 : pc * (HD / 2);
-        for (int i = 0; i < 2 * nt; ++i, ++issued) {
-          const int jj = 2 * j + i, rs = jj % RST;
-          if (!wait(&r_empty[rs], ((jj / RST) & 1) ^ 1)) break;
-          const int s = tb * BN + i * PT_RAW + piece * pc;
-          const bool want = piece < np && s < p.len;
-          const int pg = want ? __ldg(g.table + p.seq * g.tstride + (s >> g.pshift)) : -1;
+        const int* tab = g.table + p.seq * g.tstride;
+        // page ids are fetched a tile ahead
+        auto page_of = [&](int i) {
+          const int s = (tb + i) * BN + lane * g.seg;
+          return i < nt && lane < np && s < p.len ? __ldg(tab + (s >> g.pshift)) : -1;
+        };
+        int pg = page_of(0);
+        for (int i = 0; i < nt; ++i) {
+          const int s = (tb + i) * BN + lane * g.seg;
           const bool on = unsigned(pg) < unsigned(g.npages);
-          if (want && !on && a.b.status) atomicOr(a.b.status, KV4_BAD);
+          if (!on && lane < np && s < p.len && a.b.status) atomicOr(a.b.status, KV4_BAD);
+          const uint8_t* src = g.pages + pg * g.page_bytes + int64_t(p.h * nblk + (s & (g.page - 1)) / g.seg) * g.blk;
           const unsigned have = __ballot_sync(0xffffffffu, on);
-          int bits = 0;  // by 16 slots
-          for (int k = 0; k < np; ++k)
-            if ((have >> (4 * k)) & 1) bits |= (pc == 16 ? 1 : 3) << k;
-          if (lane == 0) {
-            r_have[rs] = bits;
-            mbar_expect_tx(&r_full[rs], unsigned(__popc(have)) / 4 * unsigned(2 * pc * (HD / 2 + NG * 4)));
+          pg = page_of(i + 1);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv, ++issued) {
+            const int ss = 2 * (j + i) + kv, rs = ss % RST;
+            if (!wait(&r_empty[rs], ((ss / RST) & 1) ^ 1)) break;
+            if (lane == 0) {
+              r_have[rs] = int(have);
+              mbar_expect_tx(&r_full[rs], unsigned(__popc(have)) * unsigned(half));
+            }
+            __syncwarp();
+            if (on) bulk_g2s_keep(sm + Sh::R_OFF + rs * Sh::RAW + lane * half, src + kv * half, unsigned(half), &r_full[rs]);
           }
-          __syncwarp();
-          if (on) {
-            const uint8_t* blk = g.pages + pg * g.page_bytes + int64_t(p.h * nblk + (s & (g.page - 1)) / g.seg) * g.blk +
-                                 (part >> 1) * (g.blk / 2) + (part & 1) * (g.seg * (HD / 2));
-            uint8_t* d = sm + Sh::R_OFF + rs * Sh::RAW + (part >> 1) * (Sh::CODES + Sh::PARAMS) + (part & 1) * Sh::CODES;
-            bulk_g2s_keep(d + piece * bytes, blk + ((s & (g.seg - 1)) / pc) * bytes, unsigned(bytes), &r_full[rs]);
-          }
+          if (*abort_flag) break;
         }
       });
       if (*abort_flag)  // copies in flight land before the CTA may end
-        for (int i = max(0, issued - RST); i < issued; ++i) tg_wait(&r_full[i % RST], (i / RST) & 1);
+        for (int i = max(0, issued - RST); i < issued; ++i) pt_wait(&r_full[i % RST], (i / RST) & 1);
     }
   }
   __syncthreads();
-  if (warp == 16) {
+  if (warp == PT_MMA) {
     if (*abort_flag) {
       if (pt_elect()) tg_commit(drain);  // the products still in flight
       __syncwarp();
-      tg_wait(drain, 0);
+      pt_wait(drain, 0);
     }
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
