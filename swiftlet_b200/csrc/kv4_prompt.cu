@@ -14,7 +14,7 @@
 // (hi hi + lo hi + hi lo), f32 accumulators throughout.
 //
 // Warps: 0-7 softmax and output (two threads a row, half of the tile's slots
-// each), 8-23 unpacking, 24 MMA issue and TMEM, 25 bulk copies of the cache's
+// each), 8-15 unpacking of keys, 16-23 of values, 24 MMA issue and TMEM, 25 bulk copies of the cache's
 // bytes into a ring of stages (a tile's keys, then its values). Q stands in TMEM (its low terms in shared
 // memory), S and P share columns and are double-buffered, so Q K^T of the next
 // tile runs during the softmax of this one; the running maximum moves only
@@ -297,17 +297,11 @@ __global__ void __launch_bounds__(256) k_kv4_range(const Kv4AttnArgs a) {
   }
 }
 
-// Exponent that takes a largest |value| (f32 bits) to [2^13, 2^14).
-__device__ __forceinline__ int pt_exp(unsigned bits) { return bits ? max(-14, min(28, 13 - (int(bits >> 23) - 127))) : 0; }
+// Exponent that takes a largest |value| (f32 bits) to [2^13, 2^14), as far as
+// an f16 factor goes. Params times it are exact, but where they leave f16's
+// normal range (below 2^-28 of the largest value).
+__device__ __forceinline__ int pt_exp(unsigned bits) { return bits ? max(-14, min(14, 13 - (int(bits >> 23) - 127))) : 0; }
 __device__ __forceinline__ float pt_pow2(int e) { return __int_as_float((127 + e) << 23); }
-
-// Params times 2^x as two f16 factors of at most 2^14 (exact, but where they
-// leave f16's normal range: below 2^-28 of the largest value).
-struct PtScale {
-  __half2 h0, h1;
-  __device__ explicit PtScale(int x) : h0(__float2half2_rn(pt_pow2(x / 2))), h1(__float2half2_rn(pt_pow2(x - x / 2))) {}
-  __device__ __half2 of(uint32_t param) const { return __hmul2(__hmul2(pt_u2(param), h0), h1); }
-};
 
 // Eight codes of a word as f16 pairs (0 4)(1 5)(2 6)(3 7): the scaled value s c
 // + b, rounded once, or as two terms. The codes themselves come out of the
@@ -363,14 +357,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
   const Kv4Geo& g = a.g;
   if (tid == 0) {
     for (int s = 0; s < KST; ++s) {
-      mbar_init(&k_full[s], PT_UNPACK);
-      mbar_init(&v_full[s], PT_UNPACK);
+      mbar_init(&k_full[s], PT_UNPACK / 2);
+      mbar_init(&v_full[s], PT_UNPACK / 2);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_empty[s], 1);
     }
     for (int s = 0; s < RST; ++s) {
       mbar_init(&r_full[s], 1);
-      mbar_init(&r_empty[s], PT_UNPACK);
+      mbar_init(&r_empty[s], PT_UNPACK / 2);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
@@ -650,7 +644,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
   } else if (warp < PT_MMA) {
     // -------------------------------------------------------- unpacking ----
     pt_regs_dec<PT_REGS_UNPACK>();
-    const int ut = tid - PT_SOFT, r = ut & 7, t = ut >> 3;
+    const int ut = tid - PT_SOFT, kv = ut >> 8, r = ut & 7, t = (ut >> 3) & 31;
+    uint64_t *full = kv ? v_full : k_full, *empty = kv ? v_empty : k_empty;
+    uint8_t* dst = sm + (kv ? Sh::V_OFF : Sh::K_OFF) + t * 128 + ((r ^ (t & 7)) << 4);
     for_items([&](const PtPlace& p, int tb, int nt, int v1, int) {
       int kx, vx;
       const unsigned flags = ranges(p, kx, vx);
@@ -706,41 +702,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       fence_proxy_async();
       bar();
       bar();
-      // a thread: unit r of slot t of the tile, every 64-channel block; the
-      // keys, then the values, by the same code (the instruction cache holds
-      // it beside the softmax's)
-      const bool vnan = (flags & 1u) != 0u;
-      const int half = g.blk / 2, lseg = g.seg == 16 ? 4 : g.seg == 32 ? 5 : 6, in = t & (g.seg - 1), base = (t >> lseg) * half;
-      const int uo = base + in * (HD / 2) + ((r ^ kv4_swz(HD, t)) * (HD / 16)), po = base + g.seg * (HD / 2) + in * NG * 4;
-      const int d0 = t * 128 + ((r ^ (t & 7)) << 4);
+      // a thread: unit r of slots t and t + 32 of the tile, every 64-channel block
+      const bool vnan = kv && (flags & 1u) != 0u;
+      const __half2 sc = __float2half2_rn(pt_pow2(kv ? vx : kx));
+      const int half = g.blk / 2, lseg = g.seg == 16 ? 4 : g.seg == 32 ? 5 : 6;
+      int uo[2], po[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int s = t + 32 * q, in = s & (g.seg - 1), base = (s >> lseg) * half;
+        uo[q] = base + in * (HD / 2) + ((r ^ kv4_swz(HD, t)) * (HD / 16));
+        po[q] = base + g.seg * (HD / 2) + in * NG * 4;
+      }
 #pragma unroll 1
-      for (int i = 0; i < 2 * nt; ++i) {
-        const int jj = j + (i >> 1), st = jj % KST, kv = i & 1, ss = 2 * j + i, rs = ss % RST;
-        if (!wait((kv ? v_empty : k_empty) + st, ((jj / KST) & 1) ^ 1) || !wait(&r_full[rs], (ss / RST) & 1)) break;
+      for (int i = 0; i < nt; ++i) {
+        const int jj = j + i, st = jj % KST, ss = 2 * jj + kv, rs = ss % RST;
+        if (!wait(empty + st, ((jj / KST) & 1) ^ 1) || !wait(&r_full[rs], (ss / RST) & 1)) break;
         const uint8_t* raw = sm + Sh::R_OFF + rs * Sh::RAW;
-        uint8_t* d = sm + (kv ? Sh::V_OFF : Sh::K_OFF) + st * (T * Sh::KB) + d0;
-        const PtScale sc(kv ? vx : kx);
-        uint32_t w[NW], pr[NG];
-        kv4_ldv(raw + uo, w);
-        kv4_ldv(raw + po, pr);
-        // past the sequence, or a page outside the pool: zeros (the softmax gives such slots no weight)
-        if ((tb + (i >> 1)) * BN + t >= p.len || !((r_have[rs] >> (t >> lseg)) & 1))
+        uint8_t* d = dst + st * (T * Sh::KB);
+        uint32_t w[2][NW], pr[2][NG];
+        const int have = r_have[rs], s0 = (tb + i) * BN + t;
 #pragma unroll
-          for (int k = 0; k < NG; ++k) pr[k] = 0u;
-        if (vnan && kv)
+        for (int q = 0; q < 2; ++q) {
+          kv4_ldv(raw + uo[q], w[q]);
+          kv4_ldv(raw + po[q], pr[q]);
+          // past the sequence, or a page outside the pool: zeros (the softmax gives such slots no weight)
+          if (s0 + 32 * q >= p.len || !((have >> ((t + 32 * q) >> lseg)) & 1))
 #pragma unroll
-          for (int k = 0; k < NG; ++k)
-            if (!(fabsf(kv4_param(pr[k]).x) < INFINITY) || !(fabsf(kv4_param(pr[k]).y) < INFINITY)) pr[k] = 0u;
+            for (int k = 0; k < NG; ++k) pr[q][k] = 0u;
+          if (vnan)
+#pragma unroll
+            for (int k = 0; k < NG; ++k)
+              if (!(fabsf(kv4_param(pr[q][k]).x) < INFINITY) || !(fabsf(kv4_param(pr[q][k]).y) < INFINITY)) pr[q][k] = 0u;
+        }
         mbar_arrive(&r_empty[rs]);
 #pragma unroll
-        for (int k = 0; k < NW; ++k) {
-          uint4 hi, lo;
-          pt_unpack<SPLIT>(w[k], sc.of(pr[k * 64 / GROUP]), hi, lo);
-          *reinterpret_cast<uint4*>(d + k * (BN * 128)) = hi;
-          if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + k * (BN * 128)) = lo;
-        }
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int k = 0; k < NW; ++k) {
+            uint4 hi, lo;
+            pt_unpack<SPLIT>(w[q][k], __hmul2(pt_u2(pr[q][k * 64 / GROUP]), sc), hi, lo);
+            *reinterpret_cast<uint4*>(d + q * (32 * 128) + k * (BN * 128)) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + q * (32 * 128) + k * (BN * 128)) = lo;
+          }
         fence_proxy_async();
-        mbar_arrive((kv ? v_full : k_full) + st);
+        mbar_arrive(full + st);
       }
     });
   } else {
@@ -750,29 +755,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       // The warp stays together, so that descriptors live in uniform
       // registers; one elected lane issues.
       constexpr uint32_t ids = pt_idesc(BN, false), idp = pt_idesc(HD, true);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       for_items([&](const PtPlace&, int, int nt, int, int) {
         bar();
         bar();
         tg_fence_after();
         auto qk = [&](int i) {
-          const int jj = j + i, st = jj % KST, b = jj & 1;
+          const int jj = __shfl_sync(0xffffffffu, j + i, 0), st = jj % KST, b = jj & 1;
           if (!wait(&k_full[st], (jj / KST) & 1)) return false;
           tg_fence_after();
           const uint64_t kd = tg_desc(smem_u32(sm + Sh::K_OFF + st * (T * Sh::KB)));
-          const uint32_t d = tmem + Sh::S_COL + b * BN;
+          const uint32_t d = tm + Sh::S_COL + b * BN;
           if (pt_elect()) {
 #pragma unroll
             for (int w = 0; w < NW; ++w)
 #pragma unroll
               for (int k = 0; k < 4; ++k)  // 16 channels: 32 bytes of the 128-byte rows
-                pt_mma_ts(d, tmem + Sh::Q_COL + w * 32 + k * 8, kd + ((w * (BN * 128) + k * 32) >> 4), ids, w + k > 0);
+                pt_mma_ts(d, tm + Sh::Q_COL + w * 32 + k * 8, kd + ((w * (BN * 128) + k * 32) >> 4), ids, w + k > 0);
             if (SPLIT) {
               const uint64_t qd = tg_desc(smem_u32(sm + Sh::Q_OFF));
 #pragma unroll
               for (int w = 0; w < NW; ++w)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                  pt_mma_ts(d, tmem + Sh::Q_COL + w * 32 + k * 8, kd + ((Sh::KB + w * (BN * 128) + k * 32) >> 4), ids, true);
+                  pt_mma_ts(d, tm + Sh::Q_COL + w * 32 + k * 8, kd + ((Sh::KB + w * (BN * 128) + k * 32) >> 4), ids, true);
                   pt_mma_ss(d, qd + ((w * (PT_ROWS * 128) + k * 32) >> 4), kd + ((w * (BN * 128) + k * 32) >> 4), ids, true);
                 }
             }
@@ -786,18 +792,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         for (int i = 0; i < nt && ok; ++i) {
           // S of tile i + 1 takes the columns P of tile i - 1 was read from: products complete in order
           if (i + 1 < nt) ok = qk(i + 1);
-          const int jj = j + i, st = jj % KST, b = jj & 1;
+          const int jj = __shfl_sync(0xffffffffu, j + i, 0), st = jj % KST, b = jj & 1;
           if (!ok || !wait(&v_full[st], (jj / KST) & 1) || !wait(&p_full[b], (jj >> 1) & 1)) break;
           tg_fence_after();
           const uint64_t vd = pt_desc_n(smem_u32(sm + Sh::V_OFF + st * (T * Sh::KB)), BN * 128);
-          const uint32_t pc = tmem + Sh::S_COL + b * BN;
+          const uint32_t pc = tm + Sh::S_COL + b * BN;
           if (pt_elect()) {
 #pragma unroll
             for (int k = 0; k < BN / 16; ++k) {
-              pt_mma_ts(tmem + Sh::O_COL, pc + k * 8, vd + ((k * 2048) >> 4), idp, k > 0 || i > 0);
+              pt_mma_ts(tm + Sh::O_COL, pc + k * 8, vd + ((k * 2048) >> 4), idp, k > 0 || i > 0);
               if (SPLIT) {
-                pt_mma_ts(tmem + Sh::O_COL, pc + 32 + k * 8, vd + ((k * 2048) >> 4), idp, true);
-                pt_mma_ts(tmem + Sh::O_COL, pc + k * 8, vd + ((Sh::KB + k * 2048) >> 4), idp, true);
+                pt_mma_ts(tm + Sh::O_COL, pc + 32 + k * 8, vd + ((k * 2048) >> 4), idp, true);
+                pt_mma_ts(tm + Sh::O_COL, pc + k * 8, vd + ((Sh::KB + k * 2048) >> 4), idp, true);
               }
             }
             tg_commit(&o_done[b]);
