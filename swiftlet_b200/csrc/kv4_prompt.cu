@@ -14,8 +14,8 @@
 // (hi hi + lo hi + hi lo), f32 accumulators throughout.
 //
 // Warps: 0-7 softmax and output (two threads a row, half of the tile's slots
-// each), 8-15 unpacking of keys, 16-23 of values, 24 MMA issue and TMEM, 25 bulk copies of the cache's
-// bytes into a ring of stages (a tile's keys, then its values). Q stands in TMEM (its low terms in shared
+// each), 8-15 unpacking of keys, 16-23 of values, 24 MMA issue and TMEM, 25 and 26 bulk copies
+// of the cache's bytes (a tile's keys, a tile's values) into a ring of stages. Q stands in TMEM (its low terms in shared
 // memory), S and P share columns and are double-buffered, so Q K^T of the next
 // tile runs during the softmax of this one; the running maximum moves only
 // when it has grown by 2^8, so O in TMEM is rarely touched. Bound: the tensor
@@ -53,7 +53,9 @@ template <int HD, int GROUP, bool SPLIT>
 struct PtShape {
   static constexpr int T = SPLIT ? 2 : 1;                  // f16 terms of an operand
   static constexpr int KST = HD == 256 && SPLIT ? 1 : 2;   // buffers of unpacked keys, and of values
-  static constexpr int RST = HD == 256 && SPLIT ? 3 : 4;   // copied stages
+  // Copied stages: the keys' and the values', rings of their own, for a wait by
+  // parity tells two neighbouring phases apart and no more.
+  static constexpr int RK = 2, RV = HD == 256 && SPLIT ? 1 : 2, RST = RK + RV;
   static constexpr int QB = PT_ROWS * HD * 2;              // bytes of one term of Q
   static constexpr int KB = PT_BN * HD * 2;                // of one term of a tile's keys (values)
   static constexpr int RAW = PT_BN * (HD / 2 + 4 * (HD / GROUP));  // bytes of a tile's keys (values) as they are held
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       __syncwarp();
       // every role takes the same decision to leave, or one would wait for another
       bool over = *abort_flag != 0;
-      if (warp != PT_COPY) {
+      if (warp <= PT_MMA) {
         over = pt_bar_any<PT_MEET>(1, over);
         tg_fence_after();
       }
@@ -715,8 +717,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       }
 #pragma unroll 1
       for (int i = 0; i < nt; ++i) {
-        const int jj = j + i, st = jj % KST, ss = 2 * jj + kv, rs = ss % RST;
-        if (!wait(empty + st, ((jj / KST) & 1) ^ 1) || !wait(&r_full[rs], (ss / RST) & 1)) break;
+        const int jj = j + i, st = jj % KST, rs = kv ? Sh::RK + jj % Sh::RV : jj % Sh::RK;
+        if (!wait(empty + st, ((jj / KST) & 1) ^ 1) || !wait(&r_full[rs], (jj / (kv ? Sh::RV : Sh::RK)) & 1)) break;
         const uint8_t* raw = sm + Sh::R_OFF + rs * Sh::RAW;
         uint8_t* d = dst + st * (T * Sh::KB);
         uint32_t w[2][NW], pr[2][NG];
@@ -812,10 +814,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           __syncwarp();
         }
       });
-    } else if (warp == PT_COPY) {
+    } else if (warp == PT_COPY || warp == PT_COPY + 1) {
       // --------------------------------------------------- bulk copies ----
       // A stage is a tile's keys with their params, or its values with theirs:
       // one copy a block (one in all from pages of 64 slots on), a lane each.
+      const int kv = warp - PT_COPY, ring = kv ? Sh::RV : Sh::RK, base = kv ? Sh::RK : 0;
       const int nblk = g.page / g.seg, np = BN / g.seg, half = g.blk / 2;
       int issued = 0;
       for_items([&](const PtPlace& p, int tb, int nt, int, int) {
@@ -826,29 +829,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           return i < nt && lane < np && s < p.len ? __ldg(tab + (s >> g.pshift)) : -1;
         };
         int pg = page_of(0);
-        for (int i = 0; i < nt; ++i) {
-          const int s = (tb + i) * BN + lane * g.seg;
+        for (int i = 0; i < nt; ++i, ++issued) {
+          const int s = (tb + i) * BN + lane * g.seg, jj = j + i, rs = base + jj % ring;
           const bool on = unsigned(pg) < unsigned(g.npages);
           if (!on && lane < np && s < p.len && a.b.status) atomicOr(a.b.status, KV4_BAD);
-          const uint8_t* src = g.pages + pg * g.page_bytes + int64_t(p.h * nblk + (s & (g.page - 1)) / g.seg) * g.blk;
+          const uint8_t* src = g.pages + pg * g.page_bytes + int64_t(p.h * nblk + (s & (g.page - 1)) / g.seg) * g.blk + kv * half;
           const unsigned have = __ballot_sync(0xffffffffu, on);
           pg = page_of(i + 1);
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv, ++issued) {
-            const int ss = 2 * (j + i) + kv, rs = ss % RST;
-            if (!wait(&r_empty[rs], ((ss / RST) & 1) ^ 1)) break;
-            if (lane == 0) {
-              r_have[rs] = int(have);
-              mbar_expect_tx(&r_full[rs], unsigned(__popc(have)) * unsigned(half));
-            }
-            __syncwarp();
-            if (on) bulk_g2s_keep(sm + Sh::R_OFF + rs * Sh::RAW + lane * half, src + kv * half, unsigned(half), &r_full[rs]);
+          if (!wait(&r_empty[rs], ((jj / ring) & 1) ^ 1)) break;
+          if (lane == 0) {
+            r_have[rs] = int(have);
+            mbar_expect_tx(&r_full[rs], unsigned(__popc(have)) * unsigned(half));
           }
-          if (*abort_flag) break;
+          __syncwarp();
+          if (on) bulk_g2s_keep(sm + Sh::R_OFF + rs * Sh::RAW + lane * half, src, unsigned(half), &r_full[rs]);
         }
       });
       if (*abort_flag)  // copies in flight land before the CTA may end
-        for (int i = max(0, issued - RST); i < issued; ++i) pt_wait(&r_full[i % RST], (i / RST) & 1);
+        for (int i = max(0, issued - ring); i < issued; ++i) pt_wait(&r_full[base + i % ring], (i / ring) & 1);
     }
   }
   __syncthreads();
