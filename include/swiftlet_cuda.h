@@ -340,8 +340,8 @@ typedef struct swl_kv4_cache {
  * tokens of sequence i (any number, 0 included), which take its last slots:
  * lens[i] counts the slots with the new ones. total bounds the rows, max_new
  * the new tokens of one sequence, max_len the slots of one sequence (a length
- * outside [0, max_len] is held to it). Rows from start[nseq] on are neither
- * read nor written. status (device int32, may be NULL; never cleared): bit 0,
+ * outside [0, max_len] is held to it). Rows from start[nseq] on (total at
+ * most) are not used, and not written. status (device int32, may be NULL; never cleared): bit 0,
  * a bounded wait inside a kernel gave up and the results are incomplete; bit
  * 1, a length outside [0, max_len] or a page outside the pool (such slots
  * are skipped as if masked). */

@@ -81,95 +81,151 @@ bool vec_rows(const Kv4Rows& r, int dt) {
   return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.ts * e % 16 == 0 && r.hs * e % 16 == 0;
 }
 
+// Where a token of the block goes: its slot's block for kv head 0 (null: no
+// slot, or a page outside the pool), the row in it, the sequence and slot.
+struct IoToken {
+  uint8_t* blk;
+  int t, seq, slot;
+};
+constexpr int IO_TOKENS = 16;  // tokens of a block at most
+constexpr int IO_U = 4;        // rows a warp has in flight
+
 template <int DT, bool READ>
-__global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool vk, bool vv) {
+__global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool vk, bool vv, int tokens) {
+  __shared__ IoToken tok[IO_TOKENS];
   const Kv4Geo& g = a.g;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int lpr = g.hd / 8, rpw = 32 / lpr;       // lanes a row, rows a warp
-  const int per = (g.kvh * 2 + rpw - 1) / rpw;    // warps a token
-  const int64_t wid = int64_t(blockIdx.x) * (IO_THREADS / 32) + warp;
-  const int j = int(wid / per);
-  if (j >= a.b.total) return;
-  const int seq = kv4_seq_of(a.b, j);
-  if (seq < 0) return;
-  int row0;
-  const int n = kv4_new(a.b, seq, row0);
-  const int len = kv4_len(a.b, seq);
-  const int slot = len - n + (j - row0);
-  if (slot < 0 || slot >= len) return;  // more new tokens than slots: the first of them have none
-  const int row = int(wid % per) * rpw + lane / lpr, l = lane % lpr;
-  const bool on = row < g.kvh * 2;
-  const int h = on ? row >> 1 : 0, kv = row & 1;
-  uint8_t* blk = kv4_block(g, g.table, g.tstride, seq, h, slot, a.b.status);
-  if (!blk) return;  // the same page for the whole warp
-  const int t = slot & (g.seg - 1);
-  uint8_t* base = blk + (kv ? g.blk / 2 : 0);
-  uint32_t* word = reinterpret_cast<uint32_t*>(base + t * (g.hd / 2) + ((l & 7) ^ kv4_swz(g.hd, t)) * (g.hd / 16) + (l >> 3) * 4);
-  uint32_t* par = reinterpret_cast<uint32_t*>(base + g.seg * (g.hd / 2)) + t * g.ng + l * 8 / g.group;
-  const Kv4Rows& r = kv ? a.v : a.k;
-  const int64_t at = j * r.ts + h * r.hs + l * 8;
-  const bool vec = kv ? vv : vk;
-  float x[8];
-  if (READ) {
-    if (!on) return;
-    const float2 sb = kv4_param(*par);
-    const uint32_t w = *word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j0 = blockIdx.x * tokens;
+  const int lpr = g.hd / 8, rpw = 32 / lpr;  // lanes a row, rows a warp
+  const int sub = lane / lpr, l = lane % lpr;
+  const int rows = tokens * g.kvh * 2;       // row = (head, K or V) * tokens + token
+  const int step = IO_THREADS / 32 * rpw;
+  const int nb = g.page / g.seg;
+  float x[IO_U][8];
+  auto place = [&](int rid, int& j, int& h, int& kv) {
+    const int hk = rid / tokens;
+    j = j0 + rid - hk * tokens;
+    h = hk >> 1;
+    kv = hk & 1;
+    return rid < rows && j < a.b.total;
+  };
+  auto fetch = [&](int base) {  // what the inputs alone determine
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(__fmul_rn(sb.x, float((w >> (4 * e)) & 15u)), sb.y);
-    store8<DT>(r.p, at, vec, x);
-  } else {
-    if (on) load8<DT>(r.p, at, vec, x);
-    else
-      for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    float mn = x[0], mx = x[0];
-    bool bad = false;
+    for (int u = 0; u < IO_U; ++u) {
+      int j, h, kv;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      mn = fminf(mn, x[e]);
-      mx = fmaxf(mx, x[e]);
-      bad |= !(fabsf(x[e]) < INFINITY);
+      for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
+      if (!place(base + u * step + sub, j, h, kv)) continue;
+      const Kv4Rows& r = kv ? a.v : a.k;
+      load8<DT>(r.p, j * r.ts + h * r.hs + l * 8, kv ? vv : vk, x[u]);
     }
-    for (int o = 1; o < g.group / 8; o <<= 1) {
-      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      bad |= __shfl_xor_sync(0xffffffffu, int(bad), o) != 0;
+  };
+  if (!READ) fetch(warp * rpw);
+  for (int i = warp; i < tokens; i += IO_THREADS / 32) {
+    const int j = j0 + i;
+    IoToken t = {nullptr, 0, 0, 0};
+    const int seq = j < a.b.total ? kv4_seq_of(a.b, j) : -1;
+    if (seq >= 0) {
+      int row0;
+      const int n = kv4_new(a.b, seq, row0), len = kv4_len(a.b, seq);
+      t.slot = len - n + (j - row0);
+      t.seq = seq;
+      t.t = t.slot & (g.seg - 1);
+      // a negative slot: more new tokens than slots, the first of them have none
+      if (t.slot >= 0 && t.slot < len) t.blk = kv4_block(g, g.table, g.tstride, seq, 0, t.slot, a.b.status);
     }
-    const __half hb = __float2half_rn(mn), hs = __float2half_rn(__fmul_rn(__fsub_rn(mx, mn), 1.f / 15.f));
-    const float b = __half2float(hb), s = __half2float(hs);
-    bad |= !(fabsf(b) < INFINITY) || !(s < INFINITY);
-    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-    uint32_t w = 0u;
+    if (lane == 0) tok[i] = t;
+  }
+  __syncthreads();
+  for (int base = warp * rpw; base < rows; base += step * IO_U) {
+    if (!READ && base != warp * rpw) fetch(base);
+    uint32_t w[IO_U], pr[IO_U];
+    uint8_t* at[IO_U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], b), inv)), 0.f), 15.f);
-      w |= uint32_t(int(c)) << (4 * e);
+    for (int u = 0; u < IO_U; ++u) {
+      int j, h, kv;
+      at[u] = nullptr;
+      if (place(base + u * step + sub, j, h, kv) && tok[j - j0].blk)
+        at[u] = tok[j - j0].blk + int64_t(h) * nb * g.blk + (kv ? g.blk / 2 : 0);
+      if (READ && at[u]) {
+        const int t = tok[j - j0].t;
+        w[u] = *reinterpret_cast<const uint32_t*>(at[u] + t * (g.hd / 2) + ((l & 7) ^ kv4_swz(g.hd, t)) * (g.hd / 16) + (l >> 3) * 4);
+        pr[u] = reinterpret_cast<const uint32_t*>(at[u] + g.seg * (g.hd / 2))[t * g.ng + l * 8 / g.group];
+      }
     }
-    if (!on) return;
-    *word = bad ? 0u : w;
-    if (l * 8 % g.group == 0)
-      *par = bad ? 0x7e007e00u : uint32_t(__half_as_ushort(hs)) | uint32_t(__half_as_ushort(hb)) << 16;
-    if (a.weights && l == 0 && kv == 0) a.weights[(int64_t(seq) * g.kvh + h) * a.wstride + slot] = 0.f;
+#pragma unroll
+    for (int u = 0; u < IO_U; ++u) {
+      int j, h, kv;
+      const bool on = place(base + u * step + sub, j, h, kv) && at[u];
+      if (READ) {
+        if (!on) continue;
+        const Kv4Rows& r = kv ? a.v : a.k;
+        const float2 sb = kv4_param(pr[u]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[u][e] = __fadd_rn(__fmul_rn(sb.x, float((w[u] >> (4 * e)) & 15u)), sb.y);
+        store8<DT>(r.p, j * r.ts + h * r.hs + l * 8, kv ? vv : vk, x[u]);
+      } else {
+        float mn = x[u][0], mx = x[u][0];
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          mn = fminf(mn, x[u][e]);
+          mx = fmaxf(mx, x[u][e]);
+          bad |= !(fabsf(x[u][e]) < INFINITY);
+        }
+        for (int o = 1; o < g.group / 8; o <<= 1) {
+          mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          bad |= __shfl_xor_sync(0xffffffffu, int(bad), o) != 0;
+        }
+        const __half hb = __float2half_rn(mn), hs = __float2half_rn(__fmul_rn(__fsub_rn(mx, mn), 1.f / 15.f));
+        const float b = __half2float(hb), s = __half2float(hs);
+        bad |= !(fabsf(b) < INFINITY) || !(s < INFINITY);
+        const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+        uint32_t word = 0u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[u][e], b), inv)), 0.f), 15.f);
+          word |= uint32_t(int(c)) << (4 * e);
+        }
+        if (!on) continue;
+        const IoToken& k = tok[j - j0];
+        *reinterpret_cast<uint32_t*>(at[u] + k.t * (g.hd / 2) + ((l & 7) ^ kv4_swz(g.hd, k.t)) * (g.hd / 16) + (l >> 3) * 4) = bad ? 0u : word;
+        if (l * 8 % g.group == 0)
+          reinterpret_cast<uint32_t*>(at[u] + g.seg * (g.hd / 2))[k.t * g.ng + l * 8 / g.group] =
+              bad ? 0x7e007e00u : uint32_t(__half_as_ushort(hs)) | uint32_t(__half_as_ushort(hb)) << 16;
+        if (a.weights && l == 0 && kv == 0) a.weights[(int64_t(k.seq) * g.kvh + h) * a.wstride + k.slot] = 0.f;
+      }
+    }
   }
 }
 
 template <bool READ>
 void launch_io(const Kv4IoArgs& a, int dt, cudaStream_t st) {
-  const int rpw = 256 / a.g.hd, per = (a.g.kvh * 2 + rpw - 1) / rpw;
-  const int64_t warps = int64_t(a.b.total) * per, blocks = (warps + IO_THREADS / 32 - 1) / (IO_THREADS / 32);
-  if (blocks > 0x7fffffff) throw Error(ERR_UNSUPPORTED, "kv4: too many rows for one launch");
+  // tokens a block: as many as leave four blocks an SM, so that a step of a
+  // few tokens still spreads over the GPU
+  const int tokens = std::max(1, std::min(IO_TOKENS, a.b.total / 592));
   const bool vk = vec_rows(a.k, dt), vv = vec_rows(a.v, dt);
-  const dim3 grid = dim3(unsigned(blocks)), block(IO_THREADS);
-  if (dt == DT_F32) launch(k_kv4_io<DT_F32, READ>, grid, block, 0, st, false, a, vk, vv);
-  else if (dt == DT_BF16) launch(k_kv4_io<DT_BF16, READ>, grid, block, 0, st, false, a, vk, vv);
-  else launch(k_kv4_io<DT_F16, READ>, grid, block, 0, st, false, a, vk, vv);
+  const dim3 grid((a.b.total + tokens - 1) / tokens), block(IO_THREADS);
+  if (dt == DT_F32) launch(k_kv4_io<DT_F32, READ>, grid, block, 0, st, false, a, vk, vv, tokens);
+  else if (dt == DT_BF16) launch(k_kv4_io<DT_BF16, READ>, grid, block, 0, st, false, a, vk, vv, tokens);
+  else launch(k_kv4_io<DT_F16, READ>, grid, block, 0, st, false, a, vk, vv, tokens);
 }
 
 // ---------------------------------------------------------------- evict --
 // Which slots survive, per (sequence, kv head): the first `first`, the last
 // `recent`, and of the others the largest weights up to `keep` in all (ties to
-// the lowest slot, NaN as -infinity). Radix select over order-preserving
-// 32-bit keys, then the survivors' slots in ascending order.
+// the lowest slot, NaN as -infinity). A cluster of EV_CL CTAs shares the slots
+// in contiguous parts; each keeps the order-preserving 32-bit keys of its part
+// in shared memory (as far as they fit) and they select by radix, 11, 11 and 10
+// bits, adding up their histograms through distributed shared memory. Each CTA
+// then writes the survivors of its part in order, behind those of the CTAs
+// before it. Bound: the latency of the passes (reads of `len` words); one CTA
+// for all took 130 us at 65536 slots.
 constexpr int EV_THREADS = 1024;
+constexpr int EV_CL = 8;
+constexpr int EV_BINS = 2048;
+constexpr int EV_KEYS = 16384;  // keys a CTA holds
+constexpr size_t EV_SMEM = EV_KEYS * 4;
 
 __device__ __forceinline__ uint32_t ev_key(float w) {
   if (!(w == w)) w = -INFINITY;
@@ -177,6 +233,13 @@ __device__ __forceinline__ uint32_t ev_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+__device__ __forceinline__ int ev_ld(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Exclusive scan of one int a thread; returns the total.
 __device__ int ev_scan(int v, int* ex, int* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int inc = v;
@@ -205,87 +268,152 @@ __device__ int ev_scan(int v, int* ex, int* warp_sums) {
   return total;
 }
 
-__global__ void __launch_bounds__(EV_THREADS) k_kv4_evict_select(const Kv4EvictArgs a) {
-  __shared__ unsigned hist[256];
-  __shared__ int warp_sums[33];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_rem;
-  const int seq = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
+__global__ void __launch_bounds__(EV_THREADS, 1) k_kv4_evict_select(const Kv4EvictArgs a) {
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[2][EV_BINS];
+  __shared__ int warp_sums[33], s_bin, s_above, s_cnt[2];
+  const int seq = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+  const int rank = int(cluster_rank());
   const int len = kv4_len(a.b, seq), nl = min(len, a.keep);
-  if (h == 0 && tid == 0) a.new_lens[seq] = nl;
+  if (h == 0 && rank == 0 && tid == 0) a.new_lens[seq] = nl;
   const float* w = a.weights + (int64_t(seq) * a.g.kvh + h) * a.wstride;
   int* kept = a.kept + (int64_t(seq) * a.g.kvh + h) * a.kstride;
-  if (nl == len) {
-    for (int i = tid; i < len; i += EV_THREADS) kept[i] = i;
+  const int part = (len + EV_CL - 1) / EV_CL, p0 = min(len, rank * part), p1 = min(len, p0 + part);
+  if (nl == len) {  // the whole cluster takes this way
+    for (int i = p0 + tid; i < p1; i += EV_THREADS) kept[i] = i;
     return;
   }
-  const int lo = a.first, hi = len - a.recent;  // candidates [lo, hi); first + recent <= keep < len
-  uint32_t mask = 0u;
-  if (tid == 0) { s_prefix = 0u; s_rem = a.keep - a.first - a.recent; }
-  __syncthreads();
-  const bool none = s_rem == 0;
+  // candidates: [first, len - recent); first + recent <= keep < len
+  const int c0 = max(p0, a.first), c1 = min(p1, len - a.recent);
+  const int held = min(c1, c0 + EV_KEYS);
+  for (int i = c0 + tid; i < held; i += EV_THREADS) keys[i - c0] = ev_key(w[i]);
+  auto key_of = [&](int i) { return i < held ? keys[i - c0] : ev_key(w[i]); };
+  int rem = a.keep - a.first - a.recent;  // still to be found among the keys with the prefix
+  uint32_t prefix = 0u, mask = 0u;
+  const bool none = rem == 0;
   if (!none)
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int b = tid; b < 256; b += EV_THREADS) hist[b] = 0u;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      int* hs = hist[pass & 1];
+      for (int b = tid; b < EV_BINS; b += EV_THREADS) hs[b] = 0;
       __syncthreads();
-      const uint32_t prefix = s_prefix;
-      for (int i = lo + tid; i < hi; i += EV_THREADS) {
-        const uint32_t key = ev_key(w[i]);
-        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+      for (int i = c0 + tid; i < c1; i += EV_THREADS) {
+        const uint32_t key = key_of(i);
+        if ((key & mask) == prefix) atomicAdd(&hs[(key >> shift) & ((1u << bits) - 1u)], 1);
       }
-      __syncthreads();
-      if (tid == 0) {
-        int rem = s_rem, b = 255;
-        for (; b > 0; --b) {
-          if (int(hist[b]) >= rem) break;
-          rem -= int(hist[b]);
+      cluster_sync();
+      // two bins a thread, the largest first
+      int n[2], ex;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        n[k] = 0;
+        const int bin = EV_BINS - 1 - (2 * tid + k);
+        for (int c = 0; c < EV_CL; ++c) n[k] += ev_ld(dsmem_map(&hs[bin], c));
+      }
+      ev_scan(n[0] + n[1], &ex, warp_sums);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int above = ex + (k ? n[0] : 0);
+        if (above < rem && above + n[k] >= rem) {
+          s_bin = EV_BINS - 1 - (2 * tid + k);
+          s_above = above;
         }
-        s_prefix = prefix | (uint32_t(b) << shift);
-        s_rem = rem;
       }
-      mask |= 255u << shift;
+      __syncthreads();
+      prefix |= uint32_t(s_bin) << shift;
+      rem -= s_above;
+      mask |= ((1u << bits) - 1u) << shift;
       __syncthreads();
     }
-  const uint32_t thr = none ? 0xffffffffu : s_prefix;
-  int need_eq = none ? 0 : s_rem, out = 0;
-  for (int i0 = 0; i0 < len; i0 += EV_THREADS) {
-    const int i = i0 + tid;
-    const bool cand = i >= lo && i < hi;
-    const uint32_t key = cand ? ev_key(w[i]) : 0u;
-    int eq_at, at;
-    const int n_eq = ev_scan(cand && key == thr, &eq_at, warp_sums);
-    const bool take = i < len && (!cand || (key > thr && !none) || (key == thr && eq_at < need_eq));
-    const int n = ev_scan(take, &at, warp_sums);
-    if (take) kept[out + at] = i;
-    out += n;
-    need_eq -= min(need_eq, n_eq);
+  const uint32_t thr = prefix;
+  // survivors and ties at the threshold of the parts before this one
+  int gt = 0, eq = 0;
+  for (int i = p0 + tid; i < p1; i += EV_THREADS) {
+    const bool cand = i >= c0 && i < c1;
+    const uint32_t key = cand ? key_of(i) : 0u;
+    gt += !cand || (!none && key > thr);
+    eq += cand && !none && key == thr;
   }
+  gt = __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  if (tid < 2) s_cnt[tid] = 0;
+  __syncthreads();
+  if ((tid & 31) == 0) {
+    atomicAdd(&s_cnt[0], gt);
+    atomicAdd(&s_cnt[1], eq);
+  }
+  cluster_sync();
+  int gt0 = 0, eq0 = 0;
+  for (int c = 0; c < rank; ++c) {
+    gt0 += ev_ld(dsmem_map(&s_cnt[0], c));
+    eq0 += ev_ld(dsmem_map(&s_cnt[1], c));
+  }
+  cluster_arrive();  // done with the others' shared memory; theirs with this one's before the exit
+  int need = max(0, rem - eq0), out = gt0 + min(rem, eq0);
+  for (int i0 = p0; i0 < p1; i0 += EV_THREADS) {
+    const int i = i0 + tid;
+    const bool in = i < p1, cand = in && i >= c0 && i < c1;
+    const uint32_t key = cand ? key_of(i) : 0u;
+    const bool tie = cand && !none && key == thr, sure = in && (!cand || (!none && key > thr));
+    // one scan of both: ties in the high half
+    int at;
+    const int tot = ev_scan(int(sure) | int(tie) << 16, &at, warp_sums);
+    const int ties = at >> 16, place = out + (at & 0xffff) + min(ties, need);
+    if (sure || (tie && ties < need)) kept[place] = i;
+    out += (tot & 0xffff) + min(tot >> 16, need);
+    need -= min(need, tot >> 16);
+  }
+  cluster_wait();
 }
 
-// Copies survivor i of a (sequence, kv head) to slot i of the destination: one
-// warp a row, keys then values; a row's units are stored in another order in
-// another slot.
+// Copies survivors to slots 0, 1, ... of the destination: eight lanes a row (a
+// unit each; a row's units are stored in another order in another slot), keys
+// and values, two rows a lane group.
+constexpr int EC_ROWS = 64;  // survivors a block
+template <int HD>
 __global__ void __launch_bounds__(256) k_kv4_evict_copy(const Kv4EvictArgs a) {
+  constexpr int NW = HD / 64;
   const Kv4Geo& g = a.g;
-  const int seq = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31;
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int seq = blockIdx.z, h = blockIdx.y, u = threadIdx.x & 7;
   const int len = kv4_len(a.b, seq), nl = min(len, a.keep);
-  if (i >= nl) return;
+  const int i0 = blockIdx.x * EC_ROWS + (threadIdx.x >> 3);
   const int64_t pair = int64_t(seq) * g.kvh + h;
-  const int src = a.kept[pair * a.kstride + i];
-  const uint8_t* from = kv4_block(g, g.table, g.tstride, seq, h, src, a.b.status);
-  uint8_t* to = kv4_block(g, a.dst, a.dstride, seq, h, i, a.b.status);
-  if (!from || !to) return;
-  const int ts = src & (g.seg - 1), td = i & (g.seg - 1), wpu = g.hd / 64, mix = kv4_swz(g.hd, ts) ^ kv4_swz(g.hd, td);
-  for (int kv = 0; kv < 2; ++kv, from += g.blk / 2, to += g.blk / 2) {
-    const uint32_t* s = reinterpret_cast<const uint32_t*>(from + ts * (g.hd / 2));
-    uint32_t* d = reinterpret_cast<uint32_t*>(to + td * (g.hd / 2));
-    if (lane < 8 * wpu) d[(((lane / wpu) ^ mix) * wpu) + lane % wpu] = s[lane];
-    const uint32_t* sp = reinterpret_cast<const uint32_t*>(from + g.seg * (g.hd / 2)) + ts * g.ng;
-    uint32_t* dp = reinterpret_cast<uint32_t*>(to + g.seg * (g.hd / 2)) + td * g.ng;
-    if (lane < g.ng) dp[lane] = sp[lane];
+  int src[2], slot[2];
+  const uint8_t* from[2];
+  uint8_t* to[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    slot[k] = i0 + 32 * k;
+    src[k] = slot[k] < nl ? a.kept[pair * a.kstride + slot[k]] : -1;
   }
-  if (a.new_weights && lane == 0) a.new_weights[pair * a.nwstride + i] = a.weights[pair * a.wstride + src];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    from[k] = src[k] >= 0 ? kv4_block(g, g.table, g.tstride, seq, h, src[k], a.b.status) : nullptr;
+    to[k] = src[k] >= 0 ? kv4_block(g, a.dst, a.dstride, seq, h, slot[k], a.b.status) : nullptr;
+  }
+  uint32_t c[2][2][NW], p[2][2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+      if (from[k] && to[k]) {
+        const int t = src[k] & (g.seg - 1);
+        const uint8_t* f = from[k] + kv * (g.blk / 2);
+        kv4_ldv(f + t * (HD / 2) + (u ^ kv4_swz(HD, t)) * (HD / 16), c[k][kv]);
+        if (u < g.ng) p[k][kv] = reinterpret_cast<const uint32_t*>(f + g.seg * (HD / 2))[t * g.ng + u];
+      }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (from[k] && to[k])
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int t = slot[k] & (g.seg - 1);
+        uint8_t* d = to[k] + kv * (g.blk / 2);
+        kv4_stv(d + t * (HD / 2) + (u ^ kv4_swz(HD, t)) * (HD / 16), c[k][kv]);
+        if (u < g.ng) reinterpret_cast<uint32_t*>(d + g.seg * (HD / 2))[t * g.ng + u] = p[k][kv];
+      }
+    if (a.new_weights && u == 0 && src[k] >= 0) a.new_weights[pair * a.nwstride + slot[k]] = a.weights[pair * a.wstride + src[k]];
+  }
 }
 
 // ------------------------------------------------------------- arguments --
@@ -408,9 +536,13 @@ void launch_kv4_append(const Kv4IoArgs& a, int dt, cudaStream_t st) { launch_io<
 void launch_kv4_read(const Kv4IoArgs& a, int dt, cudaStream_t st) { launch_io<true>(a, dt, st); }
 
 void launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t st) {
-  launch(k_kv4_evict_select, dim3(a.g.kvh, a.b.nseq), dim3(EV_THREADS), 0, st, false, a);
+  launch_cluster(k_kv4_evict_select, dim3(EV_CL, a.g.kvh, a.b.nseq), dim3(EV_THREADS), dim3(EV_CL, 1, 1), EV_SMEM, st, false, a);
   const int most = std::min(a.keep, a.b.max_len);
-  if (most > 0) launch(k_kv4_evict_copy, dim3((most + 7) / 8, a.g.kvh, a.b.nseq), dim3(256), 0, st, false, a);
+  if (most < 1) return;
+  const dim3 grid((most + EC_ROWS - 1) / EC_ROWS, a.g.kvh, a.b.nseq), block(256);
+  if (a.g.hd == 64) launch(k_kv4_evict_copy<64>, grid, block, 0, st, false, a);
+  else if (a.g.hd == 128) launch(k_kv4_evict_copy<128>, grid, block, 0, st, false, a);
+  else launch(k_kv4_evict_copy<256>, grid, block, 0, st, false, a);
 }
 
 }  // namespace swl

@@ -195,6 +195,12 @@ __device__ __forceinline__ void kv4_ldv(const uint8_t* p, uint32_t (&w)[N]) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
+template <int N>
+__device__ __forceinline__ void kv4_stv(uint8_t* p, const uint32_t (&w)[N]) {
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
 // Scale and bias of a group from its word.
 __device__ __forceinline__ float2 kv4_param(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
