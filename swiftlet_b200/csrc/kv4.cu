@@ -24,6 +24,18 @@ namespace {
 // both: it reads back as NaN instead of as something plausible.
 constexpr int IO_THREADS = 256;
 
+// Minimum and maximum that are NaN when either operand is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <int DT>
 __device__ __forceinline__ void load8(const uint8_t* p, int64_t i, bool vec, float (&x)[8]) {
   if (DT == DT_F32) {
@@ -91,19 +103,19 @@ constexpr int IO_TOKENS = 16;  // tokens of a block at most
 constexpr int IO_U = 4;        // rows a warp has in flight
 
 template <int DT, bool READ>
-__global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool vk, bool vv, int tokens) {
+__global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool vk, bool vv, int tshift) {
   __shared__ IoToken tok[IO_TOKENS];
   const Kv4Geo& g = a.g;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j0 = blockIdx.x * tokens;
-  const int lpr = g.hd / 8, rpw = 32 / lpr;  // lanes a row, rows a warp
-  const int sub = lane / lpr, l = lane % lpr;
+  const int tokens = 1 << tshift, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j0 = blockIdx.x * tokens;
+  const int ls = g.hd == 256 ? 5 : g.hd == 128 ? 4 : 3, rpw = 32 >> ls;  // log2 of the lanes a row, rows a warp
+  const int sub = lane >> ls, l = lane & ((1 << ls) - 1), gs = g.group == 64 ? 3 : 4;  // log2 of the lanes a group
   const int rows = tokens * g.kvh * 2;       // row = (head, K or V) * tokens + token
   const int step = IO_THREADS / 32 * rpw;
   const int nb = g.page / g.seg;
   float x[IO_U][8];
   auto place = [&](int rid, int& j, int& h, int& kv) {
-    const int hk = rid / tokens;
-    j = j0 + rid - hk * tokens;
+    const int hk = rid >> tshift;
+    j = j0 + (rid & (tokens - 1));
     h = hk >> 1;
     kv = hk & 1;
     return rid < rows && j < a.b.total;
@@ -149,7 +161,7 @@ __global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool v
       if (READ && at[u]) {
         const int t = tok[j - j0].t;
         w[u] = *reinterpret_cast<const uint32_t*>(at[u] + t * (g.hd / 2) + ((l & 7) ^ kv4_swz(g.hd, t)) * (g.hd / 16) + (l >> 3) * 4);
-        pr[u] = reinterpret_cast<const uint32_t*>(at[u] + g.seg * (g.hd / 2))[t * g.ng + l * 8 / g.group];
+        pr[u] = reinterpret_cast<const uint32_t*>(at[u] + g.seg * (g.hd / 2))[t * g.ng + (l >> gs)];
       }
     }
 #pragma unroll
@@ -160,38 +172,44 @@ __global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool v
         if (!on) continue;
         const Kv4Rows& r = kv ? a.v : a.k;
         const float2 sb = kv4_param(pr[u]);
+        // a code at bit 4e of 2^23's mantissa is 2^23 + 16^e c; s c is exact, so
+        // one rounding remains
+        const float s16[5] = {sb.x, sb.x * 0x1p-4f, sb.x * 0x1p-8f, sb.x * 0x1p-12f, sb.x * 0x1p-16f};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[u][e] = __fadd_rn(__fmul_rn(sb.x, float((w[u] >> (4 * e)) & 15u)), sb.y);
+        for (int e = 0; e < 8; ++e) {
+          const int at4 = e < 5 ? e : e - 3;
+          const uint32_t bits = (e < 5 ? w[u] : w[u] >> 12) & (15u << (4 * at4));
+          x[u][e] = fmaf(__uint_as_float(bits | 0x4b000000u) - 8388608.f, s16[at4], sb.y);
+        }
         store8<DT>(r.p, j * r.ts + h * r.hs + l * 8, kv ? vv : vk, x[u]);
       } else {
         float mn = x[u][0], mx = x[u][0];
-        bool bad = false;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          mn = fminf(mn, x[u][e]);
-          mx = fmaxf(mx, x[u][e]);
-          bad |= !(fabsf(x[u][e]) < INFINITY);
+        for (int e = 1; e < 8; ++e) {
+          mn = min_nan(mn, x[u][e]);
+          mx = max_nan(mx, x[u][e]);
         }
         for (int o = 1; o < g.group / 8; o <<= 1) {
-          mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          bad |= __shfl_xor_sync(0xffffffffu, int(bad), o) != 0;
+          mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         }
         const __half hb = __float2half_rn(mn), hs = __float2half_rn(__fmul_rn(__fsub_rn(mx, mn), 1.f / 15.f));
         const float b = __half2float(hb), s = __half2float(hs);
-        bad |= !(fabsf(b) < INFINITY) || !(s < INFINITY);
+        const bool bad = !(fabsf(b) < INFINITY) || !(s < INFINITY) || !(mx < INFINITY);
         const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+        // held to [0, 15] first, a value is rounded by adding 1.5 * 2^23: the
+        // code is the sum's last bits, over those of the constant
         uint32_t word = 0u;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[u][e], b), inv)), 0.f), 15.f);
-          word |= uint32_t(int(c)) << (4 * e);
+          const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[u][e], b), inv), 0.f), 15.f);
+          word += (__float_as_uint(__fadd_rn(c, 12582912.f)) - 0x4b400000u) << (4 * e);
         }
         if (!on) continue;
         const IoToken& k = tok[j - j0];
         *reinterpret_cast<uint32_t*>(at[u] + k.t * (g.hd / 2) + ((l & 7) ^ kv4_swz(g.hd, k.t)) * (g.hd / 16) + (l >> 3) * 4) = bad ? 0u : word;
-        if (l * 8 % g.group == 0)
-          reinterpret_cast<uint32_t*>(at[u] + g.seg * (g.hd / 2))[k.t * g.ng + l * 8 / g.group] =
+        if ((l & ((1 << gs) - 1)) == 0)
+          reinterpret_cast<uint32_t*>(at[u] + g.seg * (g.hd / 2))[k.t * g.ng + (l >> gs)] =
               bad ? 0x7e007e00u : uint32_t(__half_as_ushort(hs)) | uint32_t(__half_as_ushort(hb)) << 16;
         if (a.weights && l == 0 && kv == 0) a.weights[(int64_t(k.seq) * g.kvh + h) * a.wstride + k.slot] = 0.f;
       }
@@ -203,12 +221,14 @@ template <bool READ>
 void launch_io(const Kv4IoArgs& a, int dt, cudaStream_t st) {
   // tokens a block: as many as leave four blocks an SM, so that a step of a
   // few tokens still spreads over the GPU
-  const int tokens = std::max(1, std::min(IO_TOKENS, a.b.total / 592));
+  int tshift = 0;
+  while ((2 << tshift) <= IO_TOKENS && (a.b.total >> (tshift + 1)) >= 592) ++tshift;
+  const int tokens = 1 << tshift;
   const bool vk = vec_rows(a.k, dt), vv = vec_rows(a.v, dt);
   const dim3 grid((a.b.total + tokens - 1) / tokens), block(IO_THREADS);
-  if (dt == DT_F32) launch(k_kv4_io<DT_F32, READ>, grid, block, 0, st, false, a, vk, vv, tokens);
-  else if (dt == DT_BF16) launch(k_kv4_io<DT_BF16, READ>, grid, block, 0, st, false, a, vk, vv, tokens);
-  else launch(k_kv4_io<DT_F16, READ>, grid, block, 0, st, false, a, vk, vv, tokens);
+  if (dt == DT_F32) launch(k_kv4_io<DT_F32, READ>, grid, block, 0, st, false, a, vk, vv, tshift);
+  else if (dt == DT_BF16) launch(k_kv4_io<DT_BF16, READ>, grid, block, 0, st, false, a, vk, vv, tshift);
+  else launch(k_kv4_io<DT_F16, READ>, grid, block, 0, st, false, a, vk, vv, tshift);
 }
 
 // ---------------------------------------------------------------- evict --
@@ -222,7 +242,7 @@ void launch_io(const Kv4IoArgs& a, int dt, cudaStream_t st) {
 // before it. Bound: the latency of the passes (reads of `len` words); one CTA
 // for all took 130 us at 65536 slots.
 constexpr int EV_THREADS = 1024;
-constexpr int EV_CL = 8;
+constexpr int EV_CL = 8;       // CTAs a cluster at most
 constexpr int EV_BINS = 2048;
 constexpr int EV_KEYS = 16384;  // keys a CTA holds
 constexpr size_t EV_SMEM = EV_KEYS * 4;
@@ -233,6 +253,9 @@ __device__ __forceinline__ uint32_t ev_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+__device__ __forceinline__ void ev_ld2(uint32_t addr, int& a, int& b) {
+  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
+}
 __device__ __forceinline__ int ev_ld(uint32_t addr) {
   int v;
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -270,15 +293,15 @@ __device__ int ev_scan(int v, int* ex, int* warp_sums) {
 
 __global__ void __launch_bounds__(EV_THREADS, 1) k_kv4_evict_select(const Kv4EvictArgs a) {
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[2][EV_BINS];
+  __shared__ __align__(8) int hist[2][EV_BINS];
   __shared__ int warp_sums[33], s_bin, s_above, s_cnt[2];
   const int seq = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
-  const int rank = int(cluster_rank());
+  const int rank = int(cluster_rank()), ncl = gridDim.x;  // one cluster in x
   const int len = kv4_len(a.b, seq), nl = min(len, a.keep);
   if (h == 0 && rank == 0 && tid == 0) a.new_lens[seq] = nl;
   const float* w = a.weights + (int64_t(seq) * a.g.kvh + h) * a.wstride;
   int* kept = a.kept + (int64_t(seq) * a.g.kvh + h) * a.kstride;
-  const int part = (len + EV_CL - 1) / EV_CL, p0 = min(len, rank * part), p1 = min(len, p0 + part);
+  const int part = (len + ncl - 1) / ncl, p0 = min(len, rank * part), p1 = min(len, p0 + part);
   if (nl == len) {  // the whole cluster takes this way
     for (int i = p0 + tid; i < p1; i += EV_THREADS) kept[i] = i;
     return;
@@ -307,8 +330,12 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_kv4_evict_select(const Kv4Evi
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         n[k] = 0;
-        const int bin = EV_BINS - 1 - (2 * tid + k);
-        for (int c = 0; c < EV_CL; ++c) n[k] += ev_ld(dsmem_map(&hs[bin], c));
+      }
+      for (int c = 0; c < ncl; ++c) {
+        int lo, hi;
+        ev_ld2(dsmem_map(&hs[EV_BINS - 2 - 2 * tid], c), lo, hi);
+        n[0] += hi;
+        n[1] += lo;
       }
       ev_scan(n[0] + n[1], &ex, warp_sums);
 #pragma unroll
@@ -536,7 +563,12 @@ void launch_kv4_append(const Kv4IoArgs& a, int dt, cudaStream_t st) { launch_io<
 void launch_kv4_read(const Kv4IoArgs& a, int dt, cudaStream_t st) { launch_io<true>(a, dt, st); }
 
 void launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t st) {
-  launch_cluster(k_kv4_evict_select, dim3(EV_CL, a.g.kvh, a.b.nseq), dim3(EV_THREADS), dim3(EV_CL, 1, 1), EV_SMEM, st, false, a);
+  // as many CTAs a (sequence, head) as one wave of the GPU has for them: 64
+  // x 2 of at most 4608 slots took 52 us with eight each (seven waves), two
+  // of 65536 take 33 us with eight, 130 us with one
+  int cl = EV_CL;
+  while (cl > 1 && int64_t(cl) * a.g.kvh * a.b.nseq > 148) cl >>= 1;
+  launch_cluster(k_kv4_evict_select, dim3(cl, a.g.kvh, a.b.nseq), dim3(EV_THREADS), dim3(cl, 1, 1), EV_SMEM, st, false, a);
   const int most = std::min(a.keep, a.b.max_len);
   if (most < 1) return;
   const dim3 grid((most + EC_ROWS - 1) / EC_ROWS, a.g.kvh, a.b.nseq), block(256);

@@ -144,8 +144,9 @@ __device__ __forceinline__ Place find_place(const Kv4AttnArgs& a, int64_t flat) 
       const int src = __ffs(hit) - 1;
       const int64_t before = base + __shfl_sync(0xffffffffu, incl - cnt, src);
       load_seq(a, i0 + src, p);
-      p.item = int((flat - before) / p.tiles);
-      p.tile = int((flat - before) % p.tiles);
+      const int64_t rem = flat - before;
+      p.item = rem >> 32 ? int(rem / p.tiles) : int(unsigned(rem) / unsigned(p.tiles));
+      p.tile = int(rem - int64_t(p.item) * p.tiles);
       return p;
     }
     base += __shfl_sync(0xffffffffu, incl, 31);
@@ -288,9 +289,18 @@ struct AttnShared {
 __host__ __device__ constexpr int part_floats(int hd) { return 2 * AT_COLS + AT_COLS * hd; }
 
 __device__ __forceinline__ float* attn_lse(const Kv4AttnArgs& a) { return a.lse ? a.lse : reinterpret_cast<float*>(a.work); }
-__device__ __forceinline__ float* attn_parts(const Kv4AttnArgs& a) {
-  return reinterpret_cast<float*>(a.work + (int64_t(a.b.total) * a.heads * 4 + 15) / 16 * 16);
+// The item that begins in a share and goes on: shares first .. last hold its
+// parts (first < 0: none).
+struct AtJoin {
+  int first, last, row0, n, cb, h, every, pad;  // every: no share is empty
+};
+__device__ __forceinline__ AtJoin* attn_joins(const Kv4AttnArgs& a) {
+  return reinterpret_cast<AtJoin*>(a.work + (int64_t(a.b.total) * a.heads * 4 + 15) / 16 * 16);
 }
+__device__ __forceinline__ float* attn_parts(const Kv4AttnArgs& a) { return reinterpret_cast<float*>(attn_joins(a) + AT_GRID); }
+// First tile of a share, and the share that a tile is in.
+__device__ __forceinline__ int64_t share_begin(int64_t total, int x) { return total * x / AT_GRID; }
+__device__ __forceinline__ int share_of(int64_t total, int64_t tile) { return int(((tile + 1) * AT_GRID + total - 1) / total) - 1; }
 
 // One output of a row, gated.
 __device__ __forceinline__ void write_out(const Kv4AttnArgs& a, int64_t row, int hq, int ch, float v) {
@@ -307,7 +317,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch();
   const int64_t total = total_tiles(a);
-  const int64_t r0 = total * blockIdx.x / gridDim.x, r1 = total * (blockIdx.x + 1) / gridDim.x;
+  const int64_t r0 = share_begin(total, blockIdx.x), r1 = share_begin(total, blockIdx.x + 1);
+  if (threadIdx.x == 0) attn_joins(a)[blockIdx.x].first = -1;
   if (r0 == r1) return;
   Place p = find_place(a, r0);
   const Kv4Geo& g = a.g;
@@ -324,6 +335,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
     const int v1 = int(min(int64_t(p.tiles), p.tile + (r1 - f)));
     // real tiles tb .. t1 - 1; the item's first part of several goes to slot 1, a later one (the share's first) to slot 0
     const int tb = max(0, p.tile - AT_HEAD), t1 = v1 - AT_HEAD, slot = p.tile == 0 ? 1 : 0;
+    if (threadIdx.x == 0 && p.tile == 0 && v1 < p.tiles) {
+      const int first = share_of(total, f + AT_HEAD), last = share_of(total, f + p.tiles - 1);
+      if (first < last) attn_joins(a)[blockIdx.x] = AtJoin{first, last, p.row0, p.n, cb, h, total >= AT_GRID, 0};
+    }
     f += v1 - p.tile;
     if (t1 <= 0) continue;  // only overhead of the next share's item
     // units u0, u0 + 16, ... < u1 are this warp's
@@ -611,38 +626,26 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
 }
 
 // Joins the parts of the item that begins in share x and goes on: one block per
-// (share, column).
+// (share, column), a thread a channel.
 template <int HD>
 __global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
-  const int nc = gridDim.x, x = blockIdx.x, col = blockIdx.y;
-  const int64_t total = total_tiles(a);
-  const int64_t r0 = total * x / nc, r1 = total * (x + 1) / nc;
-  Place p = {};
-  if (r0 < r1) p = find_place(a, r1 - 1);
-  const int64_t begin = r1 - 1 - p.tile, end = begin + p.tiles;
-  const int h = p.item % a.g.kvh, cb = p.item / a.g.kvh;
-  const int ci = cb * AT_COLS + col, tok = ci / a.rep, hq = h * a.rep + ci % a.rep;
-  pdl_wait();  // by every block: this launch ends after the one before it
-  if (r0 == r1 || begin < r0 || end <= r1 || tok >= p.n) return;
+  pdl_wait();
+  const int x = blockIdx.x, col = blockIdx.y;
+  const AtJoin d = attn_joins(a)[x];
+  if (d.first < 0) return;
+  const int ci = d.cb * AT_COLS + col, tok = ci / a.rep, hq = d.h * a.rep + ci % a.rep;
+  if (tok >= d.n) return;
   __shared__ float wt[AT_GRID];
   __shared__ float red[32];
   const float* parts = attn_parts(a);
   auto part = [&](int i) { return parts + (int64_t(i) * 2 + (i == x ? 1 : 0)) * part_floats(HD); };
-  // shares x .. last hold parts of the item, those with no tile of it none
-  int last = x;
-  while (last + 1 < nc && total * (last + 1) / nc < end) ++last;
-  const int np = last - x + 1;
-  auto has = [&](int i) {
-    const int64_t lo = max(begin + AT_HEAD, total * (x + i) / nc), hi = min(end, total * (x + i + 1) / nc);
-    return lo < hi;
-  };
-  // all its tiles in one share: written there
-  int one = x;
-  while (total * (one + 1) / nc <= begin + AT_HEAD) ++one;
-  if (one == last) return;
+  int64_t total = 0;
+  if (!d.every) total = total_tiles(a);  // fewer tiles than shares: the empty ones have no part
+  const int np = d.last - d.first + 1;
   float M = -INFINITY;
   for (int i = threadIdx.x; i < np; i += HD) {
-    const float mi = has(i) ? __ldcg(part(x + i) + col) : -INFINITY;
+    const bool has = d.every || share_begin(total, d.first + i) < share_begin(total, d.first + i + 1);
+    const float mi = has ? __ldcg(part(d.first + i) + col) : -INFINITY;
     wt[i] = mi;
     M = fmaxf(M, mi);
   }
@@ -655,7 +658,7 @@ __global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
   float L = 0.f;
   for (int i = threadIdx.x; i < np; i += HD) {
     const float mi = wt[i], f = mi == -INFINITY ? 0.f : ex2(mi - M);
-    if (mi != -INFINITY) L += __ldcg(part(x + i) + AT_COLS + col) * f;
+    if (mi != -INFINITY) L += __ldcg(part(d.first + i) + AT_COLS + col) * f;
     wt[i] = f;
   }
   L = block_sum(L, red);
@@ -663,10 +666,10 @@ __global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
 #pragma unroll 8
   for (int i = 0; i < np; ++i) {
     const float f = wt[i];
-    if (f != 0.f) v = fmaf(f, __ldcg(part(x + i) + 2 * AT_COLS + col * HD + threadIdx.x), v);
+    if (f != 0.f) v = fmaf(f, __ldcg(part(d.first + i) + 2 * AT_COLS + col * HD + threadIdx.x), v);
   }
   v = M == -INFINITY ? 0.f : v / L;
-  const int64_t row = p.row0 + tok;
+  const int64_t row = d.row0 + tok;
   write_out(a, row, hq, threadIdx.x, v);
   if (threadIdx.x == 0) attn_lse(a)[row * a.heads + hq] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * LN2;
 }
@@ -778,7 +781,7 @@ void run_dt(const Kv4AttnArgs& a, cudaStream_t st) {
 
 int64_t kv4_attention_work(const Kv4Geo& g, const Kv4Batch& b, int heads) {
   if (!few_rows(b, heads / g.kvh)) return kv4_prompt_work(g, b, heads);
-  return (int64_t(b.total) * heads * 4 + 15) / 16 * 16 + int64_t(AT_GRID) * 2 * part_floats(g.hd) * 4;
+  return (int64_t(b.total) * heads * 4 + 15) / 16 * 16 + AT_GRID * int64_t(sizeof(AtJoin)) + int64_t(AT_GRID) * 2 * part_floats(g.hd) * 4;
 }
 
 void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {

@@ -215,11 +215,11 @@ __device__ __forceinline__ PtPlace pt_find(const Kv4AttnArgs& a, int bn, int64_t
       const unsigned hit = __ballot_sync(0xffffffffu, base + incl > flat);
       if (hit) {
         const int src = __ffs(hit) - 1;
-        const int64_t rem = flat - base - __shfl_sync(0xffffffffu, incl - cnt, src);
+        const unsigned rem = unsigned(flat - base - __shfl_sync(0xffffffffu, incl - cnt, src));
         p.qt = q0 + src;
         p.tiles = pt_tiles(p.n, p.len, a.rep, bn, p.qt);
-        p.h = int(rem / p.tiles);
-        p.tile = int(rem % p.tiles);
+        p.h = int(rem / unsigned(p.tiles));
+        p.tile = int(rem % unsigned(p.tiles));
         return p;
       }
       base += __shfl_sync(0xffffffffu, incl, 31);
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
   const uint32_t tmem = *tmem_slot;
   pdl_launch();
   const int64_t total = pt_total(a, BN);
-  const int64_t r0 = total * blockIdx.x / gridDim.x, r1 = total * (blockIdx.x + 1) / gridDim.x;
+  const int64_t r0 = total * blockIdx.x / PT_GRID, r1 = total * (blockIdx.x + 1) / PT_GRID;
   pdl_wait();  // the ranges
   auto fail = [&]() {
     if (a.b.status) atomicOr(a.b.status, 1);
@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         const PtPlace p = pt_find(a, BN, r1 - 1);
         const int64_t begin = r1 - 1 - p.tile, end = begin + p.tiles;
         if (begin >= r0 && end > r1) {
-          const int nc = gridDim.x;
+          const int nc = PT_GRID;
           int first = blockIdx.x, last = blockIdx.x;
           while (total * (first + 1) / nc <= begin + PT_HEAD) ++first;
           while (last + 1 < nc && total * (last + 1) / nc < end) ++last;
