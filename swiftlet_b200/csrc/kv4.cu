@@ -93,110 +93,100 @@ bool vec_rows(const Kv4Rows& r, int dt) {
   return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.ts * e % 16 == 0 && r.hs * e % 16 == 0;
 }
 
-// Where a token of the block goes: its slot's block for kv head 0 (null: no
-// slot, or a page outside the pool), the row in it, the sequence and slot.
-struct IoToken {
-  uint8_t* blk;
-  int t, seq, slot;
-};
-constexpr int IO_TOKENS = 16;  // tokens of a block at most
-constexpr int IO_U = 4;        // rows a warp has in flight
+//
+// A warp takes 1 << tshift consecutive tokens and, of each, IO_U rows at a time
+// (K and V of some heads). The tokens' places (sequence, slot, page) are looked
+// up by a lane each. Bound: the rows' bytes in and out, next to about 100
+// instructions a row of quantising.
+constexpr int IO_TOKENS = 8;  // tokens of a warp at most
+constexpr int IO_U = 4;       // rows a warp has in flight
 
-template <int DT, bool READ>
+template <int DT, bool READ, int HD, int GROUP>
 __global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool vk, bool vv, int tshift) {
-  __shared__ IoToken tok[IO_TOKENS];
+  constexpr int LPR = HD / 8, RPW = 32 / LPR, NG = HD / GROUP;  // lanes a row, rows a warp, groups a row
   const Kv4Geo& g = a.g;
-  const int tokens = 1 << tshift, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j0 = blockIdx.x * tokens;
-  const int ls = g.hd == 256 ? 5 : g.hd == 128 ? 4 : 3, rpw = 32 >> ls;  // log2 of the lanes a row, rows a warp
-  const int sub = lane >> ls, l = lane & ((1 << ls) - 1), gs = g.group == 64 ? 3 : 4;  // log2 of the lanes a group
-  const int rows = tokens * g.kvh * 2;       // row = (head, K or V) * tokens + token
-  const int step = IO_THREADS / 32 * rpw;
-  const int nb = g.page / g.seg;
-  float x[IO_U][8];
-  auto place = [&](int rid, int& j, int& h, int& kv) {
-    const int hk = rid >> tshift;
-    j = j0 + (rid & (tokens - 1));
-    h = hk >> 1;
-    kv = hk & 1;
-    return rid < rows && j < a.b.total;
-  };
-  auto fetch = [&](int base) {  // what the inputs alone determine
-#pragma unroll
-    for (int u = 0; u < IO_U; ++u) {
-      int j, h, kv;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
-      if (!place(base + u * step + sub, j, h, kv)) continue;
-      const Kv4Rows& r = kv ? a.v : a.k;
-      load8<DT>(r.p, j * r.ts + h * r.hs + l * 8, kv ? vv : vk, x[u]);
+  const int lane = threadIdx.x & 31, sub = lane / LPR, l = lane % LPR;
+  const int64_t j0 = (int64_t(blockIdx.x) * (IO_THREADS / 32) + (threadIdx.x >> 5)) << tshift;
+  if (j0 >= a.b.total) return;
+  const int n_tok = int(min(int64_t(1) << tshift, a.b.total - j0));
+  // lane i: where token j0 + i goes
+  uint8_t* blk = nullptr;
+  int slot = 0, seq = 0;
+  if (lane < n_tok) {
+    // the last sequence that starts at or before the token
+    int lo = 0, hi = a.b.nseq;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(a.b.start + mid + 1) <= j0 + lane) lo = mid + 1; else hi = mid;
     }
-  };
-  if (!READ) fetch(warp * rpw);
-  for (int i = warp; i < tokens; i += IO_THREADS / 32) {
-    const int j = j0 + i;
-    IoToken t = {nullptr, 0, 0, 0};
-    const int seq = j < a.b.total ? kv4_seq_of(a.b, j) : -1;
-    if (seq >= 0) {
-      int row0;
+    seq = lo;
+    int row0 = 0;
+    if (seq < a.b.nseq) {
       const int n = kv4_new(a.b, seq, row0), len = kv4_len(a.b, seq);
-      t.slot = len - n + (j - row0);
-      t.seq = seq;
-      t.t = t.slot & (g.seg - 1);
+      slot = len - n + int(j0 + lane - row0);
       // a negative slot: more new tokens than slots, the first of them have none
-      if (t.slot >= 0 && t.slot < len) t.blk = kv4_block(g, g.table, g.tstride, seq, 0, t.slot, a.b.status);
+      if (j0 + lane >= row0 && slot >= 0 && slot < len) blk = kv4_block(g, g.table, g.tstride, seq, 0, slot, a.b.status);
     }
-    if (lane == 0) tok[i] = t;
   }
-  __syncthreads();
-  for (int base = warp * rpw; base < rows; base += step * IO_U) {
-    if (!READ && base != warp * rpw) fetch(base);
-    uint32_t w[IO_U], pr[IO_U];
-    uint8_t* at[IO_U];
+  const int64_t hblk = int64_t(g.page / g.seg) * g.blk;
+  for (int i = 0; i < n_tok; ++i) {
+    uint8_t* const tb = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(blk), i));
+    if (!tb) continue;
+    const int s = __shfl_sync(0xffffffffu, slot, i), sq = __shfl_sync(0xffffffffu, seq, i), t = s & (g.seg - 1);
+    const int wo = t * (HD / 2) + ((l & 7) ^ kv4_swz(HD, t)) * (HD / 16) + (l >> 3) * 4, po = g.seg * (HD / 2) + (t * NG + l * 8 / GROUP) * 4;
+    const int64_t kj = (j0 + i) * a.k.ts + l * 8, vj = (j0 + i) * a.v.ts + l * 8;
+    for (int h0 = sub; h0 - sub < g.kvh; h0 += IO_U / 2 * RPW) {
+      float x[IO_U][8];
+      uint32_t w[IO_U], pr[IO_U];
 #pragma unroll
-    for (int u = 0; u < IO_U; ++u) {
-      int j, h, kv;
-      at[u] = nullptr;
-      if (place(base + u * step + sub, j, h, kv) && tok[j - j0].blk)
-        at[u] = tok[j - j0].blk + int64_t(h) * nb * g.blk + (kv ? g.blk / 2 : 0);
-      if (READ && at[u]) {
-        const int t = tok[j - j0].t;
-        w[u] = *reinterpret_cast<const uint32_t*>(at[u] + t * (g.hd / 2) + ((l & 7) ^ kv4_swz(g.hd, t)) * (g.hd / 16) + (l >> 3) * 4);
-        pr[u] = reinterpret_cast<const uint32_t*>(at[u] + g.seg * (g.hd / 2))[t * g.ng + (l >> gs)];
-      }
-    }
+      for (int u = 0; u < IO_U; ++u) {
+        const int h = h0 + (u >> 1) * RPW, kv = u & 1;
+        w[u] = pr[u] = 0u;
+        if (!READ)
 #pragma unroll
-    for (int u = 0; u < IO_U; ++u) {
-      int j, h, kv;
-      const bool on = place(base + u * step + sub, j, h, kv) && at[u];
-      if (READ) {
-        if (!on) continue;
-        const Kv4Rows& r = kv ? a.v : a.k;
-        const float2 sb = kv4_param(pr[u]);
-        // a code at bit 4e of 2^23's mantissa is 2^23 + 16^e c; s c is exact, so
-        // one rounding remains
-        const float s16[5] = {sb.x, sb.x * 0x1p-4f, sb.x * 0x1p-8f, sb.x * 0x1p-12f, sb.x * 0x1p-16f};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int at4 = e < 5 ? e : e - 3;
-          const uint32_t bits = (e < 5 ? w[u] : w[u] >> 12) & (15u << (4 * at4));
-          x[u][e] = fmaf(__uint_as_float(bits | 0x4b000000u) - 8388608.f, s16[at4], sb.y);
+          for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
+        if (h >= g.kvh) continue;
+        if (READ) {
+          const uint8_t* d = tb + h * hblk + (kv ? g.blk / 2 : 0);
+          w[u] = *reinterpret_cast<const uint32_t*>(d + wo);
+          pr[u] = *reinterpret_cast<const uint32_t*>(d + po);
+        } else {
+          load8<DT>(kv ? a.v.p : a.k.p, kv ? vj + h * a.v.hs : kj + h * a.k.hs, kv ? vv : vk, x[u]);
         }
-        store8<DT>(r.p, j * r.ts + h * r.hs + l * 8, kv ? vv : vk, x[u]);
-      } else {
+      }
+#pragma unroll
+      for (int u = 0; u < IO_U; ++u) {
+        const int h = h0 + (u >> 1) * RPW, kv = u & 1;
+        if (READ) {
+          if (h >= g.kvh) continue;
+          const float2 sb = kv4_param(pr[u]);
+          // a code at bit 4e of 2^23's mantissa is 2^23 + 16^e c; s c is exact, so
+          // one rounding remains
+          const float s16[5] = {sb.x, sb.x * 0x1p-4f, sb.x * 0x1p-8f, sb.x * 0x1p-12f, sb.x * 0x1p-16f};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int at4 = e < 5 ? e : e - 3;
+            const uint32_t bits = (e < 5 ? w[u] : w[u] >> 12) & (15u << (4 * at4));
+            x[u][e] = fmaf(__uint_as_float(bits | 0x4b000000u) - 8388608.f, s16[at4], sb.y);
+          }
+          store8<DT>(kv ? a.v.p : a.k.p, kv ? vj + h * a.v.hs : kj + h * a.k.hs, kv ? vv : vk, x[u]);
+          continue;
+        }
         float mn = x[u][0], mx = x[u][0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) {
           mn = min_nan(mn, x[u][e]);
           mx = max_nan(mx, x[u][e]);
         }
-        for (int o = 1; o < g.group / 8; o <<= 1) {
+#pragma unroll
+        for (int o = 1; o < GROUP / 8; o <<= 1) {
           mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         }
         const __half hb = __float2half_rn(mn), hs = __float2half_rn(__fmul_rn(__fsub_rn(mx, mn), 1.f / 15.f));
-        const float b = __half2float(hb), s = __half2float(hs);
-        const bool bad = !(fabsf(b) < INFINITY) || !(s < INFINITY) || !(mx < INFINITY);
-        const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+        const float b = __half2float(hb), sc = __half2float(hs);
+        const bool bad = !(fabsf(b) < INFINITY) || !(sc < INFINITY) || !(mx < INFINITY);
+        const float inv = sc > 0.f ? __frcp_rn(sc) : 0.f;
         // held to [0, 15] first, a value is rounded by adding 1.5 * 2^23: the
         // code is the sum's last bits, over those of the constant
         uint32_t word = 0u;
@@ -205,30 +195,38 @@ __global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool v
           const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[u][e], b), inv), 0.f), 15.f);
           word += (__float_as_uint(__fadd_rn(c, 12582912.f)) - 0x4b400000u) << (4 * e);
         }
-        if (!on) continue;
-        const IoToken& k = tok[j - j0];
-        *reinterpret_cast<uint32_t*>(at[u] + k.t * (g.hd / 2) + ((l & 7) ^ kv4_swz(g.hd, k.t)) * (g.hd / 16) + (l >> 3) * 4) = bad ? 0u : word;
-        if ((l & ((1 << gs) - 1)) == 0)
-          reinterpret_cast<uint32_t*>(at[u] + g.seg * (g.hd / 2))[k.t * g.ng + (l >> gs)] =
-              bad ? 0x7e007e00u : uint32_t(__half_as_ushort(hs)) | uint32_t(__half_as_ushort(hb)) << 16;
-        if (a.weights && l == 0 && kv == 0) a.weights[(int64_t(k.seq) * g.kvh + h) * a.wstride + k.slot] = 0.f;
+        if (h >= g.kvh) continue;
+        uint8_t* d = tb + h * hblk + (kv ? g.blk / 2 : 0);
+        *reinterpret_cast<uint32_t*>(d + wo) = bad ? 0u : word;
+        if (l % (GROUP / 8) == 0)
+          *reinterpret_cast<uint32_t*>(d + po) = bad ? 0x7e007e00u : uint32_t(__half_as_ushort(hs)) | uint32_t(__half_as_ushort(hb)) << 16;
+        if (a.weights && l == 0 && kv == 0) a.weights[(int64_t(sq) * g.kvh + h) * a.wstride + s] = 0.f;
       }
     }
   }
 }
 
-template <bool READ>
-void launch_io(const Kv4IoArgs& a, int dt, cudaStream_t st) {
-  // tokens a block: as many as leave four blocks an SM, so that a step of a
+template <int DT, bool READ>
+void launch_io_dt(const Kv4IoArgs& a, cudaStream_t st) {
+  // tokens a warp: as many as leave sixteen warps an SM, so that a step of a
   // few tokens still spreads over the GPU
   int tshift = 0;
-  while ((2 << tshift) <= IO_TOKENS && (a.b.total >> (tshift + 1)) >= 592) ++tshift;
-  const int tokens = 1 << tshift;
-  const bool vk = vec_rows(a.k, dt), vv = vec_rows(a.v, dt);
-  const dim3 grid((a.b.total + tokens - 1) / tokens), block(IO_THREADS);
-  if (dt == DT_F32) launch(k_kv4_io<DT_F32, READ>, grid, block, 0, st, false, a, vk, vv, tshift);
-  else if (dt == DT_BF16) launch(k_kv4_io<DT_BF16, READ>, grid, block, 0, st, false, a, vk, vv, tshift);
-  else launch(k_kv4_io<DT_F16, READ>, grid, block, 0, st, false, a, vk, vv, tshift);
+  while ((2 << tshift) <= IO_TOKENS && (a.b.total >> (tshift + 1)) >= 148 * 16) ++tshift;
+  const int per = IO_THREADS / 32 << tshift;
+  const bool vk = vec_rows(a.k, DT), vv = vec_rows(a.v, DT);
+  const dim3 grid((a.b.total + per - 1) / per), block(IO_THREADS);
+  if (a.g.hd == 64) launch(k_kv4_io<DT, READ, 64, 64>, grid, block, 0, st, false, a, vk, vv, tshift);
+  else if (a.g.hd == 128 && a.g.group == 64) launch(k_kv4_io<DT, READ, 128, 64>, grid, block, 0, st, false, a, vk, vv, tshift);
+  else if (a.g.hd == 128) launch(k_kv4_io<DT, READ, 128, 128>, grid, block, 0, st, false, a, vk, vv, tshift);
+  else if (a.g.group == 64) launch(k_kv4_io<DT, READ, 256, 64>, grid, block, 0, st, false, a, vk, vv, tshift);
+  else launch(k_kv4_io<DT, READ, 256, 128>, grid, block, 0, st, false, a, vk, vv, tshift);
+}
+
+template <bool READ>
+void launch_io(const Kv4IoArgs& a, int dt, cudaStream_t st) {
+  if (dt == DT_F32) launch_io_dt<DT_F32, READ>(a, st);
+  else if (dt == DT_BF16) launch_io_dt<DT_BF16, READ>(a, st);
+  else launch_io_dt<DT_F16, READ>(a, st);
 }
 
 // ---------------------------------------------------------------- evict --

@@ -118,14 +118,6 @@ __device__ __forceinline__ int kv4_new(const Kv4Batch& b, int seq, int& row0) {
   return max(0, s1 - s0);
 }
 
-// Sequence that row j belongs to, or -1 (whole warp; every lane gets it).
-__device__ __forceinline__ int kv4_seq_of(const Kv4Batch& b, int j) {
-  int n = 0;
-  for (int i = threadIdx.x & 31; i <= b.nseq; i += 32) n += __ldg(b.start + i) <= j;
-  n = __reduce_add_sync(0xffffffffu, n) - 1;
-  return n >= 0 && n < b.nseq ? n : -1;
-}
-
 __device__ __forceinline__ float kv4_ld(const uint8_t* p, int dt, int64_t i) {
   if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
   const uint16_t u = reinterpret_cast<const uint16_t*>(p)[i];
