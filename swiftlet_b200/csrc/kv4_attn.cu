@@ -39,7 +39,7 @@ constexpr int AT_WARPS = 12;                // three per scheduler at 168 regist
 constexpr int AT_THREADS = AT_WARPS * 32;
 constexpr int AT_UNIT = 16;                 // slots a warp takes at a time: the MMA's M (keys) and K (values)
 constexpr int AT_TILE = 128;                // slots of a tile, the grain in which work is shared out
-constexpr int AT_HEAD = 2;                  // what an item costs beside its tiles, in tiles
+constexpr int AT_HEAD = 4;                  // what an item costs beside its tiles, in tiles
 constexpr int AT_COLS = 8;                  // query columns (token, head) of an item: the MMA's N
 constexpr int AT_GRID = 148;                // one CTA per SM
 constexpr int WT_WARPS = 8;                 // warps of the weight kernel: one tile
@@ -236,40 +236,48 @@ __device__ __forceinline__ void stage_q(const Kv4AttnArgs& a, const Place& p, in
 template <int HD, int GROUP, bool SPLIT, typename QF>
 __device__ __forceinline__ void scores(const uint32_t (&kw)[2][2][HD / 64], const uint32_t (&kp)[2][HD / GROUP],
                                        const float (&qsum)[2][HD / GROUP], QF qf, float (&sc)[4]) {
+  // the groups' sums side by side: one chain of products each, so that a
+  // product does not wait for the one before it
+  constexpr int NG = HD / GROUP;
+  float acc[NG][4];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.f;
+#pragma unroll
+  for (int w = 0; w < GROUP / 64; ++w)
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        uint32_t a0[NG], a1[NG], a2[NG], a3[NG], b[NG][SPLIT ? 4 : 2];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const int wi = g * (GROUP / 64) + w;
+          if (SPLIT) {
+            unpack_centred(st ? kw[hf][0][wi] >> 7 : kw[hf][0][wi] << 1, a0[g], a2[g]);
+            unpack_centred(st ? kw[hf][1][wi] >> 7 : kw[hf][1][wi] << 1, a1[g], a3[g]);
+          } else {
+            unpack_plain(st ? kw[hf][0][wi] >> 8 : kw[hf][0][wi], a0[g], a2[g]);
+            unpack_plain(st ? kw[hf][1][wi] >> 8 : kw[hf][1][wi], a1[g], a3[g]);
+          }
+          qf((wi * 2 + hf) * 2 + st, b[g]);
+          mma16816(acc[g], a0[g], a1[g], a2[g], a3[g], b[g][0], b[g][1]);
+        }
+        if constexpr (SPLIT)
+#pragma unroll
+          for (int g = 0; g < NG; ++g) mma16816(acc[g], a0[g], a1[g], a2[g], a3[g], b[g][2], b[g][3]);
+      }
   sc[0] = sc[1] = sc[2] = sc[3] = 0.f;
 #pragma unroll
-  for (int g = 0; g < HD / GROUP; ++g) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < GROUP / 64; ++w) {
-      const int wi = g * (GROUP / 64) + w;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          uint32_t a0, a1, a2, a3;
-          if (SPLIT) {
-            unpack_centred(st ? kw[hf][0][wi] >> 7 : kw[hf][0][wi] << 1, a0, a2);
-            unpack_centred(st ? kw[hf][1][wi] >> 7 : kw[hf][1][wi] << 1, a1, a3);
-          } else {
-            unpack_plain(st ? kw[hf][0][wi] >> 8 : kw[hf][0][wi], a0, a2);
-            unpack_plain(st ? kw[hf][1][wi] >> 8 : kw[hf][1][wi], a1, a3);
-          }
-          uint32_t b[SPLIT ? 4 : 2];
-          qf((wi * 2 + hf) * 2 + st, b);
-          mma16816(acc, a0, a1, a2, a3, b[0], b[1]);
-          if constexpr (SPLIT) mma16816(acc, a0, a1, a2, a3, b[2], b[3]);
-        }
-    }
+  for (int g = 0; g < NG; ++g) {
     float2 s0 = kv4_param(kp[0][g]), s1 = kv4_param(kp[1][g]);
     if (SPLIT) {  // the middle of the group
       s0.y = fmaf(7.5f, s0.x, s0.y);
       s1.y = fmaf(7.5f, s1.x, s1.y);
     }
-    sc[0] = fmaf(s0.x, acc[0], fmaf(s0.y, qsum[0][g], sc[0]));
-    sc[1] = fmaf(s0.x, acc[1], fmaf(s0.y, qsum[1][g], sc[1]));
-    sc[2] = fmaf(s1.x, acc[2], fmaf(s1.y, qsum[0][g], sc[2]));
-    sc[3] = fmaf(s1.x, acc[3], fmaf(s1.y, qsum[1][g], sc[3]));
+    sc[0] = fmaf(s0.x, acc[g][0], fmaf(s0.y, qsum[0][g], sc[0]));
+    sc[1] = fmaf(s0.x, acc[g][1], fmaf(s0.y, qsum[1][g], sc[1]));
+    sc[2] = fmaf(s1.x, acc[g][2], fmaf(s1.y, qsum[0][g], sc[2]));
+    sc[3] = fmaf(s1.x, acc[g][3], fmaf(s1.y, qsum[1][g], sc[3]));
   }
 }
 
@@ -447,19 +455,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
           if (!live1) vp[1][i] = 0u;
         }
       }
-      // running maximum of each column, and of the value scales; a NaN score
-      // counts as infinity, so that the column ends as NaN
-      auto up_nan = [](float v) { return v != v ? INFINITY : v; };
-      float mx[2] = {fmaxf(up_nan(x[0]), up_nan(x[2])), fmaxf(up_nan(x[1]), up_nan(x[3]))};
+      // running maximum of each column, and of the value scales
+      float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], d));
         mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], d));
       }
-      unsigned sb = 0u;
+      unsigned sb = __vmaxu2(vp[0][0], vp[1][0]);  // scales are the low halves, and positive
 #pragma unroll
-      for (int i = 0; i < NG; ++i) sb = max(sb, max(vp[0][i] & 0x7fffu, vp[1][i] & 0x7fffu));
-      sb = __reduce_max_sync(0xffffffffu, min(sb, 0x7bffu));
+      for (int i = 1; i < NG; ++i) sb = __vmaxu2(sb, __vmaxu2(vp[0][i], vp[1][i]));
+      sb = __reduce_max_sync(0xffffffffu, min(sb & 0xffffu, 0x7bffu));
       // The reference point moves only when the maximum has outgrown it by
       // 2^8 or the scales theirs: p then stays below 2^8, p s below 2^15.
       if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f) || sb > smax) {
@@ -526,25 +532,27 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
 #pragma unroll
         for (int w = 0; w < GROUP / 64; ++w) {
           const int wi = gi * (GROUP / 64) + w;
+          uint32_t av[4][4];
 #pragma unroll
           for (int pt = 0; pt < 2; ++pt) {
             const uint32_t sel = pt ? 0x7632u : 0x5410u;
             const uint32_t ab = prmt(vw[0][wi], vw[1][wi], sel), cd = prmt(vw[2][wi], vw[3][wi], sel);
 #pragma unroll
             for (int st2 = 0; st2 < 2; ++st2) {
-              uint32_t a0, a1, a2, a3;
+              uint32_t(&f)[4] = av[pt * 2 + st2];
               if (SPLIT) {
-                unpack_centred(st2 ? ab >> 7 : ab << 1, a0, a1);
-                unpack_centred(st2 ? cd >> 7 : cd << 1, a2, a3);
+                unpack_centred(st2 ? ab >> 7 : ab << 1, f[0], f[1]);
+                unpack_centred(st2 ? cd >> 7 : cd << 1, f[2], f[3]);
               } else {
-                unpack_plain(st2 ? ab >> 8 : ab, a0, a1);
-                unpack_plain(st2 ? cd >> 8 : cd, a2, a3);
+                unpack_plain(st2 ? ab >> 8 : ab, f[0], f[1]);
+                unpack_plain(st2 ? cd >> 8 : cd, f[2], f[3]);
               }
-              float(&d)[4] = o[wi * 4 + pt * 2 + st2];
-              mma16816(d, a0, a1, a2, a3, bh0, bh1);
-              if (SPLIT) mma16816(d, a0, a1, a2, a3, bl0, bl1);
+              mma16816(o[wi * 4 + pt * 2 + st2], f[0], f[1], f[2], f[3], bh0, bh1);
             }
           }
+          if (SPLIT)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma16816(o[wi * 4 + k], av[k][0], av[k][1], av[k][2], av[k][3], bl0, bl1);
         }
       }
       __syncwarp();
@@ -569,7 +577,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
     if (r == 0) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        sh.m[warp][2 * c + q] = m[q];
+        // a NaN score leaves the maximum alone, but not the sum: infinity makes
+        // the column NaN when it is joined
+        sh.m[warp][2 * c + q] = l[q] != l[q] ? INFINITY : m[q];
         sh.l[warp][2 * c + q] = l[q];
       }
     }
