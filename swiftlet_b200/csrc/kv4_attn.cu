@@ -775,6 +775,7 @@ void run(const Kv4AttnArgs& a, cudaStream_t st) {
     launch(k_kv4_attn_join<HD>, dim3(AT_GRID, AT_COLS), dim3(HD), 0, st, true, a);
   } else {
     launch_kv4_prompt(a, st);
+    return;
   }
   if (a.weights && a.b.max_len > 0)
     launch(k_kv4_weights<HD, GROUP, SPLIT>, dim3((a.b.max_len + AT_TILE - 1) / AT_TILE, a.g.kvh, a.b.nseq), dim3(WT_WARPS * 32), 0, st,

@@ -903,12 +903,275 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4AttnArgs a) {
   if (lane == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * P_LN2;
 }
 
+// ------------------------------------------------------- accumulated weight --
+// weights[t] += sum over the rows that see slot t of exp(score - lse): S^T = K
+// Q^T by tcgen05.mma with 128 slots as M (a thread a slot and half of the
+// columns, so the sums stay in a register) and 64 query rows as N. The slots'
+// keys are unpacked once, into TMEM; the queries come as f16 tiles that
+// k_kv4_queries lays out once for all of them. A CTA owns its slots: every sum
+// has one order. Bound: 512 cycles of MMA (16-bit inputs, 256 channels) and 512
+// of exponentials a step of 128 x 64.
+constexpr int WQ_COLS = 64;  // query rows of a tile
+
+template <int HD, bool SPLIT>
+struct WqShape {
+  static constexpr int T = SPLIT ? 2 : 1;
+  static constexpr int TILE = WQ_COLS * HD * 2;             // one term of a tile's queries
+  static constexpr int BLOB = T * TILE + WQ_COLS * 16;      // with {factor, log2 of the sum, last slot, 0} a row
+  static constexpr int ST = 3;
+  static constexpr int BAR_OFF = (ST * BLOB + 1023) / 1024 * 1024;
+  static constexpr int TOTAL = BAR_OFF + (2 * ST + 5) * 8 + 16 + 128 * 4 + 1024;
+  static constexpr int COLS = 2 * WQ_COLS + T * HD / 2 <= 256 ? 256 : 512;  // TMEM
+  static constexpr int K_COL = 2 * WQ_COLS;
+};
+constexpr int WQ_THREADS = 320;  // 8 warps of slots, the MMA warp, the copy warp
+
+// First tile of a sequence's queries of a kv head (ceil(n rep / 64) of them fit before the next sequence's).
+__host__ __device__ inline int64_t wq_first(int64_t row0, int rep, int seq) { return row0 * rep / WQ_COLS + seq; }
+__host__ __device__ inline int64_t wq_tiles(int64_t total, int rep, int nseq) { return total * rep / WQ_COLS + nseq + 1; }
+
+// A warp a (row, query head).
+template <int HD, bool SPLIT>
+__global__ void __launch_bounds__(256) k_kv4_queries(const Kv4AttnArgs a) {
+  using Sh = WqShape<HD, SPLIT>;
+  const int lane = threadIdx.x & 31;
+  const int64_t wid = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t j = wid / a.heads;
+  const int hq = int(wid - j * a.heads), h = hq / a.rep;
+  if (j >= a.b.total) return;
+  int lo_s = 0, hi_s = a.b.nseq;  // the sequence the row belongs to
+  while (lo_s < hi_s) {
+    const int mid = (lo_s + hi_s) >> 1;
+    if (__ldg(a.b.start + mid + 1) <= j) lo_s = mid + 1; else hi_s = mid;
+  }
+  if (lo_s >= a.b.nseq) return;
+  int row0;
+  const int n = kv4_new(a.b, lo_s, row0), len = kv4_len(a.b, lo_s), t = int(j) - row0;
+  if (t < 0 || t >= n) return;
+  const int ci = t * a.rep + hq - h * a.rep, r = ci % WQ_COLS;
+  uint8_t* blob = reinterpret_cast<uint8_t*>(pt_parts(a)) +
+                  (h * wq_tiles(a.b.total, a.rep, a.b.nseq) + wq_first(row0, a.rep, lo_s) + ci / WQ_COLS) * Sh::BLOB;
+  float x[8], am = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  if (lane < HD / 8) kv4_ld8(a.q.p, a.dt, j * a.q.ts + hq * a.q.hs + lane * 8, kv4_vec(a.q, a.dt), x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[e]));
+  am = warp_max(am);
+  int ex = am > 0.f && am < INFINITY ? 12 - (int(__float_as_uint(am) >> 23) - 127) : 0;
+  ex = max(-60, min(60, ex));
+  const float up = pt_pow2(ex);
+  if (lane < HD / 8) {
+    uint4 hi, lo;
+    uint32_t *H = &hi.x, *L = &lo.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // the order the codes come unpacked in
+      const float v0 = x[i] * up, v4 = x[i + 4] * up;
+      const __half2 hh = __floats2half2_rn(v0, v4);
+      H[i] = pt_h2(hh);
+      if (SPLIT) {
+        const float2 ff = __half22float2(hh);
+        L[i] = pt_h2(__floats2half2_rn(v0 - ff.x, v4 - ff.y));
+      }
+    }
+    const int off = (lane >> 3) * (WQ_COLS * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+    *reinterpret_cast<uint4*>(blob + off) = hi;
+    if (SPLIT) *reinterpret_cast<uint4*>(blob + Sh::TILE + off) = lo;
+  }
+  if (lane == 0)
+    reinterpret_cast<float4*>(blob + Sh::T * Sh::TILE)[r] =
+        make_float4(a.scale * P_LOG2E * pt_pow2(-ex), pt_lse(a)[j * a.heads + hq] * P_LOG2E, __int_as_float(len - n + t), 0.f);
+}
+
+template <int HD, int GROUP, bool SPLIT>
+__global__ void __launch_bounds__(WQ_THREADS, SPLIT ? 1 : 2) k_kv4_prompt_weights(const Kv4AttnArgs a) {
+  using Sh = WqShape<HD, SPLIT>;
+  constexpr int T = Sh::T, ST = Sh::ST, NG = HD / GROUP, NW = HD / 64, HC = WQ_COLS / 2;
+  extern __shared__ __align__(1024) uint8_t wq_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wq_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sm + Sh::BAR_OFF);
+  uint64_t *q_empty = q_full + ST, *s_full = q_empty + ST, *s_empty = s_full + 2, *drain = s_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* half_sum = reinterpret_cast<float*>(tmem_slot + 4);
+  const Kv4Geo& g = a.g;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, seq = blockIdx.z;
+  int row0;
+  const int n = kv4_new(a.b, seq, row0), len = kv4_len(a.b, seq), tile0 = blockIdx.x * 128;
+  if (tile0 >= len || n == 0) return;
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1 + 256);  // the MMAs that read the tile, the threads that read its rows' factors
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_empty[s], 256);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(Sh::COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tg_fence_before();
+  __syncthreads();
+  tg_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto fail = [&]() {
+    if (a.b.status) atomicOr(a.b.status, 1);
+    *abort_flag = 1;
+  };
+  auto wait = [&](uint64_t* b, unsigned ph) {
+    if (__all_sync(0xffffffffu, pt_wait(b, ph) && !*abort_flag)) return true;
+    fail();
+    return false;
+  };
+  // the query tiles that hold a row that sees the first slot
+  const int q0 = max(0, tile0 - (len - n)) * a.rep / WQ_COLS, nq = (n * a.rep + WQ_COLS - 1) / WQ_COLS - q0;
+  const int row = tid & 127, hf = (tid >> 7) & 1, slot = tile0 + row;
+  const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+  bool there = false;
+  float kscale = 1.f;
+  if (warp < 8) {
+    // the slot's keys, half of the units of each 64-channel block, to TMEM
+    unsigned mk = 0u;
+    if (lane < RG_SPLIT) mk = unsigned(__ldcg(pt_ranges(a) + (int64_t(seq) * g.kvh + h) * RG_SPLIT + lane).x);
+    const int kx = pt_exp(__reduce_max_sync(0xffffffffu, mk));
+    kscale = pt_pow2(-kx);
+    const __half2 sc = __float2half2_rn(pt_pow2(kx));
+    const uint8_t* blk = slot < len ? kv4_block(g, g.table, g.tstride, seq, h, slot, a.b.status) : nullptr;
+    there = blk != nullptr;
+    uint32_t w[4][NW], pr[NG];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int k = 0; k < NW; ++k) w[u][k] = 0u;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) pr[k] = 0u;
+    if (blk) {
+      const int t = slot & (g.seg - 1);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) kv4_ldv(blk + t * (HD / 2) + ((hf * 4 + u) ^ kv4_swz(HD, t)) * (HD / 16), w[u]);
+      kv4_ldv(blk + g.seg * (HD / 2) + t * NG * 4, pr);
+    }
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      uint32_t hi[16], lo[16];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        pt_unpack<SPLIT>(w[u][k], __hmul2(pt_u2(pr[k * 64 / GROUP]), sc), *reinterpret_cast<uint4*>(hi + 4 * u), *reinterpret_cast<uint4*>(lo + 4 * u));
+      pt_st16(lanes + Sh::K_COL + k * 32 + hf * 16, hi);
+      if (SPLIT) pt_st16(lanes + Sh::K_COL + HD / 2 + k * 32 + hf * 16, lo);
+    }
+    pt_st_wait();
+    tg_fence_before();
+  }
+  __syncthreads();
+  tg_fence_after();
+  if (warp < 8) {
+    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < nq; ++i) {
+      const int b = i & 1, st = i % ST;
+      // the copy is complete when its products are; the wait makes it visible here
+      if (!wait(&s_full[b], (i >> 1) & 1) || !wait(&q_full[st], (i / ST) & 1)) break;
+      tg_fence_after();
+      uint32_t s[HC];
+      pt_ld32(lanes + b * WQ_COLS + hf * HC, s);
+      tg_ld_wait();
+      tg_fence_before();
+      mbar_arrive(&s_empty[b]);
+      const float4* meta = reinterpret_cast<const float4*>(sm + st * Sh::BLOB + T * Sh::TILE) + hf * HC;
+      const int left = n * a.rep - (q0 + i) * WQ_COLS - hf * HC;  // rows of the tile from this half's first on
+      if (left >= HC && tile0 + 127 <= __float_as_int(meta[0].z)) {
+#pragma unroll
+        for (int e = 0; e < HC; ++e) {
+          const float4 f = meta[e];
+          s4[e & 3] += pt_ex2(fmaf(__uint_as_float(s[e]), f.x * kscale, -f.y));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < HC; ++e) {
+          const float4 f = meta[e];
+          if (e < left && slot <= __float_as_int(f.z)) s4[e & 3] += pt_ex2(fmaf(__uint_as_float(s[e]), f.x * kscale, -f.y));
+        }
+      }
+      mbar_arrive(&q_empty[st]);
+    }
+    const float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    if (hf) half_sum[row] = sum;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (!hf && there) a.weights[(int64_t(seq) * g.kvh + h) * a.wstride + slot] += sum + half_sum[row];
+  } else if (warp == 8) {
+    constexpr uint32_t ids = pt_idesc(WQ_COLS, false);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    for (int i = 0; i < nq; ++i) {
+      const int b = i & 1, st = i % ST;
+      if (!wait(&q_full[st], (i / ST) & 1) || !wait(&s_empty[b], ((i >> 1) & 1) ^ 1)) break;
+      tg_fence_after();
+      const uint64_t qd = tg_desc(smem_u32(sm + st * Sh::BLOB));
+      if (pt_elect()) {
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t d = tm + b * WQ_COLS, ak = tm + Sh::K_COL + w * 32 + k * 8;
+            const uint64_t bd = qd + ((w * (WQ_COLS * 128) + k * 32) >> 4);
+            pt_mma_ts(d, ak, bd, ids, w + k > 0);
+            if (SPLIT) {
+              pt_mma_ts(d, ak + HD / 2, bd, ids, true);
+              pt_mma_ts(d, ak, bd + (Sh::TILE >> 4), ids, true);
+            }
+          }
+        tg_commit(&s_full[b]);
+        tg_commit(&q_empty[st]);
+      }
+      __syncwarp();
+    }
+  } else {
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(pt_parts(a)) +
+                         (h * wq_tiles(a.b.total, a.rep, a.b.nseq) + wq_first(row0, a.rep, seq) + q0) * Sh::BLOB;
+    int i = 0;
+    for (; i < nq; ++i) {
+      const int st = i % ST;
+      if (!wait(&q_empty[st], ((i / ST) & 1) ^ 1)) break;
+      if (lane == 0) {
+        mbar_expect_tx(&q_full[st], Sh::BLOB);
+        bulk_g2s_keep(sm + st * Sh::BLOB, src + int64_t(i) * Sh::BLOB, Sh::BLOB, &q_full[st]);
+      }
+      __syncwarp();
+    }
+    if (*abort_flag)  // copies in flight land before the CTA may end
+      for (int k = max(0, i - ST); k < i; ++k) pt_wait(&q_full[k % ST], (k / ST) & 1);
+  }
+  tg_fence_before();
+  __syncthreads();
+  tg_fence_after();
+  if (warp == 8) {
+    if (*abort_flag) {
+      if (pt_elect()) tg_commit(drain);  // the products still in flight
+      __syncwarp();
+      pt_wait(drain, 0);
+    }
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Sh::COLS));
+  }
+}
+
 template <int HD, int GROUP, bool SPLIT>
 void run(const Kv4AttnArgs& a, cudaStream_t st) {
   using Sh = PtShape<HD, GROUP, SPLIT>;
   launch(k_kv4_range, dim3(RG_SPLIT, a.b.nseq * a.g.kvh), dim3(256), 0, st, false, a);
   launch(k_kv4_prompt<HD, GROUP, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS), Sh::TOTAL, st, true, a);
   launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(256), 0, st, true, a);
+  if (a.weights && a.b.max_len > 0) {
+    const int64_t rows = int64_t(a.b.total) * a.heads;
+    launch(k_kv4_queries<HD, SPLIT>, dim3(unsigned((rows + 7) / 8)), dim3(256), 0, st, false, a);
+    launch(k_kv4_prompt_weights<HD, GROUP, SPLIT>, dim3((a.b.max_len + 127) / 128, a.g.kvh, a.b.nseq), dim3(WQ_THREADS),
+           WqShape<HD, SPLIT>::TOTAL, st, false, a);
+  }
 }
 
 template <int HD, int GROUP>
@@ -920,7 +1183,11 @@ void run_dt(const Kv4AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int64_t kv4_prompt_work(const Kv4Geo& g, const Kv4Batch& b, int heads) {
-  return pt_lse_bytes(b.total, heads) + pt_range_bytes(b.nseq, g.kvh) + PT_GRID * int64_t(sizeof(PtJoin)) + int64_t(PT_GRID) * 2 * pt_part_floats(g.hd) * 4;
+  // the parts' space holds the weight kernel's queries after them (as for f32, the larger)
+  const int rep = heads / g.kvh;
+  const int64_t parts = int64_t(PT_GRID) * 2 * pt_part_floats(g.hd) * 4;
+  const int64_t queries = g.kvh * wq_tiles(b.total, rep, b.nseq) * (2 * WQ_COLS * g.hd * 2 + WQ_COLS * 16);
+  return pt_lse_bytes(b.total, heads) + pt_range_bytes(b.nseq, g.kvh) + PT_GRID * int64_t(sizeof(PtJoin)) + std::max(parts, queries);
 }
 
 void launch_kv4_prompt(const Kv4AttnArgs& a, cudaStream_t st) {
