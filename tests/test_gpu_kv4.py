@@ -447,6 +447,115 @@ def test_captured_and_replayed_with_other_lengths():
               weights=w.cpu().numpy().astype(np.float64), before=np.zeros((3, 2, 700)))
 
 
+def test_many_short_sequences():
+    """More sequences than a warp has lanes, most of them without new tokens, rows of the buffers left over."""
+    rng = np.random.default_rng(12)
+    lens = [int(x) for x in rng.integers(0, 40, 150)]
+    for new in ([1] * 150, [int(x) for x in rng.integers(0, 4, 150)], [0] * 149 + [30]):
+        lens2 = [max(m, n) if n > 4 else m for m, n in zip(lens, new)]
+        c = Cache(150, 40, 1, 64, page=16)
+        c.fill(lens2, rng)
+        got, lse, q = attend(c, lens2, new, 8, rng)
+        check(c, lens2, new, 8, got, lse, q)
+
+
+def test_total_above_the_rows():
+    """`total` is a bound: rows between start[nseq] and it belong to nobody and stay as they are."""
+    torch, _ = _torch()
+    c = Cache(2, 60, 2, 64)
+    c.fill([60, 20], np.random.default_rng(0))
+    for new in ([1, 1], [9, 20]):
+        rows = sum(new)
+        b = c.batch([60, 20], new)
+        b.total = rows + 40
+        q = torch.randn(rows + 40, 16, 64, device="cuda")
+        out, lse = torch.full_like(q, 7.0), torch.full((rows + 40, 16), 7.0, device="cuda")
+        w = torch.zeros(2, 2, 60, device="cuda")
+        n = swl.kv4_attention_workspace(c.desc(), b, 16)
+        work = torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+        swl.kv4_attention_device(c.desc(), b, 16, q.data_ptr(), out.data_ptr(), scale=0.125, d_lse=lse.data_ptr(), d_weights=w.data_ptr(),
+                                 weights_stride=60, d_work=work.data_ptr(), work_bytes=n)
+        x, y = torch.full((rows + 40, 2, 64), 7.0, device="cuda"), torch.full((rows + 40, 2, 64), 7.0, device="cuda")
+        swl.kv4_read_device(c.desc(), b, x.data_ptr(), y.data_ptr())
+        before = c.pool.clone()
+        swl.kv4_append_device(c.desc(), b, x.data_ptr(), y.data_ptr())  # what was read, and rows of sevens that have no slot
+        swl.kv4_read_device(c.desc(), b, x.data_ptr(), y.data_ptr())
+        torch.cuda.synchronize()
+        assert (out[rows:] == 7).all() and (lse[rows:] == 7).all() and (x[rows:] == 7).all() and (y[rows:] == 7).all()
+        changed = (before != c.pool).view(-1, swl.kv4_page_bytes(2, 64, 64, 64)).any(1).nonzero().flatten().tolist()
+        assert set(changed) <= set(c.table.flatten().tolist())
+        c.pool.copy_(before)
+        check(c, [60, 20], new, 8, out[:rows].cpu().numpy().astype(np.float64), lse[:rows].cpu().numpy().astype(np.float64),
+              q[:rows].cpu().numpy().astype(np.float64)[:, :, None], weights=w.cpu().numpy().astype(np.float64), before=np.zeros((2, 2, 60)))
+
+
+def test_offsets_beyond_32_bits():
+    """Pages above 4 GiB of the pool, for every call."""
+    torch, _ = _torch()
+    rng = np.random.default_rng(5)
+    c = Cache(2, 200, 2, 256)
+    pb = swl.kv4_page_bytes(2, 256, 64, 64)
+    n = (5 << 30) // pb
+    c.pool = torch.empty(n * pb, dtype=torch.uint8, device="cuda")
+    c.num = n
+    c.table = torch.from_numpy((n - 1 - np.arange(8, dtype=np.int32)).reshape(2, 4)).cuda()
+    c.spare = n - 9 - np.arange(8, dtype=np.int32)
+    c.fill([200, 130], rng)
+    for new in ([1, 1], [40, 3]):
+        got, lse, q = attend(c, [200, 130], new, 8, rng)
+        check(c, [200, 130], new, 8, got, lse, q)
+    w = torch.from_numpy(rng.random((2, 2, 200)).astype(np.float32)).cuda()
+    check_evict(c, [200, 130], w, 128, 4, 20)
+
+
+def test_negative_and_zero_scale():
+    rng = np.random.default_rng(13)
+    for scale in (-0.07, 0.0):
+        for new in (1, 20):
+            c = Cache(1, 150, 2, 128)
+            c.fill([150], rng)
+            got, lse, q = attend(c, [150], [new], 4, rng, scale=scale)
+            check(c, [150], [new], 4, got, lse, q, scale=scale)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams with workspaces of their own, a captured prompt among them, replayed with other lengths."""
+    torch, _ = _torch()
+    rng = np.random.default_rng(14)
+    c = Cache(3, 900, 2, 256)
+    lens = [900, 300, 64]
+    c.fill(lens, rng)
+    runs = []
+    for k, new in enumerate(([1, 1, 1], [70, 5, 20])):
+        rows = sum(new)
+        q = torch.randn(rows, 16, 256, device="cuda")
+        out, lse, w = torch.empty_like(q), torch.empty(rows, 16, device="cuda"), torch.zeros(3, 2, 900, device="cuda")
+        b = c.batch(lens, new)
+        n = swl.kv4_attention_workspace(c.desc(), b, 16)
+        work = torch.empty(n, dtype=torch.uint8, device="cuda")
+        s = torch.cuda.Stream()
+
+        def call(stream, q=q, out=out, lse=lse, w=w, b=b, work=work, n=n):
+            swl.kv4_attention_device(c.desc(), b, 16, q.data_ptr(), out.data_ptr(), scale=1 / 16, d_lse=lse.data_ptr(),
+                                     d_weights=w.data_ptr(), weights_stride=900, d_work=work.data_ptr(), work_bytes=n, stream=stream)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            call(torch.cuda.current_stream().cuda_stream)
+        runs.append((new, q, out, lse, w, b, g, s))
+    for m in (lens, [500, 5, 63]):
+        for new, q, out, lse, w, b, g, s in runs:
+            b.keep[1].copy_(torch.tensor(m, dtype=torch.int32))
+            w.zero_()
+        torch.cuda.synchronize()
+        for *_, g, s in runs:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for new, q, out, lse, w, b, g, s in runs:
+            check(c, m, new, 8, out.cpu().numpy().astype(np.float64), lse.cpu().numpy().astype(np.float64),
+                  q.cpu().numpy().astype(np.float64)[:, :, None], weights=w.cpu().numpy().astype(np.float64), before=np.zeros((3, 2, 900)))
+
+
 # -------------------------------------------------------------------- evict --
 def survivors(w, n, keep, first, recent):
     if n <= keep:
