@@ -547,12 +547,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
                 unpack_plain(st2 ? ab >> 8 : ab, f[0], f[1]);
                 unpack_plain(st2 ? cd >> 8 : cd, f[2], f[3]);
               }
-              mma16816(o[wi * 4 + pt * 2 + st2], f[0], f[1], f[2], f[3], bh0, bh1);
+              if (!SPLIT) mma16816(o[wi * 4 + pt * 2 + st2], f[0], f[1], f[2], f[3], bh0, bh1);
             }
           }
-          if (SPLIT)
+          if (SPLIT) {
+            // the accumulators truncate: a unit's sums (the small products
+            // first) are made apart and added with correct rounding
+            float d[4][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma16816(o[wi * 4 + k], av[k][0], av[k][1], av[k][2], av[k][3], bl0, bl1);
+            for (int k = 0; k < 4; ++k) {
+              d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.f;
+              mma16816(d[k], av[k][0], av[k][1], av[k][2], av[k][3], bl0, bl1);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma16816(d[k], av[k][0], av[k][1], av[k][2], av[k][3], bh0, bh1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[wi * 4 + k][e] += d[k][e];
+          }
         }
       }
       __syncwarp();

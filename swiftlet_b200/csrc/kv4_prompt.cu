@@ -8,10 +8,16 @@
 //   O += P V (M 128, N head_dim, K BN; A from TMEM, V as an N-major operand).
 // Keys and values are unpacked to f16 on their way into shared memory, scaled
 // by a power of two so that the largest value of the sequence and head is
-// just below 2^14 (k_kv4_range reads the params for it). 16-bit inputs: one
-// product each, values rounded to 11 bits like the inputs themselves. f32
-// inputs: every operand as two f16 terms (22 bits) and three products each
-// (hi hi + lo hi + hi lo), f32 accumulators throughout.
+// just below 2^14 (k_kv4_range reads the params for it). Keys are two f16
+// terms: lse and the weights are f32 whatever the inputs' type, and with keys
+// of 11 bits scores were off by 1e-4. 16-bit inputs: queries and values are one
+// term (values rounded to 11 bits like the inputs themselves), so two products
+// make S and one O. f32 inputs: all operands are two terms (22 bits) and
+// three products each make S and O (hi lo, lo hi, hi hi).
+// The tensor cores' f32 accumulators truncate: every product added takes up to
+// 2^-24 off the size of what it is added to. S is built from its small terms up;
+// for f32 inputs O is taken out of TMEM every PT_FLUSH tiles and added up with
+// correct rounding (without that, outputs were off by 1.5e-5 after some 30 tiles).
 //
 // Warps: 0-7 softmax and output (two threads a row, half of the tile's slots
 // each), 8-15 unpacking of keys, 16-23 of values, 24 MMA issue and TMEM, 25 and 26 bulk copies
@@ -46,22 +52,24 @@ constexpr int PT_MMA = (PT_SOFT + PT_UNPACK) / 32, PT_COPY = PT_MMA + 1;  // war
 // Registers a thread: 72 at launch, then 256 x 96 + 512 x 64 + 128 x 56 (= 896 x 72).
 constexpr int PT_REGS_SOFT = 96, PT_REGS_UNPACK = 64, PT_REGS_ISSUE = 56;
 constexpr int PT_HEAD = 12;                             // cost of an item beside its tiles, in tiles
+constexpr int PT_FLUSH = 4;                             // tiles that O of f32 inputs stays in TMEM
 constexpr int RG_SPLIT = 16;                            // blocks a (sequence, head) of the range kernel
 constexpr float P_LOG2E = 1.4426950408889634f, P_LN2 = 0.6931471805599453f;
 
 template <int HD, int GROUP, bool SPLIT>
 struct PtShape {
-  static constexpr int T = SPLIT ? 2 : 1;                  // f16 terms of an operand
+  static constexpr int T = SPLIT ? 2 : 1;                  // f16 terms of queries, weights and values
+  static constexpr int KT = 2;                             // and of keys
   static constexpr int KST = HD == 256 && SPLIT ? 1 : 2;   // buffers of unpacked keys, and of values
   // Copied stages: the keys' and the values', rings of their own, for a wait by
   // parity tells two neighbouring phases apart and no more.
-  static constexpr int RK = 2, RV = HD == 256 && SPLIT ? 1 : 2, RST = RK + RV;
+  static constexpr int RK = 2, RV = HD == 256 ? 1 : 2, RST = RK + RV;
   static constexpr int QB = PT_ROWS * HD * 2;              // bytes of one term of Q
   static constexpr int KB = PT_BN * HD * 2;                // of one term of a tile's keys (values)
   static constexpr int RAW = PT_BN * (HD / 2 + 4 * (HD / GROUP));  // bytes of a tile's keys (values) as they are held
   // low terms of Q, keys (first the high terms of Q, on their way to TMEM), values, copied stages
   static constexpr int SCR = 8 * 32 * 33 * 4;              // the output's scratch, over the key buffers
-  static constexpr int KS = KST * T * KB > SCR ? KST * T * KB : (SCR + 1023) / 1024 * 1024;
+  static constexpr int KS = KST * KT * KB > SCR ? KST * KT * KB : (SCR + 1023) / 1024 * 1024;
   static constexpr int Q_OFF = 0, K_OFF = SPLIT ? QB : 0, V_OFF = K_OFF + KS, R_OFF = V_OFF + KST * T * KB;
   static constexpr int M_OFF = R_OFF + RST * RAW;          // the rows' factors and limits, exchange of the halves
   static constexpr int BAR_OFF = M_OFF + PT_ROWS * 16;
@@ -143,6 +151,29 @@ __device__ __forceinline__ bool pt_elect() {
   uint32_t ok;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
   return ok != 0;
+}
+// Channel of a column within eight: the order in which codes come unpacked.
+__device__ __forceinline__ constexpr int pt_channel(int col) { return (col >> 1) + 4 * (col & 1); }
+// Adds O's columns of a row (HD / 2 of them at TMEM address t) to p, [by
+// four][rows], which holds f times as much (nothing yet: on false).
+template <int HD>
+__device__ __forceinline__ void pt_add_out(uint32_t t, float4* p, bool on, float f) {
+#pragma unroll 1
+  for (int q = 0; q < HD / 64; ++q) {
+    uint32_t o[32];
+    pt_ld32(t + q * 32, o);
+    tg_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float4* at = p + (q * 8 + e) * PT_ROWS;
+      float4 v = on ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+      v.x = fmaf(v.x, f, __uint_as_float(o[4 * e]));
+      v.y = fmaf(v.y, f, __uint_as_float(o[4 * e + 1]));
+      v.z = fmaf(v.z, f, __uint_as_float(o[4 * e + 2]));
+      v.w = fmaf(v.w, f, __uint_as_float(o[4 * e + 3]));
+      *at = v;
+    }
+  }
 }
 // Barrier `id` of N threads; true when `v` is true for any of them.
 template <int N = 64>
@@ -305,22 +336,24 @@ __global__ void __launch_bounds__(256) k_kv4_range(const Kv4AttnArgs a) {
 __device__ __forceinline__ int pt_exp(unsigned bits) { return bits ? max(-14, min(14, 13 - (int(bits >> 23) - 127))) : 0; }
 __device__ __forceinline__ float pt_pow2(int e) { return __int_as_float((127 + e) << 23); }
 
-// Eight codes of a word as f16 pairs (0 4)(1 5)(2 6)(3 7): the scaled value s c
-// + b, rounded once, or as two terms. The codes themselves come out of the
-// bits exactly: 1024 + c (or 1024 + 16 c) less the constant.
-template <bool SPLIT>
-__device__ __forceinline__ void pt_unpack(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
-  uint32_t* H = &hi.x;
-  uint32_t* L = &lo.x;
-  const __half2 m0 = pt_u2(0xe400e400u);                          // -1024
-  const __half2 r = pt_u2(0x2c002c00u), m1 = pt_u2(0xd400d400u);  // 1 / 16, -64
-  __half2 c[4];
+// Eight codes of a word as f16 pairs (0 4)(1 5)(2 6)(3 7), the codes exact.
+__device__ __forceinline__ void pt_codes(uint32_t w, __half2 (&c)[4]) {
+  const __half2 m0 = pt_u2(0xe400e400u);                          // 1024 + c less 1024
+  const __half2 r = pt_u2(0x2c002c00u), m1 = pt_u2(0xd400d400u);  // (1024 + 16 c) / 16 less 64
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t x = i ? w >> 8 : w;
     c[2 * i] = __hadd2(pt_u2((x & 0x000f000fu) | 0x64006400u), m0);
     c[2 * i + 1] = __hfma2(pt_u2((x & 0x00f000f0u) | 0x64006400u), r, m1);
   }
+}
+// Their scaled values s c + b: rounded once, or two terms of them (22 bits).
+template <bool SPLIT>
+__device__ __forceinline__ void pt_unpack(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
+  uint32_t* H = &hi.x;
+  uint32_t* L = &lo.x;
+  __half2 c[4];
+  pt_codes(w, c);
   if (!SPLIT) {
     const __half2 s = __low2half2(sb), b = __high2half2(sb);
 #pragma unroll
@@ -339,11 +372,35 @@ __device__ __forceinline__ void pt_unpack(uint32_t w, __half2 sb, uint4& hi, uin
     }
   }
 }
+// Keys for 16-bit inputs, in f16 arithmetic alone: with e = c - 7.5, s e =
+// fl(s e) + (its residual, which an FMA gives exactly), and the group's middle
+// b + 7.5 s joins the residual (rounded by 2^-12 of the middle, which is a
+// fraction of a step where a group is spread about zero).
+__device__ __forceinline__ void pt_unpack_keys(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
+  uint32_t* H = &hi.x;
+  uint32_t* L = &lo.x;
+  const __half2 s = __low2half2(sb), mid = __hfma2(s, pt_u2(0x47804780u), __high2half2(sb));  // 7.5
+  const __half2 m0 = pt_u2(0xe00fe00fu);                          // 512 + c less 519.5
+  const __half2 r = pt_u2(0x2c002c00u), m1 = pt_u2(0xd0f0d0f0u);  // (512 + 16 c) / 16 less 39.5
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = i < 2 ? w << 1 : w >> 7;
+    const __half2 e = i & 1 ? __hfma2(pt_u2((x & 0x01e001e0u) | 0x60006000u), r, m1) : __hadd2(pt_u2((x & 0x001e001eu) | 0x60006000u), m0);
+    const __half2 h = __hmul2(e, s);
+    H[i] = pt_h2(h);
+    L[i] = pt_h2(__hadd2(__hfma2(e, s, __hneg2(h)), mid));
+  }
+}
+template <bool SPLIT>
+__device__ __forceinline__ void pt_unpack_k(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
+  if (SPLIT) pt_unpack<true>(w, sb, hi, lo);
+  else pt_unpack_keys(w, sb, hi, lo);
+}
 
 template <int HD, int GROUP, bool SPLIT>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs a) {
   using Sh = PtShape<HD, GROUP, SPLIT>;
-  constexpr int BN = PT_BN, T = Sh::T, KST = Sh::KST, RST = Sh::RST, NG = HD / GROUP, NW = HD / 64;
+  constexpr int BN = PT_BN, T = Sh::T, KT = Sh::KT, KST = Sh::KST, RST = Sh::RST, NG = HD / GROUP, NW = HD / 64;
   extern __shared__ __align__(1024) uint8_t pt_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
   float* row_mul = reinterpret_cast<float*>(sm + Sh::M_OFF);
@@ -467,10 +524,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       const int lim_lo = __reduce_min_sync(0xffffffffu, lim);
       bar();
       float m = -INFINITY, l = 0.f;
+      // f32 inputs: what O was when it was last taken out of TMEM, relative to
+      // the maximum mo; where the parts go, [channels by four][rows]
+      float4* const part4 = reinterpret_cast<float4*>(pt_parts(a) + (int64_t(blockIdx.x) * 2 + slot_of_part) * pt_part_floats(HD) + 2 * PT_ROWS) +
+                            hf * (HD / 8) * PT_ROWS + row;
+      float mo = 0.f;
+      bool pending = false;  // a wait that gave up
       for (int i = 0; i < nt; ++i) {
         const int jj = j + i, b = jj & 1;
         // the halves of a row leave together, or one would wait for the other
-        const bool dead = !wait(&s_full[b], (jj >> 1) & 1);
+        const bool dead = !wait(&s_full[b], (jj >> 1) & 1) || pending;
         tg_fence_after();
         uint32_t s[HB];
         pt_ld32(lanes + Sh::S_COL + b * BN + hf * HB, s);
@@ -495,7 +558,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
         // both halves have read S when the pair has met: P may take its place
         tg_fence_before();
-        if (pt_bar_any(pair, mx > m + 8.f || dead)) {
+        const bool any = pt_bar_any(pair, mx > m + 8.f || dead), flush = SPLIT && i > 0 && i % PT_FLUSH == 0;
+        if (flush) {
+          pending = !wait(&o_done[b ^ 1], ((jj - 1) >> 1) & 1);
+          tg_fence_after();
+          pt_add_out<HD>(lanes + Sh::O_COL + hf * (HD / 2), part4, i > PT_FLUSH, mo == -INFINITY ? 0.f : pt_ex2(mo - m));
+          mo = m;
+        }
+        if (any) {
           xch[hf * PT_ROWS + row] = mx;
           if (pt_bar_any(pair, dead)) break;
           mx = fmaxf(mx, xch[(hf ^ 1) * PT_ROWS + row]);
@@ -505,7 +575,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           m = mn;
           l *= al;
           bool late = false;
-          if (i > 0) {
+          if (i > 0 && !flush) {
             // every earlier product has landed before O is scaled
             late = !wait(&o_done[b ^ 1], ((jj - 1) >> 1) & 1);
             tg_fence_after();
@@ -569,6 +639,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       l += xch[(hf ^ 1) * PT_ROWS + row];
       const bool none = l == 0.f;
       const float fac = none ? 0.f : whole ? pt_pow2(-vx) / l : pt_pow2(-vx);
+      const bool more = SPLIT && nt > PT_FLUSH;  // O was taken out before
+      const float fo = !more || mo == -INFINITY ? 0.f : pt_ex2(mo - m);
       const unsigned ci0 = unsigned(p.qt * PT_ROWS + (warp & 3) * 32);
       if (hf == 0) {
         const unsigned ci = ci0 + lane;
@@ -592,12 +664,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         pt_ld32(lanes + Sh::O_COL + c0, o);
         tg_ld_wait();
         const bool nan = (bad >> (c0 / GROUP)) & 1;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float4 p4 = make_float4(0.f, 0.f, 0.f, 0.f);
+          float4* at = part4 + (q * 8 + e / 4) * PT_ROWS;
+          if (more) p4 = *at;
+          float v[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[k] = nan ? NAN : none ? 0.f : (more ? fmaf(v[k], fo, __uint_as_float(o[e + k])) : __uint_as_float(o[e + k])) * fac;
+            o[e + k] = __float_as_uint(v[k]);
+          }
+          if (!whole) *at = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        if (!whole) continue;
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {  // column order within eight: 0 4 1 5 2 6 3 7
-          const int ch = (e & ~7) + ((e & 7) >> 1) + 4 * (e & 1);
-          scr[lane * 33 + ch] = nan ? NAN : none ? 0.f : __uint_as_float(o[e]) * fac;
-        }
+        for (int e = 0; e < 32; ++e) scr[lane * 33 + (e & ~7) + pt_channel(e & 7)] = __uint_as_float(o[e]);
         __syncwarp();
         const int ch = (lane & 3) * 8;
 #pragma unroll
@@ -606,13 +689,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = scr[rr * 33 + ch + e];
-          if (!whole) {
-            float* part = pt_parts(a) + (int64_t(blockIdx.x) * 2 + slot_of_part) * pt_part_floats(HD);
-            float4* d = reinterpret_cast<float4*>(part + 2 * PT_ROWS + ((warp & 3) * 32 + rr) * HD + c0 + ch);
-            d[0] = make_float4(v[0], v[1], v[2], v[3]);
-            d[1] = make_float4(v[4], v[5], v[6], v[7]);
-            continue;
-          }
           const unsigned ci = ci0 + rr;
           const int tok = int(ci / unsigned(a.rep)), hq = p.h * a.rep + int(ci % unsigned(a.rep));
           if (tok >= p.n) continue;
@@ -720,7 +796,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         const int jj = j + i, st = jj % KST, rs = kv ? Sh::RK + jj % Sh::RV : jj % Sh::RK;
         if (!wait(empty + st, ((jj / KST) & 1) ^ 1) || !wait(&r_full[rs], (jj / (kv ? Sh::RV : Sh::RK)) & 1)) break;
         const uint8_t* raw = sm + Sh::R_OFF + rs * Sh::RAW;
-        uint8_t* d = dst + st * (T * Sh::KB);
+        uint8_t* d = dst + st * ((kv ? T : KT) * Sh::KB);
         uint32_t w[2][NW], pr[2][NG];
         const int have = r_have[rs], s0 = (tb + i) * BN + t;
 #pragma unroll
@@ -737,15 +813,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
               if (!(fabsf(kv4_param(pr[q][k]).x) < INFINITY) || !(fabsf(kv4_param(pr[q][k]).y) < INFINITY)) pr[q][k] = 0u;
         }
         mbar_arrive(&r_empty[rs]);
+        if (kv) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
-          for (int k = 0; k < NW; ++k) {
-            uint4 hi, lo;
-            pt_unpack<SPLIT>(w[q][k], __hmul2(pt_u2(pr[q][k * 64 / GROUP]), sc), hi, lo);
-            *reinterpret_cast<uint4*>(d + q * (32 * 128) + k * (BN * 128)) = hi;
-            if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + q * (32 * 128) + k * (BN * 128)) = lo;
-          }
+            for (int k = 0; k < NW; ++k) {
+              uint4 hi, lo;
+              pt_unpack<SPLIT>(w[q][k], __hmul2(pt_u2(pr[q][k * 64 / GROUP]), sc), hi, lo);
+              *reinterpret_cast<uint4*>(d + q * (32 * 128) + k * (BN * 128)) = hi;
+              if (SPLIT) *reinterpret_cast<uint4*>(d + Sh::KB + q * (32 * 128) + k * (BN * 128)) = lo;
+            }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+              uint4 hi, lo;
+              pt_unpack_k<SPLIT>(w[q][k], __hmul2(pt_u2(pr[q][k * 64 / GROUP]), sc), hi, lo);
+              *reinterpret_cast<uint4*>(d + q * (32 * 128) + k * (BN * 128)) = hi;
+              *reinterpret_cast<uint4*>(d + Sh::KB + q * (32 * 128) + k * (BN * 128)) = lo;
+            }
+        }
         fence_proxy_async();
         mbar_arrive(full + st);
       }
@@ -766,24 +854,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           const int jj = __shfl_sync(0xffffffffu, j + i, 0), st = jj % KST, b = jj & 1;
           if (!wait(&k_full[st], (jj / KST) & 1)) return false;
           tg_fence_after();
-          const uint64_t kd = tg_desc(smem_u32(sm + Sh::K_OFF + st * (T * Sh::KB)));
+          const uint64_t kd = tg_desc(smem_u32(sm + Sh::K_OFF + st * (KT * Sh::KB)));
           const uint32_t d = tm + Sh::S_COL + b * BN;
           if (pt_elect()) {
+            // the small products first; 16 channels are 32 bytes of the 128-byte rows
 #pragma unroll
             for (int w = 0; w < NW; ++w)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)  // 16 channels: 32 bytes of the 128-byte rows
-                pt_mma_ts(d, tm + Sh::Q_COL + w * 32 + k * 8, kd + ((w * (BN * 128) + k * 32) >> 4), ids, w + k > 0);
+              for (int k = 0; k < 4; ++k)
+                pt_mma_ts(d, tm + Sh::Q_COL + w * 32 + k * 8, kd + ((Sh::KB + w * (BN * 128) + k * 32) >> 4), ids, w + k > 0);
             if (SPLIT) {
               const uint64_t qd = tg_desc(smem_u32(sm + Sh::Q_OFF));
 #pragma unroll
               for (int w = 0; w < NW; ++w)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  pt_mma_ts(d, tm + Sh::Q_COL + w * 32 + k * 8, kd + ((Sh::KB + w * (BN * 128) + k * 32) >> 4), ids, true);
+                for (int k = 0; k < 4; ++k)
                   pt_mma_ss(d, qd + ((w * (PT_ROWS * 128) + k * 32) >> 4), kd + ((w * (BN * 128) + k * 32) >> 4), ids, true);
-                }
             }
+#pragma unroll
+            for (int w = 0; w < NW; ++w)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) pt_mma_ts(d, tm + Sh::Q_COL + w * 32 + k * 8, kd + ((w * (BN * 128) + k * 32) >> 4), ids, true);
             tg_commit(&s_full[b]);
             tg_commit(&k_empty[st]);
           }
@@ -800,13 +891,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           const uint64_t vd = pt_desc_n(smem_u32(sm + Sh::V_OFF + st * (T * Sh::KB)), BN * 128);
           const uint32_t pc = tm + Sh::S_COL + b * BN;
           if (pt_elect()) {
+            const bool on = SPLIT ? i % PT_FLUSH != 0 : i > 0;  // O goes on
 #pragma unroll
             for (int k = 0; k < BN / 16; ++k) {
-              pt_mma_ts(tm + Sh::O_COL, pc + k * 8, vd + ((k * 2048) >> 4), idp, k > 0 || i > 0);
               if (SPLIT) {
-                pt_mma_ts(tm + Sh::O_COL, pc + 32 + k * 8, vd + ((k * 2048) >> 4), idp, true);
+                pt_mma_ts(tm + Sh::O_COL, pc + 32 + k * 8, vd + ((k * 2048) >> 4), idp, k > 0 || on);
                 pt_mma_ts(tm + Sh::O_COL, pc + k * 8, vd + ((Sh::KB + k * 2048) >> 4), idp, true);
               }
+              pt_mma_ts(tm + Sh::O_COL, pc + k * 8, vd + ((k * 2048) >> 4), idp, SPLIT || k > 0 || on);
             }
             tg_commit(&o_done[b]);
             tg_commit(&v_empty[st]);
@@ -890,12 +982,12 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4AttnArgs a) {
     const float mi = __ldcg(q + r), f = mi == -INFINITY ? 0.f : pt_ex2(mi - M);
     L = fmaf(__ldcg(q + PT_ROWS + r), f, L);
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = fmaf(__ldcg(q + 2 * PT_ROWS + int64_t(r) * HD + e * 32 + lane), f, v[e]);
+    for (int e = 0; e < E; ++e) v[e] = fmaf(__ldcg(q + 2 * PT_ROWS + ((e * 32 + lane) / 4 * PT_ROWS + r) * 4 + lane % 4), f, v[e]);
   }
   const int64_t row = d.row0 + tok;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int ch = e * 32 + lane;
+    const int ch = e * 32 + (lane & ~7) + pt_channel(lane & 7);
     float o = L == 0.f ? v[e] : v[e] / L;  // an empty row: zeros
     if (a.gate.p) o *= kv4_sigmoid(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch));
     kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, o);
@@ -921,7 +1013,7 @@ struct WqShape {
   static constexpr int ST = 3;
   static constexpr int BAR_OFF = (ST * BLOB + 1023) / 1024 * 1024;
   static constexpr int TOTAL = BAR_OFF + (2 * ST + 5) * 8 + 16 + 128 * 4 + 1024;
-  static constexpr int COLS = 2 * WQ_COLS + T * HD / 2 <= 256 ? 256 : 512;  // TMEM
+  static constexpr int COLS = 2 * WQ_COLS + HD <= 256 ? 256 : 512;  // TMEM: S twice, two terms of the keys
   static constexpr int K_COL = 2 * WQ_COLS;
 };
 constexpr int WQ_THREADS = 320;  // 8 warps of slots, the MMA warp, the copy warp
@@ -1062,9 +1154,9 @@ __global__ void __launch_bounds__(WQ_THREADS, SPLIT ? 1 : 2) k_kv4_prompt_weight
       uint32_t hi[16], lo[16];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        pt_unpack<SPLIT>(w[u][k], __hmul2(pt_u2(pr[k * 64 / GROUP]), sc), *reinterpret_cast<uint4*>(hi + 4 * u), *reinterpret_cast<uint4*>(lo + 4 * u));
+        pt_unpack_k<SPLIT>(w[u][k], __hmul2(pt_u2(pr[k * 64 / GROUP]), sc), *reinterpret_cast<uint4*>(hi + 4 * u), *reinterpret_cast<uint4*>(lo + 4 * u));
       pt_st16(lanes + Sh::K_COL + k * 32 + hf * 16, hi);
-      if (SPLIT) pt_st16(lanes + Sh::K_COL + HD / 2 + k * 32 + hf * 16, lo);
+      pt_st16(lanes + Sh::K_COL + HD / 2 + k * 32 + hf * 16, lo);
     }
     pt_st_wait();
     tg_fence_before();
@@ -1113,18 +1205,22 @@ __global__ void __launch_bounds__(WQ_THREADS, SPLIT ? 1 : 2) k_kv4_prompt_weight
       tg_fence_after();
       const uint64_t qd = tg_desc(smem_u32(sm + st * Sh::BLOB));
       if (pt_elect()) {
+        // the small products first
+        const uint32_t d = tm + b * WQ_COLS;
 #pragma unroll
         for (int w = 0; w < NW; ++w)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t d = tm + b * WQ_COLS, ak = tm + Sh::K_COL + w * 32 + k * 8;
+            const uint32_t ak = tm + Sh::K_COL + w * 32 + k * 8;
             const uint64_t bd = qd + ((w * (WQ_COLS * 128) + k * 32) >> 4);
-            pt_mma_ts(d, ak, bd, ids, w + k > 0);
-            if (SPLIT) {
-              pt_mma_ts(d, ak + HD / 2, bd, ids, true);
-              pt_mma_ts(d, ak, bd + (Sh::TILE >> 4), ids, true);
-            }
+            pt_mma_ts(d, ak + HD / 2, bd, ids, w + k > 0);
+            if (SPLIT) pt_mma_ts(d, ak, bd + (Sh::TILE >> 4), ids, true);
           }
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            pt_mma_ts(d, tm + Sh::K_COL + w * 32 + k * 8, qd + ((w * (WQ_COLS * 128) + k * 32) >> 4), ids, true);
         tg_commit(&s_full[b]);
         tg_commit(&q_empty[st]);
       }
