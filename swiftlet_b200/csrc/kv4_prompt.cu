@@ -12,7 +12,8 @@
 // terms: lse and the weights are f32 whatever the inputs' type, and with keys
 // of 11 bits scores were off by 1e-4. 16-bit inputs: queries and values are one
 // term (values rounded to 11 bits like the inputs themselves), so two products
-// make S and one O. f32 inputs: all operands are two terms (22 bits) and
+// make S and one O; for f16 the weights are two terms and O takes two (with
+// one, outputs were off by 1.6 times their own rounding, with two 1.2 times). f32 inputs: all operands are two terms (22 bits) and
 // three products each make S and O (hi lo, lo hi, hi hi).
 // The tensor cores' f32 accumulators truncate: every product added takes up to
 // 2^-24 off the size of what it is added to. S is built from its small terms up;
@@ -500,6 +501,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
     const int hf = warp >> 2, row = tid & (PT_ROWS - 1), pair = 2 + (warp & 3);
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
     constexpr int HB = BN / 2;
+    const bool two_p = a.dt == DT_F16;
     for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part) {
       int kx, vx;
       const unsigned flags = ranges(p, kx, vx);
@@ -595,21 +597,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         tg_fence_after();
         const float mm = m == -INFINITY ? 0.f : m;
         float l4[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t hi[HB / 2], lo[SPLIT ? HB / 2 : 1];
+        uint32_t hi[HB / 2], lo[HB / 2];
+        const auto weigh = [&](bool two) {
 #pragma unroll
-        for (int e = 0; e < HB / 2; ++e) {
-          const float p0 = pt_ex2(fmaf(__uint_as_float(s[2 * e]), mul, -mm)), p1 = pt_ex2(fmaf(__uint_as_float(s[2 * e + 1]), mul, -mm));
-          l4[2 * (e & 1)] += p0;
-          l4[2 * (e & 1) + 1] += p1;
-          const __half2 hh = __floats2half2_rn(p0, p1);
-          hi[e] = pt_h2(hh);
-          if (SPLIT) {
-            const float2 ff = __half22float2(hh);
-            lo[e] = pt_h2(__floats2half2_rn(p0 - ff.x, p1 - ff.y));
+          for (int e = 0; e < HB / 2; ++e) {
+            const float p0 = pt_ex2(fmaf(__uint_as_float(s[2 * e]), mul, -mm)), p1 = pt_ex2(fmaf(__uint_as_float(s[2 * e + 1]), mul, -mm));
+            l4[2 * (e & 1)] += p0;
+            l4[2 * (e & 1) + 1] += p1;
+            const __half2 hh = __floats2half2_rn(p0, p1);
+            hi[e] = pt_h2(hh);
+            if (two) {
+              const float2 ff = __half22float2(hh);
+              lo[e] = pt_h2(__floats2half2_rn(p0 - ff.x, p1 - ff.y));
+            }
           }
-        }
-        pt_st16(lanes + Sh::S_COL + b * BN + hf * 16, hi);
-        if (SPLIT) pt_st16(lanes + Sh::S_COL + b * BN + 32 + hf * 16, lo);
+          pt_st16(lanes + Sh::S_COL + b * BN + hf * 16, hi);
+          if (two) pt_st16(lanes + Sh::S_COL + b * BN + 32 + hf * 16, lo);
+        };
+        if (SPLIT || two_p) weigh(true);
+        else weigh(false);
         l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
         pt_st_wait();
         tg_fence_before();
@@ -900,6 +906,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
               }
               pt_mma_ts(tm + Sh::O_COL, pc + k * 8, vd + ((k * 2048) >> 4), idp, SPLIT || k > 0 || on);
             }
+            if (!SPLIT && a.dt == DT_F16)
+#pragma unroll
+              for (int k = 0; k < BN / 16; ++k) pt_mma_ts(tm + Sh::O_COL, pc + 32 + k * 8, vd + ((k * 2048) >> 4), idp, true);
             tg_commit(&o_done[b]);
             tg_commit(&v_empty[st]);
           }
