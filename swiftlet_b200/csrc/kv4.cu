@@ -104,6 +104,7 @@ constexpr int IO_U = 4;       // rows a warp has in flight
 template <int DT, bool READ, int HD, int GROUP>
 __global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool vk, bool vv, int tshift) {
   constexpr int LPR = HD / 8, RPW = 32 / LPR, NG = HD / GROUP;  // lanes a row, rows a warp, groups a row
+  pdl_wait();
   const Kv4Geo& g = a.g;
   const int lane = threadIdx.x & 31, sub = lane / LPR, l = lane % LPR;
   const int64_t j0 = (int64_t(blockIdx.x) * (IO_THREADS / 32) + (threadIdx.x >> 5)) << tshift;
@@ -215,11 +216,11 @@ void launch_io_dt(const Kv4IoArgs& a, cudaStream_t st) {
   const int per = IO_THREADS / 32 << tshift;
   const bool vk = vec_rows(a.k, DT), vv = vec_rows(a.v, DT);
   const dim3 grid((a.b.total + per - 1) / per), block(IO_THREADS);
-  if (a.g.hd == 64) launch(k_kv4_io<DT, READ, 64, 64>, grid, block, 0, st, false, a, vk, vv, tshift);
-  else if (a.g.hd == 128 && a.g.group == 64) launch(k_kv4_io<DT, READ, 128, 64>, grid, block, 0, st, false, a, vk, vv, tshift);
-  else if (a.g.hd == 128) launch(k_kv4_io<DT, READ, 128, 128>, grid, block, 0, st, false, a, vk, vv, tshift);
-  else if (a.g.group == 64) launch(k_kv4_io<DT, READ, 256, 64>, grid, block, 0, st, false, a, vk, vv, tshift);
-  else launch(k_kv4_io<DT, READ, 256, 128>, grid, block, 0, st, false, a, vk, vv, tshift);
+  if (a.g.hd == 64) launch(k_kv4_io<DT, READ, 64, 64>, grid, block, 0, st, true, a, vk, vv, tshift);
+  else if (a.g.hd == 128 && a.g.group == 64) launch(k_kv4_io<DT, READ, 128, 64>, grid, block, 0, st, true, a, vk, vv, tshift);
+  else if (a.g.hd == 128) launch(k_kv4_io<DT, READ, 128, 128>, grid, block, 0, st, true, a, vk, vv, tshift);
+  else if (a.g.group == 64) launch(k_kv4_io<DT, READ, 256, 64>, grid, block, 0, st, true, a, vk, vv, tshift);
+  else launch(k_kv4_io<DT, READ, 256, 128>, grid, block, 0, st, true, a, vk, vv, tshift);
 }
 
 template <bool READ>
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_kv4_evict_select(const Kv4Evi
   extern __shared__ uint32_t keys[];
   __shared__ __align__(8) int hist[2][EV_BINS];
   __shared__ int warp_sums[33], s_bin, s_above, s_cnt[2];
+  pdl_wait();
   const int seq = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
   const int rank = int(cluster_rank()), ncl = gridDim.x;  // one cluster in x
   const int len = kv4_len(a.b, seq), nl = min(len, a.keep);
@@ -398,6 +400,7 @@ constexpr int EC_ROWS = 64;  // survivors a block
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv4_evict_copy(const Kv4EvictArgs a) {
   constexpr int NW = HD / 64;
+  pdl_wait();
   const Kv4Geo& g = a.g;
   const int seq = blockIdx.z, h = blockIdx.y, u = threadIdx.x & 7;
   const int len = kv4_len(a.b, seq), nl = min(len, a.keep);
@@ -566,13 +569,13 @@ void launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t st) {
   // of 65536 take 33 us with eight, 130 us with one
   int cl = EV_CL;
   while (cl > 1 && int64_t(cl) * a.g.kvh * a.b.nseq > 148) cl >>= 1;
-  launch_cluster(k_kv4_evict_select, dim3(cl, a.g.kvh, a.b.nseq), dim3(EV_THREADS), dim3(cl, 1, 1), EV_SMEM, st, false, a);
+  launch_cluster(k_kv4_evict_select, dim3(cl, a.g.kvh, a.b.nseq), dim3(EV_THREADS), dim3(cl, 1, 1), EV_SMEM, st, true, a);
   const int most = std::min(a.keep, a.b.max_len);
   if (most < 1) return;
   const dim3 grid((most + EC_ROWS - 1) / EC_ROWS, a.g.kvh, a.b.nseq), block(256);
-  if (a.g.hd == 64) launch(k_kv4_evict_copy<64>, grid, block, 0, st, false, a);
-  else if (a.g.hd == 128) launch(k_kv4_evict_copy<128>, grid, block, 0, st, false, a);
-  else launch(k_kv4_evict_copy<256>, grid, block, 0, st, false, a);
+  if (a.g.hd == 64) launch(k_kv4_evict_copy<64>, grid, block, 0, st, true, a);
+  else if (a.g.hd == 128) launch(k_kv4_evict_copy<128>, grid, block, 0, st, true, a);
+  else launch(k_kv4_evict_copy<256>, grid, block, 0, st, true, a);
 }
 
 }  // namespace swl

@@ -300,7 +300,8 @@ __device__ __forceinline__ float* attn_lse(const Kv4AttnArgs& a) { return a.lse 
 // The item that begins in a share and goes on: shares first .. last hold its
 // parts (first < 0: none).
 struct AtJoin {
-  int first, last, row0, n, cb, h, every, pad;  // every: no share is empty
+  int first, last, row0, n, cb, h;
+  int64_t total;  // of the launch
 };
 __device__ __forceinline__ AtJoin* attn_joins(const Kv4AttnArgs& a) {
   return reinterpret_cast<AtJoin*>(a.work + (int64_t(a.b.total) * a.heads * 4 + 15) / 16 * 16);
@@ -323,6 +324,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
   extern __shared__ __align__(128) uint8_t at_raw[];
   Sh& sh = *reinterpret_cast<Sh*>(at_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
   pdl_launch();
   const int64_t total = total_tiles(a);
   const int64_t r0 = share_begin(total, blockIdx.x), r1 = share_begin(total, blockIdx.x + 1);
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
     const int tb = max(0, p.tile - AT_HEAD), t1 = v1 - AT_HEAD, slot = p.tile == 0 ? 1 : 0;
     if (threadIdx.x == 0 && p.tile == 0 && v1 < p.tiles) {
       const int first = share_of(total, f + AT_HEAD), last = share_of(total, f + p.tiles - 1);
-      if (first < last) attn_joins(a)[blockIdx.x] = AtJoin{first, last, p.row0, p.n, cb, h, total >= AT_GRID, 0};
+      if (first < last) attn_joins(a)[blockIdx.x] = AtJoin{first, last, p.row0, p.n, cb, h, total};
     }
     f += v1 - p.tile;
     if (t1 <= 0) continue;  // only overhead of the next share's item
@@ -662,12 +664,11 @@ __global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
   __shared__ float red[32];
   const float* parts = attn_parts(a);
   auto part = [&](int i) { return parts + (int64_t(i) * 2 + (i == x ? 1 : 0)) * part_floats(HD); };
-  int64_t total = 0;
-  if (!d.every) total = total_tiles(a);  // fewer tiles than shares: the empty ones have no part
   const int np = d.last - d.first + 1;
   float M = -INFINITY;
   for (int i = threadIdx.x; i < np; i += HD) {
-    const bool has = d.every || share_begin(total, d.first + i) < share_begin(total, d.first + i + 1);
+    // with fewer tiles than shares some are empty, and have no part
+    const bool has = d.total >= AT_GRID || share_begin(d.total, d.first + i) < share_begin(d.total, d.first + i + 1);
     const float mi = has ? __ldcg(part(d.first + i) + col) : -INFINITY;
     wt[i] = mi;
     M = fmaxf(M, mi);
@@ -708,6 +709,7 @@ __global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs
   constexpr int NG = HD / GROUP, NW = HD / 64;
   __shared__ __align__(16) QStage<HD, SPLIT> sq[2];
   __shared__ float slse[2][AT_COLS];
+  pdl_wait();
   const Kv4Geo& g = a.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int h = blockIdx.y;
@@ -784,15 +786,16 @@ bool few_rows(const Kv4Batch& b, int rep) { return int64_t(b.max_new) * rep <= A
 template <int HD, int GROUP, bool SPLIT>
 void run(const Kv4AttnArgs& a, cudaStream_t st) {
   if (few_rows(a.b, a.rep)) {
-    launch(k_kv4_attn<HD, GROUP, SPLIT>, dim3(AT_GRID), dim3(AT_THREADS), sizeof(AttnShared<HD, GROUP, SPLIT>), st, false, a);
-    launch(k_kv4_attn_join<HD>, dim3(AT_GRID, AT_COLS), dim3(HD), 0, st, true, a);
+    launch(k_kv4_attn<HD, GROUP, SPLIT>, dim3(AT_GRID), dim3(AT_THREADS), sizeof(AttnShared<HD, GROUP, SPLIT>), st, true, a);
+    if (a.b.max_len > AT_TILE)  // or every item is one tile, and written at once
+      launch(k_kv4_attn_join<HD>, dim3(AT_GRID, AT_COLS), dim3(HD), 0, st, true, a);
   } else {
     launch_kv4_prompt(a, st);
     return;
   }
   if (a.weights && a.b.max_len > 0)
     launch(k_kv4_weights<HD, GROUP, SPLIT>, dim3((a.b.max_len + AT_TILE - 1) / AT_TILE, a.g.kvh, a.b.nseq), dim3(WT_WARPS * 32), 0, st,
-           false, a);
+           true, a);
 }
 
 template <int HD, int GROUP>

@@ -280,7 +280,8 @@ __device__ __forceinline__ void pt_next(const Kv4AttnArgs& a, int bn, PtPlace& p
 // The item that begins in a share and goes on: shares first .. last hold its
 // parts (first < 0: none).
 struct PtJoin {
-  int first, last, row0, n, qt, h, pad[2];
+  int first, last, row0, n, qt, h;
+  int64_t total;  // of the launch
 };
 
 // Workspace: lse rows, ranges, joins, parts.
@@ -298,6 +299,7 @@ __device__ __forceinline__ float* pt_parts(const Kv4AttnArgs& a) { return reinte
 // as f32 bits, and flags (bit 0: a value group is NaN, bit 1: a page outside the
 // pool), over one of RG_SPLIT shares of the slots a block.
 __global__ void __launch_bounds__(256) k_kv4_range(const Kv4AttnArgs a) {
+  pdl_wait();
   pdl_launch();
   const int seq = blockIdx.y / a.g.kvh, h = blockIdx.y % a.g.kvh;
   int row0;
@@ -711,7 +713,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
       tg_fence_before();
     });
     if (warp == 0) {  // what the join kernel has to do for this share
-      PtJoin d = {-1, -1, 0, 0, 0, 0, {0, 0}};
+      PtJoin d = {-1, -1, 0, 0, 0, 0, 0};
       if (r0 < r1) {
         const PtPlace p = pt_find(a, BN, r1 - 1);
         const int64_t begin = r1 - 1 - p.tile, end = begin + p.tiles;
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           int first = blockIdx.x, last = blockIdx.x;
           while (total * (first + 1) / nc <= begin + PT_HEAD) ++first;
           while (last + 1 < nc && total * (last + 1) / nc < end) ++last;
-          if (first < last) d = PtJoin{first, last, p.row0, p.n, p.qt, p.h, {0, 0}};
+          if (first < last) d = PtJoin{first, last, p.row0, p.n, p.qt, p.h, total};
         }
       }
       if (lane == 0) pt_joins(a)[blockIdx.x] = d;
@@ -972,7 +974,7 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4AttnArgs a) {
   const unsigned ci = unsigned(d.qt * PT_ROWS + r);
   const int tok = int(ci / unsigned(a.rep)), hq = d.h * a.rep + int(ci % unsigned(a.rep));
   if (tok >= d.n) return;
-  const int64_t total = pt_total(a, PT_BN), step = pt_part_floats(HD);
+  const int64_t total = d.total, step = pt_part_floats(HD);
   auto part = [&](int i) { return pt_parts(a) + (int64_t(i) * 2 + (i == x ? 1 : 0)) * step; };
   // shares without tiles (fewer tiles than CTAs) have no part
   auto has = [&](int i) { return i == d.first || total * i / PT_GRID < total * (i + 1) / PT_GRID; };
@@ -1035,6 +1037,7 @@ __host__ __device__ inline int64_t wq_tiles(int64_t total, int rep, int nseq) { 
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(256) k_kv4_queries(const Kv4AttnArgs a) {
   using Sh = WqShape<HD, SPLIT>;
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t wid = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int64_t j = wid / a.heads;
@@ -1095,6 +1098,7 @@ __global__ void __launch_bounds__(WQ_THREADS, SPLIT ? 1 : 2) k_kv4_prompt_weight
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* half_sum = reinterpret_cast<float*>(tmem_slot + 4);
+  pdl_wait();
   const Kv4Geo& g = a.g;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, seq = blockIdx.z;
   int row0;
@@ -1268,14 +1272,15 @@ __global__ void __launch_bounds__(WQ_THREADS, SPLIT ? 1 : 2) k_kv4_prompt_weight
 template <int HD, int GROUP, bool SPLIT>
 void run(const Kv4AttnArgs& a, cudaStream_t st) {
   using Sh = PtShape<HD, GROUP, SPLIT>;
-  launch(k_kv4_range, dim3(RG_SPLIT, a.b.nseq * a.g.kvh), dim3(256), 0, st, false, a);
+  launch(k_kv4_range, dim3(RG_SPLIT, a.b.nseq * a.g.kvh), dim3(256), 0, st, true, a);
   launch(k_kv4_prompt<HD, GROUP, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS), Sh::TOTAL, st, true, a);
-  launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(256), 0, st, true, a);
+  if (a.b.max_len > PT_BN)  // or every item is one tile, and written at once
+    launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(256), 0, st, true, a);
   if (a.weights && a.b.max_len > 0) {
     const int64_t rows = int64_t(a.b.total) * a.heads;
-    launch(k_kv4_queries<HD, SPLIT>, dim3(unsigned((rows + 7) / 8)), dim3(256), 0, st, false, a);
+    launch(k_kv4_queries<HD, SPLIT>, dim3(unsigned((rows + 7) / 8)), dim3(256), 0, st, true, a);
     launch(k_kv4_prompt_weights<HD, GROUP, SPLIT>, dim3((a.b.max_len + 127) / 128, a.g.kvh, a.b.nseq), dim3(WQ_THREADS),
-           WqShape<HD, SPLIT>::TOTAL, st, false, a);
+           WqShape<HD, SPLIT>::TOTAL, st, true, a);
   }
 }
 
