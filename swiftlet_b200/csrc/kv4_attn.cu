@@ -467,7 +467,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
       unsigned sb = __vmaxu2(vp[0][0], vp[1][0]);  // scales are the low halves, and positive
 #pragma unroll
       for (int i = 1; i < NG; ++i) sb = __vmaxu2(sb, __vmaxu2(vp[0][i], vp[1][i]));
-      sb = __reduce_max_sync(0xffffffffu, min(sb & 0xffffu, 0x7bffu));
+      sb = __reduce_max_sync(0xffffffffu, sb & 0xffffu);
+      if (sb >= 0x7c00u) {  // groups that read as NaN have no say: a column that sees none of them keeps its bits
+        sb = 0u;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if ((vp[k][i] & 0x7c00u) != 0x7c00u) sb = max(sb, vp[k][i] & 0xffffu);
+        sb = __reduce_max_sync(0xffffffffu, sb);
+      }
       // The reference point moves only when the maximum has outgrown it by
       // 2^8 or the scales theirs: p then stays below 2^8, p s below 2^15.
       if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f) || sb > smax) {

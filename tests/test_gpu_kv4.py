@@ -345,6 +345,23 @@ def test_nan_and_infinity_stay_where_they_are():
             check(c, lens2, new2, 8, got[sub], lse[sub], q[sub], held=seen)
 
 
+@pytest.mark.parametrize("dtype", [0, 1], ids=["f32", "bf16"])
+def test_nan_value_leaves_other_rows_their_bits(dtype):
+    """A value group that reads as NaN, in the last of a few new tokens: the rows before it do not see it, and are as exact as
+    without it (queries so small that a score's own error is no part of the bound)."""
+    torch, _ = _torch()
+    rng = np.random.default_rng(8)
+    c = Cache(1, 20, 2, 256)
+    x = rng.standard_normal((2, 20, 2, 256)).astype(np.float32)
+    x[1, 19, :, 70] = np.inf
+    d = torch.from_numpy(x).cuda()
+    swl.kv4_append_device(c.desc(), c.batch([20], [20]), d[0].data_ptr(), d[1].data_ptr())
+    c.held[:] = quantise(x, 64).reshape(2, 1, 20, 2, 256)
+    got, lse, q = attend(c, [20], [2], 8, rng, dtype=dtype, qgain=0.02)
+    assert np.isnan(got[1, :, 64:128]).all()
+    check(c, [19], [1], 8, got[:1], lse[:1], q[:1], dtype=dtype, held=c.held)
+
+
 def test_nan_query_stays_in_its_row():
     torch, _ = _torch()
     for new in (1, 20):
