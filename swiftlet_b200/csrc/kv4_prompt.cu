@@ -301,11 +301,11 @@ __device__ __forceinline__ float* pt_parts(const Kv4AttnArgs& a) { return reinte
 __global__ void __launch_bounds__(256) k_kv4_range(const Kv4AttnArgs a) {
   pdl_wait();
   pdl_launch();
-  const int seq = blockIdx.y / a.g.kvh, h = blockIdx.y % a.g.kvh;
+  const int pair = blockIdx.x, seq = pair / a.g.kvh, h = pair % a.g.kvh;
   int row0;
   const int n = kv4_new(a.b, seq, row0), len = n ? kv4_len(a.b, seq) : 0;
   unsigned mk = 0u, mv = 0u, nan = 0u;
-  for (int s = blockIdx.x * 256 + threadIdx.x; s < len; s += 256 * RG_SPLIT) {
+  for (int s = blockIdx.y * 256 + threadIdx.x; s < len; s += 256 * RG_SPLIT) {
     const uint8_t* blk = kv4_block(a.g, a.g.table, a.g.tstride, seq, h, s, a.b.status);
     if (!blk) {
       nan |= 2u;
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(256) k_kv4_range(const Kv4AttnArgs a) {
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 8; ++w) mk = max(mk, red[0][w]), mv = max(mv, red[1][w]), nan |= red[2][w];
-    pt_ranges(a)[int64_t(blockIdx.y) * RG_SPLIT + blockIdx.x] = make_int4(int(mk), int(mv), int(nan), 0);
+    pt_ranges(a)[int64_t(pair) * RG_SPLIT + blockIdx.y] = make_int4(int(mk), int(mv), int(nan), 0);
   }
 }
 
@@ -1272,7 +1272,7 @@ __global__ void __launch_bounds__(WQ_THREADS, SPLIT ? 1 : 2) k_kv4_prompt_weight
 template <int HD, int GROUP, bool SPLIT>
 void run(const Kv4AttnArgs& a, cudaStream_t st) {
   using Sh = PtShape<HD, GROUP, SPLIT>;
-  launch(k_kv4_range, dim3(RG_SPLIT, a.b.nseq * a.g.kvh), dim3(256), 0, st, true, a);
+  launch(k_kv4_range, dim3(a.b.nseq * a.g.kvh, RG_SPLIT), dim3(256), 0, st, true, a);
   launch(k_kv4_prompt<HD, GROUP, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS), Sh::TOTAL, st, true, a);
   if (a.b.max_len > PT_BN)  // or every item is one tile, and written at once
     launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(256), 0, st, true, a);
@@ -1302,7 +1302,6 @@ int64_t kv4_prompt_work(const Kv4Geo& g, const Kv4Batch& b, int heads) {
 
 void launch_kv4_prompt(const Kv4AttnArgs& a, cudaStream_t st) {
   if (int64_t(a.b.total) * a.rep > 0x7fffff00) throw Error(ERR_UNSUPPORTED, "kv4: more than 2^31 query rows a kv head");
-  if (int64_t(a.b.nseq) * a.g.kvh > 65535) throw Error(ERR_UNSUPPORTED, "kv4: more than 65535 sequences x kv heads with prompts");
   if (a.g.hd == 64) run_dt<64, 64>(a, st);
   else if (a.g.hd == 128) a.g.group == 64 ? run_dt<128, 64>(a, st) : run_dt<128, 128>(a, st);
   else a.g.group == 64 ? run_dt<256, 64>(a, st) : run_dt<256, 128>(a, st);
