@@ -15,16 +15,20 @@
 // and outputs are f32. Columns are scaled by powers of two on their way into
 // f16 (q by its largest element, p by the largest group scale seen), which
 // changes no bit of the result but keeps both terms in range.
-// For 16-bit inputs e = c, b' = b: one LOP3 a pair. For f32 inputs e = c -
-// 7.5 and b' = b + 7.5 s, the middle of the group (10 instructions per 8 codes
-// instead of 5): the accumulators truncate, so a sum is off by its largest
-// partial sums, and with codes of one sign those are twice the score's (its
-// error then measured 7.6e-6 on scores of 1.5) and 150 times the output's (at
-// 128k equal weights).
+// That is for f32 inputs (10 instructions per 8 codes): the accumulators
+// truncate, so a sum is off by its largest partial sums, and with codes of one
+// sign those are twice the score's (its error then measured 7.6e-6 on scores of
+// 1.5) and 150 times the output's (at 128k equal weights). For 16-bit inputs e
+// = c and b' = b: one LOP3 a pair, 5 instructions per 8 codes.
 //
 // Bound: the cache's bytes (2 (D / 2 + 4 D / g) a slot and kv head), next to
-// the instructions of unpacking and weighting, which is why codes go to the
-// tensor cores unscaled and the scales are applied to the 16 x 8 results.
+// the instructions of unpacking and weighting (f32: some 1050 a unit of 16
+// slots at 256 channels and 2.1 a cycle and SM, which is what f32 waits for),
+// which is why codes go to the tensor cores unscaled and the scales are applied
+// to the 16 x 8 results. 2 kv heads of 256 channels, 16 query heads: one
+// sequence of 131072 slots in f32 54 to 59 us (1.3 to 1.4 TB/s), 64 of 61 to
+// 8192 slots in f32 81 us (1.9 TB/s), 64 of 20000 to 32768 in bf16 230 us (4.2
+// TB/s).
 #include <algorithm>
 
 #include "kcommon.cuh"
@@ -35,7 +39,7 @@ namespace swl {
 
 namespace {
 
-constexpr int AT_WARPS = 12;                // three per scheduler at 168 registers
+constexpr int AT_WARPS = 12;                // three per scheduler at 168 registers (8 and 16 were no faster)
 constexpr int AT_THREADS = AT_WARPS * 32;
 constexpr int AT_UNIT = 16;                 // slots a warp takes at a time: the MMA's M (keys) and K (values)
 constexpr int AT_TILE = 128;                // slots of a tile, the grain in which work is shared out
@@ -88,7 +92,8 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 // ceil(len / 128) tiles (one at least); a CTA takes an equal, contiguous share
 // of all tiles, so ragged batches and single long sequences spread alike. An
 // item counts AT_HEAD tiles more, in front of its own, for its beginning and
-// end (queries, first copies, combination of the warps).
+// end (queries, first copies, combination of the warps): 64 sequences of 61
+// to 8192 slots took 97 us with one, 81 with four.
 // Every warp finds its place from the lengths in device memory: nothing of the
 // split is known to the host.
 struct Place {
@@ -712,7 +717,9 @@ __global__ void __launch_bounds__(HD) k_kv4_attn_join(const Kv4AttnArgs a) {
 // scores computed again from the keys alone (half the cache's bytes; writing
 // them out and reading them back would be as much at 8 query heads a kv head
 // and would need space of rows x slots). A CTA owns 128 slots of a kv head and
-// walks all the sequence's columns, so every sum has one order.
+// walks all the sequence's columns, so every sum has one order. Bound: latency
+// (a single token, 16 sequences of 3000 to 8200 slots in f32: 63 us with the
+// attention, of which this is some 20).
 template <int HD, int GROUP, bool SPLIT>
 __global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs a) {
   constexpr int NG = HD / GROUP, NW = HD / 64;
@@ -787,9 +794,13 @@ __global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs
   }
 }
 
-// Query rows a kv head from which the tensor-core prompt kernel is used: a
-// tile there costs the same for 1 to 128 rows, here for every 8.
-constexpr int64_t AT_FEW = 16;
+// Query rows a kv head up to which these kernels are used. A tile of the prompt
+// kernel costs the same for 1 to 128 rows, here every 8 rows take the item's
+// tiles once more. 32 sequences of 2000 slots (2 kv heads of 256 channels,
+// bf16): 16 rows 33 us here and 99 there, 64 rows 92 and 103, 96 rows 131 and
+// 106 (f32: 64 rows 138 and 150, 96 rows 197 and 155). One of 30000 slots: 64
+// rows 42 and 106, 96 rows 55 and 119.
+constexpr int64_t AT_FEW = 64;
 bool few_rows(const Kv4Batch& b, int rep) { return int64_t(b.max_new) * rep <= AT_FEW; }
 
 template <int HD, int GROUP, bool SPLIT>

@@ -4,7 +4,7 @@
 // An item is 128 query rows (token-major, the heads of one kv head adjacent)
 // of one sequence and kv head; the context is walked in tiles of BN slots:
 //   S = Q K^T (tcgen05.mma, M 128, N BN, K head_dim; accumulator in TMEM),
-//   online softmax by one thread a row, P to TMEM as f16,
+//   online softmax by two threads a row, P to TMEM as f16,
 //   O += P V (M 128, N head_dim, K BN; A from TMEM, V as an N-major operand).
 // Keys and values are unpacked to f16 on their way into shared memory, scaled
 // by a power of two so that the largest value of the sequence and head is
@@ -12,23 +12,30 @@
 // terms: lse and the weights are f32 whatever the inputs' type, and with keys
 // of 11 bits scores were off by 1e-4. 16-bit inputs: queries and values are one
 // term (values rounded to 11 bits like the inputs themselves), so two products
-// make S and one O; for f16 the weights are two terms and O takes two (with
-// one, outputs were off by 1.6 times their own rounding, with two 1.2 times). f32 inputs: all operands are two terms (22 bits) and
-// three products each make S and O (hi lo, lo hi, hi hi).
+// make S and one O; for f16 the weights are two terms and O takes two (with one,
+// outputs were off by 1.6 times their own rounding, with two 1.2 times). f32
+// inputs: all operands are two terms (22 bits) and three products each make S
+// and O (hi lo, lo hi, hi hi).
 // The tensor cores' f32 accumulators truncate: every product added takes up to
 // 2^-24 off the size of what it is added to. S is built from its small terms up;
 // for f32 inputs O is taken out of TMEM every PT_FLUSH tiles and added up with
 // correct rounding (without that, outputs were off by 1.5e-5 after some 30 tiles).
 //
 // Warps: 0-7 softmax and output (two threads a row, half of the tile's slots
-// each), 8-15 unpacking of keys, 16-23 of values, 24 MMA issue and TMEM, 25 and 26 bulk copies
-// of the cache's bytes (a tile's keys, a tile's values) into a ring of stages. Q stands in TMEM (its low terms in shared
-// memory), S and P share columns and are double-buffered, so Q K^T of the next
-// tile runs during the softmax of this one; the running maximum moves only
-// when it has grown by 2^8, so O in TMEM is rarely touched. Bound: the tensor
-// cores (a tile of 64 slots at 256 channels is 1024 cycles of MMA for 16-bit
-// inputs), next to the issue slots of the unpacking (14 instructions per 8
-// values) and of the softmax.
+// each), 8-15 unpacking of keys, 16-23 of values, 24 MMA issue and TMEM, 25 and
+// 26 bulk copies of the cache's bytes (a tile's keys, a tile's values) into a
+// ring of stages each. Q stands in TMEM (its low terms in shared memory), S and
+// P share columns and are double-buffered, so Q K^T of the next tile runs
+// during the softmax of this one; the running maximum moves only when it has
+// grown by 2^8, so O in TMEM is rarely touched. Bound: the chain of copy,
+// unpack, product, softmax, product. A tile of 64 slots at 256 channels is 1536
+// cycles of MMA for bf16 (3072 for f32), and takes some 3000 (6000): the unpack
+// (14 instructions per 8 values) and the softmax share the issue slots, and
+// shared memory holds two buffers of unpacked tiles at most (one for f32).
+// 2048 tokens on a context of 10000 (2 kv heads of 256 channels, 16 query heads,
+// bf16): 490 us, 0.61 PFLOP/s; 8192 tokens from the first (4 kv heads of 128, 16
+// query heads, f16, four products): 690 us, 0.40; 8 chunks of 33 to 200 tokens
+// on 900 to 4100 (2 of 256, f32, six products): 245 us, 0.16.
 //
 // The work is shared out like that of kv4_attn.cu: equal contiguous shares of
 // all tiles of all items over 148 CTAs, parts of an item that several CTAs
@@ -52,7 +59,9 @@ constexpr int PT_THREADS = PT_SOFT + PT_UNPACK + 128;   // and a warpgroup that 
 constexpr int PT_MMA = (PT_SOFT + PT_UNPACK) / 32, PT_COPY = PT_MMA + 1;  // warps
 // Registers a thread: 72 at launch, then 256 x 96 + 512 x 64 + 128 x 56 (= 896 x 72).
 constexpr int PT_REGS_SOFT = 96, PT_REGS_UNPACK = 64, PT_REGS_ISSUE = 56;
-constexpr int PT_HEAD = 12;                             // cost of an item beside its tiles, in tiles
+// Cost of an item beside its tiles, in tiles (queries, filling the pipeline, output): 8192 tokens
+// from the first, whose early items are short, took 1487 us with one, 690 with twelve; chunks on long contexts 285 and 248.
+constexpr int PT_HEAD = 12;
 constexpr int PT_FLUSH = 4;                             // tiles that O of f32 inputs stays in TMEM
 constexpr int RG_SPLIT = 16;                            // blocks a (sequence, head) of the range kernel
 constexpr float P_LOG2E = 1.4426950408889634f, P_LN2 = 0.6931471805599453f;
@@ -1013,7 +1022,9 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4AttnArgs a) {
 // keys are unpacked once, into TMEM; the queries come as f16 tiles that
 // k_kv4_queries lays out once for all of them. A CTA owns its slots: every sum
 // has one order. Bound: 512 cycles of MMA (16-bit inputs, 256 channels) and 512
-// of exponentials a step of 128 x 64.
+// of exponentials a step of 128 x 64. 1000 tokens on 3000 slots (2 kv heads of
+// 256 channels, 16 query heads, bf16): 115 us, where the kernel for few rows
+// took 1390.
 constexpr int WQ_COLS = 64;  // query rows of a tile
 
 template <int HD, bool SPLIT>
