@@ -973,46 +973,53 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
   }
 }
 
-// Joins the parts of the item that begins in share x and goes on: a warp a row.
+// Joins the parts of the item that begins in share x and goes on: a block eight
+// rows, a thread eight channels of one (a warp reads four runs of 128 bytes).
 template <int HD>
-__global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(HD) k_kv4_prompt_join(const Kv4AttnArgs a) {
   pdl_wait();
-  const int x = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int x = blockIdx.x, j = threadIdx.x >> 3, r = blockIdx.y * 8 + (threadIdx.x & 7);
   const PtJoin d = pt_joins(a)[x];
   if (d.first < 0) return;
   const unsigned ci = unsigned(d.qt * PT_ROWS + r);
   const int tok = int(ci / unsigned(a.rep)), hq = d.h * a.rep + int(ci % unsigned(a.rep));
-  if (tok >= d.n) return;
   const int64_t total = d.total, step = pt_part_floats(HD);
   auto part = [&](int i) { return pt_parts(a) + (int64_t(i) * 2 + (i == x ? 1 : 0)) * step; };
   // shares without tiles (fewer tiles than CTAs) have no part
-  auto has = [&](int i) { return i == d.first || total * i / PT_GRID < total * (i + 1) / PT_GRID; };
+  auto has = [&](int i) { return i == d.first || total >= PT_GRID || total * i / PT_GRID < total * (i + 1) / PT_GRID; };
+  // the row's maximum: four lanes of the warp have the row
   float M = -INFINITY, L = 0.f;
-  for (int i = d.first + lane; i <= d.last; i += 32)
+  for (int i = d.first + (j & 3); i <= d.last; i += 4)
     if (has(i)) M = fmaxf(M, __ldcg(part(i) + r));
-  M = warp_max(M);
-  constexpr int E = HD / 32;
-  float v[E];
+  M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
+  M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+  if (tok >= d.n) return;
+  float v[8];
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = 0.f;
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
 #pragma unroll 4
   for (int i = d.first; i <= d.last; ++i) {
     if (!has(i)) continue;
     const float* q = part(i);
+    const float4* o4 = reinterpret_cast<const float4*>(q + 2 * PT_ROWS) + 2 * j * PT_ROWS + r;
+    const float4 o0 = __ldcg(o4), o1 = __ldcg(o4 + PT_ROWS);
     const float mi = __ldcg(q + r), f = mi == -INFINITY ? 0.f : pt_ex2(mi - M);
     L = fmaf(__ldcg(q + PT_ROWS + r), f, L);
+    const float o[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = fmaf(__ldcg(q + 2 * PT_ROWS + ((e * 32 + lane) / 4 * PT_ROWS + r) * 4 + lane % 4), f, v[e]);
+    for (int e = 0; e < 8; ++e) v[pt_channel(e)] = fmaf(o[e], f, v[pt_channel(e)]);
   }
   const int64_t row = d.row0 + tok;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int ch = e * 32 + (lane & ~7) + pt_channel(lane & 7);
-    float o = L == 0.f ? v[e] : v[e] / L;  // an empty row: zeros
-    if (a.gate.p) o *= kv4_sigmoid(kv4_ld(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + ch));
-    kv4_st(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + ch, o);
+  for (int e = 0; e < 8; ++e) v[e] = L == 0.f ? v[e] : v[e] / L;  // an empty row: zeros
+  if (a.gate.p) {
+    float g[8];
+    kv4_ld8(a.gate.p, a.dt, row * a.gate.ts + hq * a.gate.hs + j * 8, kv4_vec(a.gate, a.dt), g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= kv4_sigmoid(g[e]);
   }
-  if (lane == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * P_LN2;
+  kv4_st8(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + j * 8, kv4_vec(a.out, a.dt), v);
+  if (j == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * P_LN2;
 }
 
 // ------------------------------------------------------- accumulated weight --
@@ -1286,7 +1293,7 @@ void run(const Kv4AttnArgs& a, cudaStream_t st) {
   launch(k_kv4_range, dim3(a.b.nseq * a.g.kvh, RG_SPLIT), dim3(256), 0, st, true, a);
   launch(k_kv4_prompt<HD, GROUP, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS), Sh::TOTAL, st, true, a);
   if (a.b.max_len > PT_BN)  // or every item is one tile, and written at once
-    launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(256), 0, st, true, a);
+    launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(HD), 0, st, true, a);
   if (a.weights && a.b.max_len > 0) {
     const int64_t rows = int64_t(a.b.total) * a.heads;
     launch(k_kv4_queries<HD, SPLIT>, dim3(unsigned((rows + 7) / 8)), dim3(256), 0, st, true, a);
