@@ -36,9 +36,71 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// Smallest and largest of a group's values: eight a lane, GROUP / 8 lanes.
+template <int GROUP>
+__device__ __forceinline__ void group_range(const float (&x)[8], float& mn, float& mx) {
+  mn = mx = x[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) {
+    mn = min_nan(mn, x[e]);
+    mx = max_nan(mx, x[e]);
+  }
+#pragma unroll
+  for (int o = 1; o < GROUP / 8; o <<= 1) {
+    mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+}
+// Two 16-bit values an instruction; min and -max travel as one word.
 template <int DT>
-__device__ __forceinline__ void load8(const uint8_t* p, int64_t i, bool vec, float (&x)[8]) {
-  if (DT == DT_F32) {
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (DT == DT_BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <int DT, int GROUP>
+__device__ __forceinline__ void group_range(const uint4& w, float& mn, float& mx) {
+  constexpr uint32_t NEG = 0x80008000u;
+  const uint32_t lo = min2_nan<DT>(min2_nan<DT>(w.x, w.y), min2_nan<DT>(w.z, w.w));
+  const uint32_t hi = min2_nan<DT>(min2_nan<DT>(w.x ^ NEG, w.y ^ NEG), min2_nan<DT>(w.z ^ NEG, w.w ^ NEG));
+  uint32_t t = min2_nan<DT>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+#pragma unroll
+  for (int o = 1; o < GROUP / 8; o <<= 1) t = min2_nan<DT>(t, __shfl_xor_sync(0xffffffffu, t, o));
+  t ^= 0x80000000u;
+  mn = DT == DT_BF16 ? bf16_to_f32(uint16_t(t)) : f16_bits_to_f32(uint16_t(t));
+  mx = DT == DT_BF16 ? bf16_to_f32(uint16_t(t >> 16)) : f16_bits_to_f32(uint16_t(t >> 16));
+}
+
+// Eight values as they come, and as f32.
+template <int DT>
+struct Row8 {
+  uint4 w;
+  __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void load(const uint8_t* p, int64_t i, bool vec) {
+    const uint16_t* f = reinterpret_cast<const uint16_t*>(p) + i;
+    if (vec) {
+      w = *reinterpret_cast<const uint4*>(f);
+    } else {
+      w.x = f[0] | uint32_t(f[1]) << 16, w.y = f[2] | uint32_t(f[3]) << 16, w.z = f[4] | uint32_t(f[5]) << 16, w.w = f[6] | uint32_t(f[7]) << 16;
+    }
+  }
+  __device__ __forceinline__ float at(int e) const {
+    const uint32_t u = e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w;
+    if (DT == DT_BF16) return __uint_as_float(e & 1 ? u & 0xffff0000u : u << 16);
+    return f16_bits_to_f32(uint16_t(e & 1 ? u >> 16 : u));
+  }
+  template <int GROUP>
+  __device__ __forceinline__ void range(float& mn, float& mx) const { group_range<DT, GROUP>(w, mn, mx); }
+};
+template <>
+struct Row8<DT_F32> {
+  float x[8];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  }
+  __device__ __forceinline__ void load(const uint8_t* p, int64_t i, bool vec) {
     const float* f = reinterpret_cast<const float*>(p) + i;
     if (vec) {
       const float4 a = reinterpret_cast<const float4*>(f)[0], b = reinterpret_cast<const float4*>(f)[1];
@@ -47,20 +109,11 @@ __device__ __forceinline__ void load8(const uint8_t* p, int64_t i, bool vec, flo
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = f[e];
     }
-  } else {
-    const uint16_t* f = reinterpret_cast<const uint16_t*>(p) + i;
-    uint16_t u[8];
-    if (vec) {
-      *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(f);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = f[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = DT == DT_BF16 ? bf16_to_f32(u[e]) : f16_bits_to_f32(u[e]);
   }
-}
-
+  __device__ __forceinline__ float at(int e) const { return x[e]; }
+  template <int GROUP>
+  __device__ __forceinline__ void range(float& mn, float& mx) const { group_range<GROUP>(x, mn, mx); }
+};
 template <int DT>
 __device__ __forceinline__ void store8(uint8_t* p, int64_t i, bool vec, const float (&x)[8]) {
   if (DT == DT_F32) {
@@ -97,9 +150,9 @@ bool vec_rows(const Kv4Rows& r, int dt) {
 // (K and V of some heads). The tokens' places (sequence, slot, page) are looked
 // up by a lane each. Bound: the rows' bytes in and out, next to about 100
 // instructions a row of quantising: nine prompts of 2500 to 9000 tokens (2 kv
-// heads of 256 channels, bf16, 137 MB each way) are written in 68 us and read in
-// 30 (2.0 and 4.5 TB/s).
-constexpr int IO_TOKENS = 8;  // tokens of a warp at most
+// heads of 256 channels, bf16, 137 MB each way) are written in 45 us and read in
+// 29 (3.0 and 4.7 TB/s).
+constexpr int IO_TOKENS = 4;  // tokens of a warp at most
 constexpr int IO_U = 4;       // rows a warp has in flight
 
 template <int DT, bool READ, int HD, int GROUP>
@@ -138,22 +191,20 @@ __global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool v
     const int wo = t * (HD / 2) + ((l & 7) ^ kv4_swz(HD, t)) * (HD / 16) + (l >> 3) * 4, po = g.seg * (HD / 2) + (t * NG + l * 8 / GROUP) * 4;
     const int64_t kj = (j0 + i) * a.k.ts + l * 8, vj = (j0 + i) * a.v.ts + l * 8;
     for (int h0 = sub; h0 - sub < g.kvh; h0 += IO_U / 2 * RPW) {
-      float x[IO_U][8];
+      Row8<DT> x[IO_U];
       uint32_t w[IO_U], pr[IO_U];
 #pragma unroll
       for (int u = 0; u < IO_U; ++u) {
         const int h = h0 + (u >> 1) * RPW, kv = u & 1;
         w[u] = pr[u] = 0u;
-        if (!READ)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
+        if (!READ) x[u].zero();
         if (h >= g.kvh) continue;
         if (READ) {
           const uint8_t* d = tb + h * hblk + (kv ? g.blk / 2 : 0);
           w[u] = *reinterpret_cast<const uint32_t*>(d + wo);
           pr[u] = *reinterpret_cast<const uint32_t*>(d + po);
         } else {
-          load8<DT>(kv ? a.v.p : a.k.p, kv ? vj + h * a.v.hs : kj + h * a.k.hs, kv ? vv : vk, x[u]);
+          x[u].load(kv ? a.v.p : a.k.p, kv ? vj + h * a.v.hs : kj + h * a.k.hs, kv ? vv : vk);
         }
       }
 #pragma unroll
@@ -164,27 +215,19 @@ __global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool v
           const float2 sb = kv4_param(pr[u]);
           // a code at bit 4e of 2^23's mantissa is 2^23 + 16^e c; s c is exact, so
           // one rounding remains
+          float y[8];
           const float s16[5] = {sb.x, sb.x * 0x1p-4f, sb.x * 0x1p-8f, sb.x * 0x1p-12f, sb.x * 0x1p-16f};
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int at4 = e < 5 ? e : e - 3;
             const uint32_t bits = (e < 5 ? w[u] : w[u] >> 12) & (15u << (4 * at4));
-            x[u][e] = fmaf(__uint_as_float(bits | 0x4b000000u) - 8388608.f, s16[at4], sb.y);
+            y[e] = fmaf(__uint_as_float(bits | 0x4b000000u) - 8388608.f, s16[at4], sb.y);
           }
-          store8<DT>(kv ? a.v.p : a.k.p, kv ? vj + h * a.v.hs : kj + h * a.k.hs, kv ? vv : vk, x[u]);
+          store8<DT>(kv ? a.v.p : a.k.p, kv ? vj + h * a.v.hs : kj + h * a.k.hs, kv ? vv : vk, y);
           continue;
         }
-        float mn = x[u][0], mx = x[u][0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) {
-          mn = min_nan(mn, x[u][e]);
-          mx = max_nan(mx, x[u][e]);
-        }
-#pragma unroll
-        for (int o = 1; o < GROUP / 8; o <<= 1) {
-          mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        }
+        float mn, mx;
+        x[u].template range<GROUP>(mn, mx);
         const __half hb = __float2half_rn(mn), hs = __float2half_rn(__fmul_rn(__fsub_rn(mx, mn), 1.f / 15.f));
         const float b = __half2float(hb), sc = __half2float(hs);
         const bool bad = !(fabsf(b) < INFINITY) || !(sc < INFINITY) || !(mx < INFINITY);
@@ -194,9 +237,10 @@ __global__ void __launch_bounds__(IO_THREADS) k_kv4_io(const Kv4IoArgs a, bool v
         uint32_t word = 0u;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[u][e], b), inv), 0.f), 15.f);
-          word += (__float_as_uint(__fadd_rn(c, 12582912.f)) - 0x4b400000u) << (4 * e);
+          const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[u].at(e), b), inv), 0.f), 15.f);
+          word += __float_as_uint(__fadd_rn(c, 12582912.f)) << (4 * e);
         }
+        word -= 0x3f400000u;  // the constant's bits, eight times
         if (h >= g.kvh) continue;
         uint8_t* d = tb + h * hblk + (kv ? g.blk / 2 : 0);
         *reinterpret_cast<uint32_t*>(d + wo) = bad ? 0u : word;
@@ -212,8 +256,8 @@ template <int DT, bool READ>
 void launch_io_dt(const Kv4IoArgs& a, cudaStream_t st) {
   // tokens a warp: as many as leave sixteen warps an SM, so that a step of a
   // few tokens still spreads over the GPU (64 tokens: 8 us with one a warp, 26
-  // with eight; nine prompts of 2500 to 9000, written and read: 119 us
-  // with one, 101 with eight)
+  // with eight; nine prompts of 2500 to 9000, written and read: 91 us with
+  // one, 74 with four, 79 with eight)
   int tshift = 0;
   while ((2 << tshift) <= IO_TOKENS && (a.b.total >> (tshift + 1)) >= 148 * 16) ++tshift;
   const int per = IO_THREADS / 32 << tshift;
