@@ -73,7 +73,7 @@ struct PtShape {
   static constexpr int KST = HD == 256 && SPLIT ? 1 : 2;   // buffers of unpacked keys, and of values
   // Copied stages: the keys' and the values', rings of their own, for a wait by
   // parity tells two neighbouring phases apart and no more.
-  static constexpr int RK = 2, RV = HD == 256 ? 1 : 2, RST = RK + RV;
+  static constexpr int RK = 1, RV = 1, RST = RK + RV;
   static constexpr int QB = PT_ROWS * HD * 2;              // bytes of one term of Q
   static constexpr int KB = PT_BN * HD * 2;                // of one term of a tile's keys (values)
   static constexpr int RAW = PT_BN * (HD / 2 + 4 * (HD / GROUP));  // bytes of a tile's keys (values) as they are held
@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
 #pragma unroll 1
       for (int i = 0; i < nt; ++i) {
         const int jj = j + i, st = jj % KST, rs = kv ? Sh::RK + jj % Sh::RV : jj % Sh::RK;
-        if (!wait(empty + st, ((jj / KST) & 1) ^ 1) || !wait(&r_full[rs], (jj / (kv ? Sh::RV : Sh::RK)) & 1)) break;
+        if (!wait(&r_full[rs], (jj / (kv ? Sh::RV : Sh::RK)) & 1)) break;
         const uint8_t* raw = sm + Sh::R_OFF + rs * Sh::RAW;
         uint8_t* d = dst + st * ((kv ? T : KT) * Sh::KB);
         uint32_t w[2][NW], pr[2][NG];
@@ -829,7 +829,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
             for (int k = 0; k < NG; ++k)
               if (!(fabsf(kv4_param(pr[q][k]).x) < INFINITY) || !(fabsf(kv4_param(pr[q][k]).y) < INFINITY)) pr[q][k] = 0u;
         }
-        mbar_arrive(&r_empty[rs]);
+        mbar_arrive(&r_empty[rs]);  // the next copy is under way while this tile waits for its buffer
+        if (!wait(empty + st, ((jj / KST) & 1) ^ 1)) break;
         if (kv) {
 #pragma unroll
           for (int q = 0; q < 2; ++q)
