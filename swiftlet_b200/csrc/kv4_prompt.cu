@@ -23,19 +23,21 @@
 //
 // Warps: 0-7 softmax and output (two threads a row, half of the tile's slots
 // each), 8-15 unpacking of keys, 16-23 of values, 24 MMA issue and TMEM, 25 and
-// 26 bulk copies of the cache's bytes (a tile's keys, a tile's values) into a
-// ring of stages each. Q stands in TMEM (its low terms in shared memory), S and
+// 26 bulk copies of the cache's bytes (a tile's keys, a tile's values). Q stands in TMEM (its low terms in shared memory), S and
 // P share columns and are double-buffered, so Q K^T of the next tile runs
 // during the softmax of this one; the running maximum moves only when it has
 // grown by 2^8, so O in TMEM is rarely touched. Bound: the chain of copy,
 // unpack, product, softmax, product. A tile of 64 slots at 256 channels is 1536
-// cycles of MMA for bf16 (3072 for f32), and takes some 3000 (6000): the unpack
-// (14 instructions per 8 values) and the softmax share the issue slots, and
-// shared memory holds two buffers of unpacked tiles at most (one for f32).
+// cycles of MMA for bf16 (3072 for f32), and takes some 3000 (6000), with every
+// role busy for two thirds of it or more: leaving out the exponentials, the
+// maxima, the keys' low terms or a third of the products changed it by 3 % at
+// most, the values' unpacking by 5, a second warp for the issue of products by
+// nothing. Shared memory holds two buffers of unpacked tiles at most (one for
+// f32), TMEM no second item.
 // 2048 tokens on a context of 10000 (2 kv heads of 256 channels, 16 query heads,
-// bf16): 490 us, 0.61 PFLOP/s; 8192 tokens from the first (4 kv heads of 128, 16
-// query heads, f16, four products): 690 us, 0.40; 8 chunks of 33 to 200 tokens
-// on 900 to 4100 (2 of 256, f32, six products): 245 us, 0.16.
+// bf16): 440 to 490 us, 0.61 to 0.68 PFLOP/s; 8192 tokens from the first (4 kv
+// heads of 128, 16 query heads, f16, four products): 690 us, 0.40; 8 chunks of 33
+// to 200 tokens on 900 to 4100 (2 of 256, f32, six products): 218 us, 0.19.
 //
 // The work is shared out like that of kv4_attn.cu: equal contiguous shares of
 // all tiles of all items over 148 CTAs, parts of an item that several CTAs
@@ -71,8 +73,11 @@ struct PtShape {
   static constexpr int T = SPLIT ? 2 : 1;                  // f16 terms of queries, weights and values
   static constexpr int KT = 2;                             // and of keys
   static constexpr int KST = HD == 256 && SPLIT ? 1 : 2;   // buffers of unpacked keys, and of values
-  // Copied stages: the keys' and the values', rings of their own, for a wait by
-  // parity tells two neighbouring phases apart and no more.
+  // Copied stages, of the keys and of the values: a stage is read into registers
+  // before the wait for the unpacked buffer, so that the next copy is under way
+  // meanwhile, and more of them gain nothing (two and one: a turn of 2048 tokens
+  // 458 us, one each 440). Each kind has its own, for a wait by parity tells two
+  // neighbouring phases apart and no more.
   static constexpr int RK = 1, RV = 1, RST = RK + RV;
   static constexpr int QB = PT_ROWS * HD * 2;              // bytes of one term of Q
   static constexpr int KB = PT_BN * HD * 2;                // of one term of a tile's keys (values)
