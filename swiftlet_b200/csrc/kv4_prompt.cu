@@ -9,8 +9,7 @@
 // Keys and values are unpacked to f16 on their way into shared memory, scaled
 // by a power of two so that the largest value of the sequence and head is
 // just below 2^14 (k_kv4_range reads the params for it). Keys are two f16
-// terms: lse and the weights are f32 whatever the inputs' type, and with keys
-// of 11 bits scores were off by 1e-4. 16-bit inputs: queries and values are one
+// terms: lse and the weights are f32 whatever the inputs' type. 16-bit inputs: queries and values are one
 // term (values rounded to 11 bits like the inputs themselves), so two products
 // make S and one O; for f16 the weights are two terms and O takes two (with one,
 // outputs were off by 1.6 times their own rounding, with two 1.2 times). f32
@@ -391,8 +390,12 @@ __device__ __forceinline__ void pt_unpack(uint32_t w, __half2 sb, uint4& hi, uin
 }
 // Keys for 16-bit inputs, in f16 arithmetic alone: with e = c - 7.5, s e =
 // fl(s e) + (its residual, which an FMA gives exactly), and the group's middle
-// b + 7.5 s joins the residual (rounded by 2^-12 of the middle, which is a
-// fraction of a step where a group is spread about zero).
+// b + 7.5 s joins the residual, rounded by 2^-12 of the middle: lse is off by
+// 6e-5 where keys are spread about zero and by 2e-4 where they are two spreads
+// away from it, a tenth of what rounding to 16 bits does to the outputs. Where
+// weights are accumulated the keys are taken to 22 bits (pt_unpack<true>: lse
+// and weights off by 1e-6), which for a turn of 2048 tokens on 10000 (256
+// channels, bf16) is 533 us instead of 442.
 __device__ __forceinline__ void pt_unpack_keys(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
   uint32_t* H = &hi.x;
   uint32_t* L = &lo.x;
@@ -408,13 +411,9 @@ __device__ __forceinline__ void pt_unpack_keys(uint32_t w, __half2 sb, uint4& hi
     L[i] = pt_h2(__hadd2(__hfma2(e, s, __hneg2(h)), mid));
   }
 }
-template <bool SPLIT>
-__device__ __forceinline__ void pt_unpack_k(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
-  if (SPLIT) pt_unpack<true>(w, sb, hi, lo);
-  else pt_unpack_keys(w, sb, hi, lo);
-}
 
-template <int HD, int GROUP, bool SPLIT>
+// EXACT: keys to 22 bits (a switch at run time costs the other form its speed).
+template <int HD, int GROUP, bool SPLIT, bool EXACT>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs a) {
   using Sh = PtShape<HD, GROUP, SPLIT>;
   constexpr int BN = PT_BN, T = Sh::T, KT = Sh::KT, KST = Sh::KST, RST = Sh::RST, NG = HD / GROUP, NW = HD / 64;
@@ -852,7 +851,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
 #pragma unroll
             for (int k = 0; k < NW; ++k) {
               uint4 hi, lo;
-              pt_unpack_k<SPLIT>(w[q][k], __hmul2(pt_u2(pr[q][k * 64 / GROUP]), sc), hi, lo);
+              const __half2 sb = __hmul2(pt_u2(pr[q][k * 64 / GROUP]), sc);
+              if constexpr (EXACT) pt_unpack<true>(w[q][k], sb, hi, lo);
+              else pt_unpack_keys(w[q][k], sb, hi, lo);
               *reinterpret_cast<uint4*>(d + q * (32 * 128) + k * (BN * 128)) = hi;
               *reinterpret_cast<uint4*>(d + Sh::KB + q * (32 * 128) + k * (BN * 128)) = lo;
             }
@@ -1191,7 +1192,7 @@ __global__ void __launch_bounds__(WQ_THREADS, SPLIT ? 1 : 2) k_kv4_prompt_weight
       uint32_t hi[16], lo[16];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        pt_unpack_k<SPLIT>(w[u][k], __hmul2(pt_u2(pr[k * 64 / GROUP]), sc), *reinterpret_cast<uint4*>(hi + 4 * u), *reinterpret_cast<uint4*>(lo + 4 * u));
+        pt_unpack<true>(w[u][k], __hmul2(pt_u2(pr[k * 64 / GROUP]), sc), *reinterpret_cast<uint4*>(hi + 4 * u), *reinterpret_cast<uint4*>(lo + 4 * u));
       pt_st16(lanes + Sh::K_COL + k * 32 + hf * 16, hi);
       pt_st16(lanes + Sh::K_COL + HD / 2 + k * 32 + hf * 16, lo);
     }
@@ -1297,7 +1298,8 @@ template <int HD, int GROUP, bool SPLIT>
 void run(const Kv4AttnArgs& a, cudaStream_t st) {
   using Sh = PtShape<HD, GROUP, SPLIT>;
   launch(k_kv4_range, dim3(a.b.nseq * a.g.kvh, RG_SPLIT), dim3(256), 0, st, true, a);
-  launch(k_kv4_prompt<HD, GROUP, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS), Sh::TOTAL, st, true, a);
+  launch(SPLIT || a.weights ? k_kv4_prompt<HD, GROUP, SPLIT, true> : k_kv4_prompt<HD, GROUP, SPLIT, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS),
+         Sh::TOTAL, st, true, a);
   if (a.b.max_len > PT_BN)  // or every item is one tile, and written at once
     launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(HD), 0, st, true, a);
   if (a.weights && a.b.max_len > 0) {

@@ -297,6 +297,33 @@ def test_weights_accumulate(kvh, rep, hd, new, dtype):
     assert torch.equal(w1, w2)
 
 
+@pytest.mark.parametrize("dtype,hd", [(1, 256), (2, 128), (0, 64)])
+def test_weights_of_prompts_keep_their_bits(dtype, hd):
+    """The weights of a prompt are f32 sums: with keys far from zero they are held to the f32 bound (16 roundings of sum |q k| scale, and
+    2^-22 of it for two f16 terms of a key) whatever the inputs' type."""
+    torch, dts = _torch()
+    rng = np.random.default_rng(21)
+    n, new, rep = 600, 100, 8
+    c = Cache(1, n, 2, hd)
+    x = torch.from_numpy((rng.standard_normal((2, n, 2, hd)) + 2).astype(np.float32)).to(dts[dtype])
+    d = x.cuda()
+    swl.kv4_append_device(c.desc(), c.batch([n], [n]), d[0].data_ptr(), d[1].data_ptr(), dtype=dtype)
+    held = quantise(x.float().numpy(), 64).astype(np.float64)
+    w = torch.zeros(1, 2, n, device="cuda")
+    _, lse, q = attend(c, [n], [new], rep, rng, dtype=dtype, weights=w)
+    want, ds, scale = np.zeros((2, n)), 0.0, 1 / math.sqrt(hd)
+    for t in range(new):
+        for h in range(2 * rep):
+            k = held[0, :n - new + t + 1, h // rep]
+            s = scale * (k @ q[t, h, 0])
+            z = s.max() + np.log(np.exp(s - s.max()).sum())
+            own = (20 * U * scale * (np.abs(k) @ np.abs(q[t, h, 0]))).max()
+            assert abs(lse[t, h] - z) <= own + 8 * U * (1 + abs(z))
+            ds = max(ds, own)
+            want[h // rep, :k.shape[0]] += np.exp(s - z)
+    assert (np.abs(w[0].cpu().numpy() - want) <= (2 * ds + 64 * U) * want + 1e-12).all()
+
+
 def test_values_of_very_different_size():
     """Values from 1e-5 to 1e4 in neighbouring groups and slots, and large scores: nothing under- or overflows on the way."""
     torch, _ = _torch()
