@@ -27,7 +27,7 @@
 // during the softmax of this one; the running maximum moves only when it has
 // grown by 2^8, so O in TMEM is rarely touched. Bound: the chain of copy,
 // unpack, product, softmax, product. A tile of 64 slots at 256 channels is 1536
-// cycles of MMA for bf16 (3072 for f32), and takes some 3000 (6000), with every
+// cycles of MMA for bf16 (twice that for f32), and takes some 3000 (6000), with every
 // role busy for two thirds of it or more: leaving out the exponentials, the
 // maxima, the keys' low terms or a third of the products changed it by 3 % at
 // most, the values' unpacking by 5, a second warp for the issue of products by
