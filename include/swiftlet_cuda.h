@@ -384,13 +384,11 @@ int swl_kv4_read_device(const swl_kv4_cache* cache, const swl_kv4_batch* batch, 
  * (-infinity for an empty row). weights (may be NULL):
  * [nseq][kv_heads][weights_stride]; every slot's softmax weight, summed over
  * the new tokens and the kv head's query heads, is added to it. Sums are f32
- * in a fixed order: the same call gives the same bits (with or without weights
-lse may differ in its last bits: for bf16 and f16 inputs and more than 64 query
-rows a kv head the scores behind it are exact to 2^-12 of a key group's middle
-without weights, to 2^-22 of the keys with them). q, out and gate have
- * one dtype; out must not overlap q or gate. work: device memory of
- * swl_kv4_attention_workspace bytes (16-byte aligned), used by one call at a
- * time; its contents need no initialisation. */
+ * in a fixed order: the same call gives the same bits, and out and lse are the
+ * same with weights as without. q, out and gate have one dtype; out must not
+ * overlap q or gate. work: device memory of swl_kv4_attention_workspace bytes
+ * (16-byte aligned), used by one call at a time; its contents need no
+ * initialisation. */
 typedef struct swl_kv4_attention {
   int32_t dtype, heads;
   float scale;

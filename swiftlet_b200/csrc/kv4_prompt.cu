@@ -9,10 +9,12 @@
 // Keys and values are unpacked to f16 on their way into shared memory, scaled
 // by a power of two so that the largest value of the sequence and head is
 // just below 2^14 (k_kv4_range reads the params for it). Keys are two f16
-// terms: lse and the weights are f32 whatever the inputs' type. 16-bit inputs: queries and values are one
-// term (values rounded to 11 bits like the inputs themselves), so two products
-// make S and one O; for f16 the weights are two terms and O takes two (with one,
-// outputs were off by 1.6 times their own rounding, with two 1.2 times). f32
+// terms, for scores, lse and the weights are f32 whatever the inputs' type.
+// 16-bit inputs: keys are taken about their group's middle and exact, the
+// middles are a product of 16 columns; queries and values are one term (values
+// rounded to 11 bits like the inputs themselves), so two products and the
+// small one make S and one O; for f16 the weights are two terms and O takes two
+// (with one, outputs were off by 1.6 times their own rounding, with two 1.2 times). f32
 // inputs: all operands are two terms (22 bits) and three products each make S
 // and O (hi lo, lo hi, hi hi).
 // The tensor cores' f32 accumulators truncate: every product added takes up to
@@ -34,8 +36,8 @@
 // nothing. Shared memory holds two buffers of unpacked tiles at most (one for
 // f32), TMEM no second item.
 // 2048 tokens on a context of 10000 (2 kv heads of 256 channels, 16 query heads,
-// bf16): 440 to 490 us, 0.61 to 0.68 PFLOP/s; 8192 tokens from the first (4 kv
-// heads of 128, 16 query heads, f16, four products): 690 us, 0.40; 8 chunks of 33
+// bf16): 455 us, 0.66 PFLOP/s; 8192 tokens from the first (4 kv
+// heads of 128, 16 query heads, f16, four products): 740 us, 0.37; 8 chunks of 33
 // to 200 tokens on 900 to 4100 (2 of 256, f32, six products): 218 us, 0.19.
 //
 // The work is shared out like that of kv4_attn.cu: equal contiguous shares of
@@ -83,9 +85,12 @@ struct PtShape {
   static constexpr int RAW = PT_BN * (HD / 2 + 4 * (HD / GROUP));  // bytes of a tile's keys (values) as they are held
   // low terms of Q, keys (first the high terms of Q, on their way to TMEM), values, copied stages
   static constexpr int SCR = 8 * 32 * 33 * 4;              // the output's scratch, over the key buffers
+  // 16-bit inputs: 16 more columns of Q and of every tile of keys, for the groups' middles (pt_middles)
+  static constexpr int XQB = SPLIT ? 0 : PT_ROWS * 32, XKB = SPLIT ? 0 : PT_BN * 32;
   static constexpr int KS = KST * KT * KB > SCR ? KST * KT * KB : (SCR + 1023) / 1024 * 1024;
   static constexpr int Q_OFF = 0, K_OFF = SPLIT ? QB : 0, V_OFF = K_OFF + KS, R_OFF = V_OFF + KST * T * KB;
-  static constexpr int M_OFF = R_OFF + RST * RAW;          // the rows' factors and limits, exchange of the halves
+  static constexpr int XQ_OFF = R_OFF + RST * RAW, XK_OFF = XQ_OFF + XQB;
+  static constexpr int M_OFF = XK_OFF + KST * XKB;         // the rows' factors and limits, exchange of the halves
   static constexpr int BAR_OFF = M_OFF + PT_ROWS * 16;
   static constexpr int NBAR = 4 * KST + 2 * RST + 7;       // k, v full / empty, raw full / empty, s full, p full, o done, drain
   static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 16 + RST * 4 + 1024;  // 1024: base alignment
@@ -107,6 +112,13 @@ __device__ __forceinline__ uint64_t pt_desc_n(uint32_t saddr, uint32_t lbo) {
   return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(lbo >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(2) << 61);
 }
+// K-major operand of 16 columns, no swizzle: blocks of eight rows x 16 bytes,
+// the two of a row's 32 bytes 128 bytes apart (LBO), the next eight rows 256 (SBO).
+__device__ __forceinline__ uint64_t pt_desc_x(uint32_t saddr) {
+  return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(128 >> 4) << 16) | (uint64_t(256 >> 4) << 32) | (uint64_t(1) << 46);
+}
+// Byte of column c of row r in such an operand.
+__device__ __forceinline__ constexpr int pt_x(int r, int c) { return (r >> 3) * 256 + (c >> 3) * 128 + (r & 7) * 16 + (c & 7) * 2; }
 __device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -388,18 +400,16 @@ __device__ __forceinline__ void pt_unpack(uint32_t w, __half2 sb, uint4& hi, uin
     }
   }
 }
-// Keys for 16-bit inputs, in f16 arithmetic alone: with e = c - 7.5, s e =
-// fl(s e) + (its residual, which an FMA gives exactly), and the group's middle
-// b + 7.5 s joins the residual, rounded by 2^-12 of the middle: lse is off by
-// 6e-5 where keys are spread about zero and by 2e-4 where they are two spreads
-// away from it, a tenth of what rounding to 16 bits does to the outputs. Where
-// weights are accumulated the keys are taken to 22 bits (pt_unpack<true>: lse
-// and weights off by 1e-6), which for a turn of 2048 tokens on 10000 (256
-// channels, bf16) is 533 us instead of 442.
+// Keys for 16-bit inputs, in f16 arithmetic alone: with e = c - 7.5, a key is
+// s e + (b + 7.5 s). The first part is fl(s e) and its residual, which an FMA
+// gives exactly (15 bits in all), the group's middle a product of its own
+// (pt_middles): scores are f32 results whatever the inputs' type. (As f32
+// inputs have them, two rounded terms of the whole value, they cost 22 % more:
+// a turn of 2048 tokens on 10000 in bf16 533 us instead of 440; this way 455.)
 __device__ __forceinline__ void pt_unpack_keys(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
   uint32_t* H = &hi.x;
   uint32_t* L = &lo.x;
-  const __half2 s = __low2half2(sb), mid = __hfma2(s, pt_u2(0x47804780u), __high2half2(sb));  // 7.5
+  const __half2 s = __low2half2(sb);
   const __half2 m0 = pt_u2(0xe00fe00fu);                          // 512 + c less 519.5
   const __half2 r = pt_u2(0x2c002c00u), m1 = pt_u2(0xd0f0d0f0u);  // (512 + 16 c) / 16 less 39.5
 #pragma unroll
@@ -408,12 +418,21 @@ __device__ __forceinline__ void pt_unpack_keys(uint32_t w, __half2 sb, uint4& hi
     const __half2 e = i & 1 ? __hfma2(pt_u2((x & 0x01e001e0u) | 0x60006000u), r, m1) : __hadd2(pt_u2((x & 0x001e001eu) | 0x60006000u), m0);
     const __half2 h = __hmul2(e, s);
     H[i] = pt_h2(h);
-    L[i] = pt_h2(__hadd2(__hfma2(e, s, __hneg2(h)), mid));
+    L[i] = pt_h2(__hfma2(e, s, __hneg2(h)));
   }
 }
+// The groups' part of a score, sum_g (sum_{i in g} q_i) (b + 7.5 s)_g, as one
+// more product of 16 columns: both factors two f16 terms (22 bits), columns g
+// hi hi, 4 + g hi lo and 8 + g lo hi of group g, the others zero.
+template <bool KEYS>
+__device__ __forceinline__ void pt_middles(uint8_t* x, int row, int g, float v) {
+  const __half hi = __float2half_rn(v), lo = __float2half_rn(v - __half2float(hi));
+  *reinterpret_cast<__half*>(x + pt_x(row, g)) = hi;
+  *reinterpret_cast<__half*>(x + pt_x(row, 4 + g)) = KEYS ? lo : hi;
+  *reinterpret_cast<__half*>(x + pt_x(row, 8 + g)) = KEYS ? hi : lo;
+}
 
-// EXACT: keys to 22 bits (a switch at run time costs the other form its speed).
-template <int HD, int GROUP, bool SPLIT, bool EXACT>
+template <int HD, int GROUP, bool SPLIT>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs a) {
   using Sh = PtShape<HD, GROUP, SPLIT>;
   constexpr int BN = PT_BN, T = Sh::T, KT = Sh::KT, KST = Sh::KST, RST = Sh::RST, NG = HD / GROUP, NW = HD / 64;
@@ -449,6 +468,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
     mbar_init(drain, 1);
     *abort_flag = 0;
     mbar_init_fence();
+  }
+  if constexpr (!SPLIT) {  // the columns that stay zero
+    for (int i = tid; i < (Sh::XQB + KST * Sh::XKB) / 16; i += PT_THREADS)
+      reinterpret_cast<uint4*>(sm + Sh::XQ_OFF)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async();
   }
   if (warp == PT_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
@@ -772,9 +796,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
 #pragma unroll
           for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[k][e]));
           am = warp_max(am);
-          int ex = am > 0.f && am < INFINITY ? 12 - (int(__float_as_uint(am) >> 23) - 127) : 0;
+          // the largest to [2^12, 2^13), or [2^5, 2^6), so that the sum of a group stays below 2^13
+          int ex = am > 0.f && am < INFINITY ? (SPLIT ? 12 : 5) - (int(__float_as_uint(am) >> 23) - 127) : 0;
           ex = max(-60, min(60, ex));
           const float up = pt_pow2(ex) * sgn;
+          float sum = 0.f;
           if (act) {
             uint4 hi, lo;
             uint32_t *H = &hi.x, *L = &lo.x;
@@ -783,6 +809,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
               const float v0 = x[k][i] * up, v4 = x[k][i + 4] * up;
               const __half2 hh = __floats2half2_rn(v0, v4);
               H[i] = pt_h2(hh);
+              if (!SPLIT) {
+                const float2 ff = __half22float2(hh);
+                sum += ff.x + ff.y;
+              }
               if (SPLIT) {
                 const float2 ff = __half22float2(hh);
                 L[i] = pt_h2(__floats2half2_rn(v0 - ff.x, v4 - ff.y));
@@ -791,6 +821,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
             const int off = (lane >> 3) * (PT_ROWS * 128) + qr * 128 + (((lane & 7) ^ (qr & 7)) << 4);
             *reinterpret_cast<uint4*>(sm + Sh::K_OFF + off) = hi;
             if (SPLIT) *reinterpret_cast<uint4*>(sm + Sh::Q_OFF + off) = lo;
+          }
+          if constexpr (!SPLIT) {
+#pragma unroll
+            for (int o = 1; o < GROUP / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (act && lane % (GROUP / 8) == 0) pt_middles<false>(sm + Sh::XQ_OFF, qr, lane / (GROUP / 8), sum);
           }
           if (lane == 0) {
             row_mul[qr] = sgn == 0.f ? 1.f : fabsf(a.scale) * P_LOG2E * pt_pow2(-ex) * pt_pow2(-kx);
@@ -812,6 +847,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         uo[q] = base + in * (HD / 2) + ((r ^ kv4_swz(HD, t)) * (HD / 16));
         po[q] = base + g.seg * (HD / 2) + in * NG * 4;
       }
+      // 16-bit inputs: the middle of group r % NG of slot t or t + 32 is this thread's
+      const bool mids = !SPLIT && !kv && r < 2 * NG;
+      const int xo = (r < NG ? po[0] : po[1]) + r % NG * 4, xr = t + (r < NG ? 0 : 32);
 #pragma unroll 1
       for (int i = 0; i < nt; ++i) {
         const int jj = j + i, st = jj % KST, rs = kv ? Sh::RK + jj % Sh::RV : jj % Sh::RK;
@@ -833,6 +871,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
             for (int k = 0; k < NG; ++k)
               if (!(fabsf(kv4_param(pr[q][k]).x) < INFINITY) || !(fabsf(kv4_param(pr[q][k]).y) < INFINITY)) pr[q][k] = 0u;
         }
+        float mid = 0.f;
+        if (mids) {
+          const float2 sb = __half22float2(__hmul2(pt_u2(*reinterpret_cast<const uint32_t*>(raw + xo)), sc));
+          mid = fmaf(7.5f, sb.x, sb.y);
+        }
         mbar_arrive(&r_empty[rs]);  // the next copy is under way while this tile waits for its buffer
         if (!wait(empty + st, ((jj / KST) & 1) ^ 1)) break;
         if (kv) {
@@ -852,11 +895,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
             for (int k = 0; k < NW; ++k) {
               uint4 hi, lo;
               const __half2 sb = __hmul2(pt_u2(pr[q][k * 64 / GROUP]), sc);
-              if constexpr (EXACT) pt_unpack<true>(w[q][k], sb, hi, lo);
+              if constexpr (SPLIT) pt_unpack<true>(w[q][k], sb, hi, lo);
               else pt_unpack_keys(w[q][k], sb, hi, lo);
               *reinterpret_cast<uint4*>(d + q * (32 * 128) + k * (BN * 128)) = hi;
               *reinterpret_cast<uint4*>(d + Sh::KB + q * (32 * 128) + k * (BN * 128)) = lo;
             }
+          if (mids) pt_middles<true>(sm + Sh::XK_OFF + st * Sh::XKB, xr, r % NG, mid);
         }
         fence_proxy_async();
         mbar_arrive(full + st);
@@ -887,6 +931,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 pt_mma_ts(d, tm + Sh::Q_COL + w * 32 + k * 8, kd + ((Sh::KB + w * (BN * 128) + k * 32) >> 4), ids, w + k > 0);
+            if constexpr (!SPLIT)
+              pt_mma_ss(d, pt_desc_x(smem_u32(sm + Sh::XQ_OFF)), pt_desc_x(smem_u32(sm + Sh::XK_OFF + st * Sh::XKB)), ids, true);
             if (SPLIT) {
               const uint64_t qd = tg_desc(smem_u32(sm + Sh::Q_OFF));
 #pragma unroll
@@ -1298,8 +1344,7 @@ template <int HD, int GROUP, bool SPLIT>
 void run(const Kv4AttnArgs& a, cudaStream_t st) {
   using Sh = PtShape<HD, GROUP, SPLIT>;
   launch(k_kv4_range, dim3(a.b.nseq * a.g.kvh, RG_SPLIT), dim3(256), 0, st, true, a);
-  launch(SPLIT || a.weights ? k_kv4_prompt<HD, GROUP, SPLIT, true> : k_kv4_prompt<HD, GROUP, SPLIT, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS),
-         Sh::TOTAL, st, true, a);
+  launch(k_kv4_prompt<HD, GROUP, SPLIT>, dim3(PT_GRID), dim3(PT_THREADS), Sh::TOTAL, st, true, a);
   if (a.b.max_len > PT_BN)  // or every item is one tile, and written at once
     launch(k_kv4_prompt_join<HD>, dim3(PT_GRID, PT_ROWS / 8), dim3(HD), 0, st, true, a);
   if (a.weights && a.b.max_len > 0) {

@@ -1,0 +1,138 @@
+"""Errors of attention over the 4-bit KV cache against 64 bits, relative to the terms that are summed (the bounds of
+test_gpu_kv4.py go by the largest value of a head).
+
+With p the softmax weights, v the values and e s a value's distance from its group's middle:
+  a score is off by ds <= 16 U sum |q k| scale (f32 sums of up to 256 products, whatever the inputs' type), which moves an
+      output by 2 ds sum p |v| at most, and by nothing where scores are zero;
+  32 U sum p |v| for the weights, their sum, the products' second terms and the division;
+  a rounding of independent operands to 11 bits is off by 2^-12 of each term at most, uniformly: a sum of them by
+      6 * 2^-12 / sqrt(3) * sqrt(sum of squares) in no one of a million cases. Few rows in 16 bits round p s (terms p s e);
+      prompts in 16 bits round p and v (two such terms of p v), f16 only v;
+  f16 has no step below 2^-24: a weight is off by half of it relative to the factor that f16 weights carry (`floor`);
+  the tensor cores' accumulators truncate: each product of 16 slots takes up to 2^-24 of the sum so far, which is at most the
+      output and six of its spreads, taken twice for the alignment of the products themselves. For 16-bit prompts that is all the
+      tiles of an item (four products each, two for f16), for few rows in 16 bits the units of a warp;
+  half a step of the output type, 2^-8 (bf16), 2^-11 (f16), 2^-24 (f32) of the value."""
+import math
+
+import numpy as np
+import pytest
+
+import swiftlet_b200 as swl
+from test_gpu_kv4 import NAMES, U, Cache, _torch, quantise
+
+pytestmark = pytest.mark.gpu
+HALF = [2.0 ** -24, 2.0 ** -8, 2.0 ** -11]
+SIX = 6 / math.sqrt(3)
+
+
+def put(c, k, v, lens, dtype):
+    """Appends k and v (f32 tensors [rows][kvh][hd] on the CPU) as whole sequences; returns what the cache holds, in 64 bits."""
+    torch, dts = _torch()
+    x = torch.stack([k, v]).to(dts[dtype])
+    d = x.cuda()
+    swl.kv4_append_device(c.desc(), c.batch(lens, lens), d[0].data_ptr(), d[1].data_ptr(), dtype=dtype)
+    torch.cuda.synchronize()
+    return torch.from_numpy(quantise(x.float().numpy(), c.group)).cuda().double()
+
+
+def call(c, lens, new, q, scale, dtype, weights=None, gate=None, want_lse=True):
+    """q [rows][heads][hd] of the type; returns out and lse in 64 bits."""
+    torch, _ = _torch()
+    H, hd = q.shape[1:]
+    b = c.batch(lens, new)
+    nb = swl.kv4_attention_workspace(c.desc(), b, H)
+    work = torch.full((nb,), 255, dtype=torch.uint8, device="cuda")
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    swl.kv4_attention_device(c.desc(), b, H, q.data_ptr(), out.data_ptr(), scale=scale, dtype=dtype,
+                             d_gate=0 if gate is None else gate.data_ptr(), d_lse=lse.data_ptr() if want_lse else 0,
+                             d_weights=0 if weights is None else weights.data_ptr(),
+                             weights_stride=0 if weights is None else weights.stride(1), d_work=work.data_ptr(), work_bytes=nb)
+    torch.cuda.synchronize()
+    assert int(c.status) == 0
+    return out, lse
+
+
+def exact(k, v, q, scale, n, group):
+    """One sequence in 64 bits: k, v [slots][kvh][hd], q [n][heads][hd], the last n slots the rows' own. Per row and head the output,
+    lse, the largest sum |q k| scale, sum p |v|, sqrt(sum (p v)^2) and sqrt(sum (p s e)^2) (s e at most: half the group's range)."""
+    torch, _ = _torch()
+    m, kvh, hd = k.shape
+    H = q.shape[1]
+    rep = H // kvh
+    g = v.view(m, kvh, hd // group, group)
+    half = ((g.amax(-1) - g.amin(-1)) / 2).repeat_interleave(group, -1)
+    res = [[] for _ in range(6)]
+    seen = torch.arange(m, device="cuda")[None] <= (m - n + torch.arange(n, device="cuda"))[:, None]
+    for h in range(H):
+        kh, vh, sh, qh = k[:, h // rep], v[:, h // rep], half[:, h // rep], q[:, h].double()
+        x = (scale * (qh @ kh.T)).masked_fill(~seen, -math.inf)
+        z = x.logsumexp(1)
+        p = (x - z[:, None]).exp()
+        mag = (abs(scale) * (qh.abs() @ kh.abs().T)).masked_fill(~seen, 0).amax(1)
+        for r, t in zip(res, (p @ vh, z, mag, p @ vh.abs(), ((p * p) @ (vh * vh)).sqrt(), ((p * p) @ (sh * sh)).sqrt())):
+            r.append(t)
+    return [torch.stack(r, 1) for r in res]
+
+
+def bound(e, dtype, few, floor, slots, ds=None):
+    """What an output may be off by; e: of `exact`, floor: step of a weight times the sum of what it multiplies."""
+    want, _, mag, pabs, pv, pse = e
+    ds = (16 * U * mag if ds is None else ds)[..., None]
+    tol = HALF[dtype] * want.abs() + (2 * ds + 32 * U) * pabs + floor
+    if dtype:
+        tol = tol + SIX * 2.0 ** -12 * (pse if few else pv * (math.sqrt(2) if dtype == 1 else 1))
+        products = slots / 16 / 12 + 1 if few else slots / 16 * dtype
+        tol = tol + 2 * products * U * (want.abs() + 6 * (pse if few else pv))
+    return tol
+
+
+def lse_bound(e, ds=None):
+    return (16 * U * e[2] if ds is None else ds) + 8 * U * (1 + e[1].abs())
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2], ids=NAMES)
+@pytest.mark.parametrize("lens,new,kvh,rep,hd,group", [([9000], [1], 2, 8, 256, 64), ([6000, 31, 2500], [1, 3, 4], 2, 8, 256, 128),
+                                                       ([5000, 700], [1, 2], 8, 4, 128, 128), ([4100], [150], 2, 8, 256, 64),
+                                                       ([700, 3300], [300, 33], 4, 4, 128, 64), ([2900], [200], 1, 8, 64, 64)])
+def test_outputs_relative_to_what_is_summed(lens, new, kvh, rep, hd, group, dtype):
+    torch, dts = _torch()
+    gen = torch.Generator().manual_seed(sum(lens) + hd)
+    c = Cache(len(lens), max(lens), kvh, hd, group)
+    held = put(c, *(torch.randn(sum(lens), kvh, hd, generator=gen) for _ in range(2)), lens, dtype)
+    q = torch.randn(sum(new), kvh * rep, hd, generator=gen).to(dts[dtype]).cuda()
+    scale = 1 / math.sqrt(hd)
+    out, lse = call(c, lens, new, q, scale, dtype)
+    few = max(new) * rep <= 64
+    j = s = 0
+    for m, n in zip(lens, new):
+        e = exact(held[0, s:s + m], held[1, s:s + m], q[j:j + n], scale, n, group)
+        err = (out[j:j + n].double() - e[0]).abs()
+        tol = bound(e, dtype, few, 0.0, m)
+        assert (err <= tol).all(), float((err / tol).max())
+        assert ((lse[j:j + n].double() - e[1]).abs() <= lse_bound(e)).all()
+        j, s = j + n, s + m
+
+
+# -------------------------------------------------- keys far from zero, lse --
+@pytest.mark.parametrize("dtype", [1, 2], ids=NAMES[1:])
+@pytest.mark.parametrize("hd,group", [(256, 64), (256, 128), (128, 64), (128, 128), (64, 64)])
+def test_prompts_of_16_bits_without_weights_are_those_with_them(hd, group, dtype):
+    """Outputs and lse do not depend on whether weights are accumulated, and lse is an f32 result whatever the inputs' type: keys two
+    spreads from zero, which have large common terms, are no less exact."""
+    torch, dts = _torch()
+    n, slots, kvh, rep = 100, 900, 2, 8
+    gen = torch.Generator().manual_seed(hd + group)
+    c = Cache(1, slots, kvh, hd, group)
+    held = put(c, torch.randn(slots, kvh, hd, generator=gen) + 2, torch.randn(slots, kvh, hd, generator=gen), [slots], dtype)
+    q = torch.randn(n, kvh * rep, hd, generator=gen).to(dts[dtype]).cuda()
+    scale = 1 / math.sqrt(hd)
+    w = torch.zeros(1, kvh, slots, device="cuda")
+    out, lse = call(c, [slots], [n], q, scale, dtype)
+    out_w, lse_w = call(c, [slots], [n], q, scale, dtype, weights=w)
+    out_n, _ = call(c, [slots], [n], q, scale, dtype, want_lse=False)
+    e = exact(held[0], held[1], q, scale, n, group)
+    assert ((lse.double() - e[1]).abs() <= lse_bound(e)).all(), float((lse.double() - e[1]).abs().max())
+    tol = bound(e, dtype, False, 0.0, slots)
+    assert ((out.double() - e[0]).abs() <= tol).all()
+    assert torch.equal(lse, lse_w) and torch.equal(out, out_w) and torch.equal(out, out_n)
