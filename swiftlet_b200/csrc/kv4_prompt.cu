@@ -27,7 +27,7 @@
 // 26 bulk copies of the cache's bytes (a tile's keys, a tile's values). Q stands in TMEM (its low terms in shared memory), S and
 // P share columns and are double-buffered, so Q K^T of the next tile runs
 // during the softmax of this one; the running maximum moves only when it has
-// grown by 2^8, so O in TMEM is rarely touched. Bound: the chain of copy,
+// grown by 2^8 (f32: 2^4), so O in TMEM is rarely touched. Bound: the chain of copy,
 // unpack, product, softmax, product. A tile of 64 slots at 256 channels is 1536
 // cycles of MMA for bf16 (twice that for f32), and takes some 3000 (6000), with every
 // role busy for two thirds of it or more: leaving out the exponentials, the
@@ -66,6 +66,15 @@ constexpr int PT_REGS_SOFT = 96, PT_REGS_UNPACK = 64, PT_REGS_ISSUE = 56;
 // from the first, whose early items are short, took 1487 us with one, 690 with twelve; chunks on long contexts 285 and 248.
 constexpr int PT_HEAD = 12;
 constexpr int PT_FLUSH = 4;                             // tiles that O of f32 inputs stays in TMEM
+// The running maximum moves when it has grown by 2^pt_slack; the weights carry
+// 2^pt_up, so that they stay below 2^15, and sums of them and outputs with them.
+// f16's smallest step, 2^-24, is then 2^-31 of the maximum or less (f32 inputs
+// 2^-35): weights that many slots share behind a dominant one are still there
+// (unscaled, those below 2^-25 were lost to the outputs: 2000 slots 18 nats
+// behind the first, f32, 2 % of the output). A slack of 2^4 costs f32 inputs 4 % (8
+// chunks 219 and 228 us) and 16-bit inputs, which gain nothing from it, 9 to 18 %.
+constexpr int pt_slack(bool split) { return split ? 4 : 8; }
+constexpr int pt_up(bool split) { return 15 - pt_slack(split); }
 constexpr int RG_SPLIT = 16;                            // blocks a (sequence, head) of the range kernel
 constexpr float P_LOG2E = 1.4426950408889634f, P_LN2 = 0.6931471805599453f;
 
@@ -540,6 +549,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
     const int hf = warp >> 2, row = tid & (PT_ROWS - 1), pair = 2 + (warp & 3);
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
     constexpr int HB = BN / 2;
+    constexpr float SLACK = pt_slack(SPLIT), UP = pt_up(SPLIT);
     const bool two_p = a.dt == DT_F16;
     for_items([&](const PtPlace& p, int tb, int nt, int v1, int slot_of_part) {
       int kx, vx;
@@ -599,7 +609,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
         // both halves have read S when the pair has met: P may take its place
         tg_fence_before();
-        const bool any = pt_bar_any(pair, mx > m + 8.f || dead), flush = SPLIT && i > 0 && i % PT_FLUSH == 0;
+        const bool any = pt_bar_any(pair, mx > m + SLACK || dead), flush = SPLIT && i > 0 && i % PT_FLUSH == 0;
         if (flush) {
           pending = !wait(&o_done[b ^ 1], ((jj - 1) >> 1) & 1);
           tg_fence_after();
@@ -610,7 +620,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           xch[hf * PT_ROWS + row] = mx;
           if (pt_bar_any(pair, dead)) break;
           mx = fmaxf(mx, xch[(hf ^ 1) * PT_ROWS + row]);
-          const bool grow = mx > m + 8.f;
+          const bool grow = mx > m + SLACK;
           const float mn = grow ? mx : m;
           const float al = m == -INFINITY ? (grow ? 0.f : 1.f) : pt_ex2(m - mn);
           m = mn;
@@ -634,7 +644,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           if (pt_bar_any(pair, late)) break;  // and xch is free again
         }
         tg_fence_after();
-        const float mm = m == -INFINITY ? 0.f : m;
+        const float mm = m == -INFINITY ? 0.f : m - UP;
         float l4[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t hi[HB / 2], lo[HB / 2];
         const auto weigh = [&](bool two) {
@@ -695,7 +705,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           part[row] = l != l ? INFINITY : m;  // a NaN sum stays NaN when parts are joined
           part[PT_ROWS + row] = l;
         } else if (tok < p.n) {
-          pt_lse(a)[int64_t(p.row0 + tok) * a.heads + hq] = none ? -INFINITY : (m + log2f(l)) * P_LN2;
+          pt_lse(a)[int64_t(p.row0 + tok) * a.heads + hq] = none ? -INFINITY : (m + log2f(l * pt_pow2(-int(UP)))) * P_LN2;
         }
       }
       // through shared memory (the key buffers: nothing reads them any more),
@@ -1031,6 +1041,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
 template <int HD>
 __global__ void __launch_bounds__(HD) k_kv4_prompt_join(const Kv4AttnArgs a) {
   pdl_wait();
+  const int UP = pt_up(a.dt == DT_F32);
   const int x = blockIdx.x, j = threadIdx.x >> 3, r = blockIdx.y * 8 + (threadIdx.x & 7);
   const PtJoin d = pt_joins(a)[x];
   if (d.first < 0) return;
@@ -1072,7 +1083,7 @@ __global__ void __launch_bounds__(HD) k_kv4_prompt_join(const Kv4AttnArgs a) {
     for (int e = 0; e < 8; ++e) v[e] *= kv4_sigmoid(g[e]);
   }
   kv4_st8(a.out.p, a.dt, row * a.out.ts + hq * a.out.hs + j * 8, kv4_vec(a.out, a.dt), v);
-  if (j == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * P_LN2;
+  if (j == 0) pt_lse(a)[row * a.heads + hq] = L == 0.f ? -INFINITY : (M + log2f(L * pt_pow2(-UP))) * P_LN2;
 }
 
 // ------------------------------------------------------- accumulated weight --

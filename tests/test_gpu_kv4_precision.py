@@ -136,3 +136,45 @@ def test_prompts_of_16_bits_without_weights_are_those_with_them(hd, group, dtype
     tol = bound(e, dtype, False, 0.0, slots)
     assert ((out.double() - e[0]).abs() <= tol).all()
     assert torch.equal(lse, lse_w) and torch.equal(out, out_w) and torch.equal(out, out_n)
+
+
+# ------------------------------------------------------------ peaked rows --
+def sink(slots, n, ahead, dtype, hd=128, kvh=2, rep=4, seed=0):
+    """Queries that slot 0's key puts `ahead` nats before the logarithm of all the others' mean, its value zero; the others' values
+    about 0.7: outputs are sums of many small weights."""
+    torch, dts = _torch()
+    gen = torch.Generator().manual_seed(seed)
+    c = Cache(1, slots, kvh, hd)
+    k = torch.randn(slots, kvh, hd, generator=gen) * 0.7
+    k[0] = torch.randn(kvh, hd, generator=gen).sign() * 2
+    v = torch.rand(slots, kvh, hd, generator=gen) + 0.2
+    v[0] = 0
+    held = put(c, k, v, [slots], dtype)
+    scale = 1 / math.sqrt(hd)
+    q = torch.randn(n, kvh * rep, hd, generator=gen).cuda().double()
+    for h in range(kvh * rep):
+        kh = held[0, :, h // rep]
+        for _ in range(3):  # the rest moves a little with q's new part
+            x = scale * (q[:, h] @ kh.T)
+            rest = x[:, 1:].logsumexp(1) - math.log(slots - 1)
+            q[:, h] += ((ahead + rest - x[:, 0]) / (scale * (kh[0] @ kh[0])))[:, None] * kh[0]
+    q = q.to(dts[dtype])
+    return c, held, q, scale
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2], ids=NAMES)
+@pytest.mark.parametrize("slots", [2000, 30000])
+@pytest.mark.parametrize("ahead", [10, 14, 18])
+def test_prompts_with_a_dominant_slot(ahead, slots, dtype):
+    """f16 weights carry 2^11 (f32 inputs) or 2^7 at the row's reference: half of f16's smallest step is 2^-36 or 2^-32 of it. Steps
+    of independent weights, so six spreads of a uniform one."""
+    torch, _ = _torch()
+    n = 40
+    c, held, q, scale = sink(slots, n, ahead, dtype)
+    e = exact(held[0], held[1], q, scale, n, c.group)
+    out, lse = call(c, [slots], [n], q, scale, dtype)
+    assert 0.01 * math.exp(-ahead) * slots < float(e[0].mean()) < slots * math.exp(-ahead)  # the small weights are the output
+    floor = SIX * (2.0 ** -32 if dtype else 2.0 ** -36) * held[1].square().sum(0).sqrt().repeat_interleave(4, 0)
+    tol = bound(e, dtype, False, floor, slots)
+    assert ((out.double() - e[0]).abs() <= tol).all(), float(((out.double() - e[0]).abs() / tol).max())
+    assert ((lse.double() - e[1]).abs() <= lse_bound(e)).all()
