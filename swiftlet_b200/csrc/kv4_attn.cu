@@ -15,19 +15,26 @@
 // and outputs are f32. Columns are scaled by powers of two on their way into
 // f16 (q by its largest element, p by the largest group scale seen), which
 // changes no bit of the result but keeps both terms in range.
-// That is for f32 inputs (10 instructions per 8 codes): the accumulators
-// truncate, so a sum is off by its largest partial sums, and with codes of one
-// sign those are twice the score's (its error then measured 7.6e-6 on scores of
-// 1.5) and 150 times the output's (at 128k equal weights). For 16-bit inputs e
-// = c and b' = b: one LOP3 a pair, 5 instructions per 8 codes.
+// The accumulators truncate, so a sum is off by its largest partial sums, and
+// with codes of one sign those are twice the score's (its error then measured
+// 7.6e-6 on scores of 1.5) and 150 times the output's (at 128k equal weights:
+// outputs 1e-2 off, all to one side). f32 inputs: codes are centred (10
+// instructions per 8 codes) and a unit's outputs added apart. 16-bit inputs: keys
+// go in as plain codes (one LOP3 a pair, 5 instructions per 8), and so do the
+// values of a unit's first 8 slots; its last 8 go in as 15 - c against -p s, at
+// the same cost, which keeps every partial sum small. With h the f16 weights as
+// they go in (signed), sum |h| e = (sum h c') - 7.5 sum h, whose last sum is one
+// more product a group, with -7.5 in every place: the rounding of p s counts
+// against e, not c (f16 outputs 6e-4 -> 3.0e-4 off, where their own rounding is
+// 2.1e-4; centring the values' codes instead cost 64 long contexts 244 us, not 226).
 //
 // Bound: the cache's bytes (2 (D / 2 + 4 D / g) a slot and kv head), next to
 // the instructions of unpacking and weighting (f32: some 1050 a unit of 16
 // slots at 256 channels and 2.1 a cycle and SM, which is what f32 waits for),
 // which is why codes go to the tensor cores unscaled and the scales are applied
 // to the 16 x 8 results. 2 kv heads of 256 channels, 16 query heads: one
-// sequence of 131072 slots in f32 54 to 59 us (1.3 to 1.4 TB/s), 64 of 61 to
-// 8192 slots in f32 81 us (1.9 TB/s), 64 of 20000 to 32768 in bf16 230 us (4.2
+// sequence of 131072 slots in f32 50 us (1.5 TB/s), 64 of 61 to
+// 8192 slots in f32 80 us (1.9 TB/s), 64 of 20000 to 32768 in bf16 226 us (4.3
 // TB/s).
 #include <algorithm>
 
@@ -75,6 +82,11 @@ __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__
 __device__ __forceinline__ void unpack_plain(uint32_t x, uint32_t& n0, uint32_t& n1) {
   n0 = x & 0x000f000fu;
   n1 = x & 0x00f000f0u;
+}
+// Of the complements, 15 - c.
+__device__ __forceinline__ void unpack_rest(uint32_t x, uint32_t& n0, uint32_t& n1) {
+  n0 = ~x & 0x000f000fu;
+  n1 = ~x & 0x00f000f0u;
 }
 __device__ __forceinline__ void unpack_centred(uint32_t x, uint32_t& n0, uint32_t& n1) {
   const __half2 m0 = u2h(0xe00fe00fu);                    // -519.5
@@ -407,13 +419,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
     }
     const int free_to = __reduce_min_sync(0xffffffffu, min(lim[0], lim[1]));  // every column sees slots up to here
     float o[NW * 4][4];
+    float hs[NG][2];       // 16-bit inputs: -7.5 sum of the f16 weights as they go in
     float pb[NG][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     int K = 0;             // p carries a factor 2^K (K = 6 - exponent of the largest value scale)
     unsigned smax = 0u;    // that scale's bits
 #pragma unroll
     for (int i = 0; i < NW * 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) pb[i][0] = pb[i][1] = 0.f;
+    for (int i = 0; i < NG; ++i) pb[i][0] = pb[i][1] = hs[i][0] = hs[i][1] = 0.f;
 
     int s = 0;
     for (int u = u0; u < u1; u += AT_WARPS) {
@@ -500,7 +513,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
           m[q] = mn;
           l[q] *= al;
 #pragma unroll
-          for (int i = 0; i < NG; ++i) pb[i][q] *= al;
+          for (int i = 0; i < NG; ++i) {
+            pb[i][q] *= al;
+            if constexpr (!SPLIT) hs[i][q] *= al;
+          }
 #pragma unroll
           for (int i = 0; i < NW * 4; ++i) {
             o[i][q] *= al;
@@ -521,11 +537,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
         float2 v0 = kv4_param(vp[0][gi]), v1 = kv4_param(vp[1][gi]);
-        if (SPLIT) {  // the middle of the group
-          v0.y = fmaf(7.5f, v0.x, v0.y);
-          v1.y = fmaf(7.5f, v1.x, v1.y);
-        }
-        float ps[4] = {pr[0] * v0.x, pr[1] * v0.x, pr[2] * v1.x, pr[3] * v1.x};
+        v0.y = fmaf(7.5f, v0.x, v0.y);  // the middle of the group
+        v1.y = fmaf(7.5f, v1.x, v1.y);
+        const float s1 = SPLIT ? v1.x : -v1.x;
+        float ps[4] = {pr[0] * v0.x, pr[1] * v0.x, pr[2] * s1, pr[3] * s1};
         if (edge) {
           float pm[4] = {pr[0] * v0.y, pr[1] * v0.y, pr[2] * v1.y, pr[3] * v1.y};
 #pragma unroll
@@ -545,6 +560,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
           bl0 = movm(h2u(__floats2half2_rn(ps[0] - f0.x, ps[1] - f0.y)));
           bl1 = movm(h2u(__floats2half2_rn(ps[2] - f1.x, ps[3] - f1.y)));
         }
+        if constexpr (!SPLIT) {
+          float d[4] = {hs[gi][0], hs[gi][1], 0.f, 0.f};  // rows are alike
+          mma16816(d, 0xc780c780u, 0xc780c780u, 0xc780c780u, 0xc780c780u, bh0, bh1);
+          hs[gi][0] = d[0];
+          hs[gi][1] = d[1];
+        }
 #pragma unroll
         for (int w = 0; w < GROUP / 64; ++w) {
           const int wi = gi * (GROUP / 64) + w;
@@ -561,7 +582,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
                 unpack_centred(st2 ? cd >> 7 : cd << 1, f[2], f[3]);
               } else {
                 unpack_plain(st2 ? ab >> 8 : ab, f[0], f[1]);
-                unpack_plain(st2 ? cd >> 8 : cd, f[2], f[3]);
+                unpack_rest(st2 ? cd >> 8 : cd, f[2], f[3]);
               }
               if (!SPLIT) mma16816(o[wi * 4 + pt * 2 + st2], f[0], f[1], f[2], f[3], bh0, bh1);
             }
@@ -602,6 +623,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
         l[q] += __shfl_xor_sync(0xffffffffu, l[q], d);
 #pragma unroll
         for (int i = 0; i < NG; ++i) pb[i][q] += __shfl_xor_sync(0xffffffffu, pb[i][q], d);
+      }
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+      if constexpr (!SPLIT) {  // these are whole in every lane
+        pb[i][0] += hs[i][0];
+        pb[i][1] += hs[i][1];
       }
     if (r == 0) {
 #pragma unroll

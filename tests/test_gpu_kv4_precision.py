@@ -178,3 +178,31 @@ def test_prompts_with_a_dominant_slot(ahead, slots, dtype):
     tol = bound(e, dtype, False, floor, slots)
     assert ((out.double() - e[0]).abs() <= tol).all(), float(((out.double() - e[0]).abs() / tol).max())
     assert ((lse.double() - e[1]).abs() <= lse_bound(e)).all()
+
+
+# ------------------------------------------------------ 16 bits at length --
+@pytest.mark.parametrize("dtype", [1, 2], ids=NAMES[1:])
+@pytest.mark.parametrize("slots", [8000, 131072])
+def test_single_tokens_of_16_bits_at_length(slots, dtype):
+    """As many items as blocks, so that a block walks whole contexts; scores of nearly zero, so that all weights count alike. The mean
+    error (an accumulator that truncates is off to one side) is held to a hundredth of the outputs' size."""
+    torch, dts = _torch()
+    nseq, kvh, rep, hd = 75, 2, 8, 128
+    gen = torch.Generator().manual_seed(slots)
+    c = Cache(1, slots, kvh, hd)
+    k, v = (torch.randn(slots, kvh, hd, generator=gen) for _ in range(2))
+    held = put(c, k, v, [slots], dtype)
+    c.table = c.table.expand(nseq, -1).contiguous()  # all sequences read the same pages
+    q = (torch.randn(nseq, kvh * rep, hd, generator=gen) * 1e-3).to(dts[dtype]).cuda()
+    out, lse = call(c, [slots] * nseq, [1] * nseq, q, 1 / math.sqrt(hd), dtype)
+    e = [torch.cat([exact(held[0], held[1], q[i:i + 1], 1 / math.sqrt(hd), 1, c.group)[j] for i in range(nseq)]) for j in range(6)]
+    err = out.double() - e[0]
+    tol = bound(e, dtype, True, 0.0, slots)
+    assert (err.abs() <= tol).all(), float((err.abs() / tol).max())
+    assert ((lse.double() - e[1]).abs() <= lse_bound(e)).all()
+    # independent errors: their mean over N outputs is their rms / sqrt(N) or so; here a twentieth of one output's rounding
+    rms = float(e[0].square().mean().sqrt())
+    assert abs(float(err.mean())) <= HALF[dtype] * rms / 20, (float(err.mean()), rms)
+    # outputs as near as their own rounding (uniform within half a step, which is HALF of the value at most) and that of p s
+    own = HALF[dtype] * rms / math.sqrt(3) + 2.0 ** -12 / math.sqrt(3) * float(e[5].square().mean().sqrt())
+    assert float(err.square().mean().sqrt()) <= own, (float(err.square().mean().sqrt()), own)
