@@ -53,6 +53,14 @@ constexpr int AT_TILE = 128;                // slots of a tile, the grain in whi
 constexpr int AT_HEAD = 4;                  // what an item costs beside its tiles, in tiles
 constexpr int AT_COLS = 8;                  // query columns (token, head) of an item: the MMA's N
 constexpr int AT_GRID = 148;                // one CTA per SM
+// The reference point of a column moves when its maximum has outgrown it by
+// 2^AT_SLACK; p carries 2^K with K = AT_UP - the exponent of the largest value
+// scale s, so that p s (s < 2^(exponent + 1)) stays below 2^15, and f16's
+// smallest step, 2^-24, is 2^-34 of the reference's p s: with a slack of 2^8 (and
+// 2^6) f32 outputs of 2000 slots 18 nats behind the first were 5e-5 off, with
+// this one 7e-6. It costs nothing (64 sequences of 61 to 8192 slots 80 us).
+constexpr float AT_SLACK = 4.f;
+constexpr int AT_UP = 10;
 constexpr int WT_WARPS = 8;                 // warps of the weight kernel: one tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -421,7 +429,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
     float o[NW * 4][4];
     float hs[NG][2];       // 16-bit inputs: -7.5 sum of the f16 weights as they go in
     float pb[NG][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int K = 0;             // p carries a factor 2^K (K = 6 - exponent of the largest value scale)
+    int K = 0;             // p carries a factor 2^K (AT_UP)
     unsigned smax = 0u;    // that scale's bits
 #pragma unroll
     for (int i = 0; i < NW * 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -495,20 +503,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_kv4_attn(const Kv4AttnArgs a)
             if ((vp[k][i] & 0x7c00u) != 0x7c00u) sb = max(sb, vp[k][i] & 0xffffu);
         sb = __reduce_max_sync(0xffffffffu, sb);
       }
-      // The reference point moves only when the maximum has outgrown it by
-      // 2^8 or the scales theirs: p then stays below 2^8, p s below 2^15.
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f) || sb > smax) {
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + AT_SLACK || mx[1] > m[1] + AT_SLACK) || sb > smax) {
         int dk = 0;
         if (sb > smax) {
           smax = sb | 0x3ffu;  // the whole binade: K goes by the exponent (s < 2^(e + 1))
           const int e = int(sb >> 10) - 15;
-          dk = 6 - e - K;
-          K = 6 - e;
+          dk = AT_UP - e - K;
+          K = AT_UP - e;
         }
         const float up = ex2(float(dk));
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const float mn = mx[q] > m[q] + 8.f ? mx[q] : m[q];
+          const float mn = mx[q] > m[q] + AT_SLACK ? mx[q] : m[q];
           const float al = m[q] == -INFINITY ? 0.f : ex2(m[q] - mn) * up;
           m[q] = mn;
           l[q] *= al;
