@@ -171,8 +171,11 @@ __device__ __forceinline__ void kv4_st8(uint8_t* p, int dt, int64_t i, bool vec,
     *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-// Output gate: the fast exponential and divide are within a few ulp.
-__device__ __forceinline__ float kv4_sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// Output gate, within a few units for any v above -87 (below, where the fast
+// divide ends, 0 for less than 2^-125). The fast exponential would be off by 1.2
+// |v| units; a correctly rounded divide costs prompts with a gate 4 % (2048
+// tokens on 10000, bf16: 468 us instead of 455).
+__device__ __forceinline__ float kv4_sigmoid(float v) { return __fdividef(1.f, 1.f + expf(-v)); }
 
 // N consecutive words of shared or global memory as one vector load.
 template <int N>

@@ -226,3 +226,21 @@ def test_few_rows_with_a_dominant_slot(ahead, slots, dtype):
     tol = bound(e, dtype, True, floor, slots)
     assert ((out.double() - e[0]).abs() <= tol).all(), float(((out.double() - e[0]).abs() / tol).max())
     assert ((lse.double() - e[1]).abs() <= lse_bound(e)).all()
+
+
+# ------------------------------------------------------------------- gates --
+@pytest.mark.parametrize("new", [1, 40])
+def test_gates_of_any_size(new):
+    """out sigmoid(gate) from -85 (a factor of 1e-37) to 85: the exponential and the quotient are off by 2 units each (CUDA's documented
+    bounds for expf and __fdividef), the sum and the product by a rounding."""
+    torch, _ = _torch()
+    gen = torch.Generator().manual_seed(new)
+    c = Cache(1, 150, 2, 128)
+    put(c, *(torch.randn(150, 2, 128, generator=gen) for _ in range(2)), [150], 0)
+    q = torch.randn(new, 8, 128, generator=gen).cuda()
+    gate = torch.linspace(-85, 85, new * 8 * 128).view(new, 8, 128).cuda()
+    plain, _ = call(c, [150], [new], q, 0.09, 0)
+    gated, _ = call(c, [150], [new], q, 0.09, 0, gate=gate)
+    want = plain.double() * gate.double().sigmoid()
+    # two units are 4 U
+    assert ((gated.double() - want).abs() <= 10 * U * want.abs() + 2.0 ** -149).all()
