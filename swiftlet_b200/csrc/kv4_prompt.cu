@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_kv4_prompt(const Kv4AttnArgs 
           am = warp_max(am);
           // the largest to [2^12, 2^13), or [2^5, 2^6), so that the sum of a group stays below 2^13
           int ex = am > 0.f && am < INFINITY ? (SPLIT ? 12 : 5) - (int(__float_as_uint(am) >> 23) - 127) : 0;
-          ex = max(-60, min(60, ex));
+          ex = max(-100, min(100, ex));
           const float up = pt_pow2(ex) * sgn;
           float sum = 0.f;
           if (act) {
@@ -1145,7 +1145,7 @@ __global__ void __launch_bounds__(256) k_kv4_queries(const Kv4AttnArgs a) {
   for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[e]));
   am = warp_max(am);
   int ex = am > 0.f && am < INFINITY ? 12 - (int(__float_as_uint(am) >> 23) - 127) : 0;
-  ex = max(-60, min(60, ex));
+  ex = max(-100, min(100, ex));
   const float up = pt_pow2(ex);
   if (lane < HD / 8) {
     uint4 hi, lo;

@@ -244,3 +244,24 @@ def test_gates_of_any_size(new):
     want = plain.double() * gate.double().sigmoid()
     # two units are 4 U
     assert ((gated.double() - want).abs() <= 10 * U * want.abs() + 2.0 ** -149).all()
+
+
+# ---------------------------------------------------------- large queries --
+@pytest.mark.parametrize("dtype", [0, 1], ids=["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("gain", [1e30, 1e-30])
+def test_queries_of_any_size(gain, new, dtype):
+    """Queries and a scale that undoes them: f32 and bf16 hold both."""
+    torch, dts = _torch()
+    gen = torch.Generator().manual_seed(new)
+    c = Cache(1, 200, 2, 128)
+    held = put(c, *(torch.randn(200, 2, 128, generator=gen) for _ in range(2)), [200], dtype)
+    q = (torch.randn(new, 8, 128, generator=gen) * gain).to(dts[dtype]).cuda()
+    scale = float(np.float32(0.09 / gain))
+    w = torch.zeros(1, 2, 200, device="cuda")
+    out, lse = call(c, [200], [new], q, scale, dtype, weights=w)
+    e = exact(held[0], held[1], q, scale, new, c.group)
+    assert ((out.double() - e[0]).abs() <= bound(e, dtype, new == 1, 0.0, 200)).all()
+    assert ((lse.double() - e[1]).abs() <= lse_bound(e)).all()
+    # every row's weights sum to one, each off by its score's error and that of lse
+    assert ((w.double().sum(2) / (4 * new) - 1).abs() <= 2 * 16 * U * e[2].max() + 64 * U).all()
