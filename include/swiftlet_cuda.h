@@ -340,11 +340,12 @@ typedef struct swl_kv4_cache {
  * tokens of sequence i (any number, 0 included), which take its last slots:
  * lens[i] counts the slots with the new ones. total bounds the rows, max_new
  * the new tokens of one sequence, max_len the slots of one sequence (a length
- * outside [0, max_len] is held to it). Rows from start[nseq] on (total at
- * most) are not used, and not written. status (device int32, may be NULL; never cleared): bit 0,
- * a bounded wait inside a kernel gave up and the results are incomplete; bit
- * 1, a length outside [0, max_len] or a page outside the pool (such slots
- * are skipped as if masked). */
+ * outside [0, max_len] is held to it); total and max_len are at most 2^31 -
+ * 4096. Rows from start[nseq] on (total at most) are not used, and not
+ * written. status (device int32, may be NULL; never cleared): bit 0, a bounded
+ * wait inside a kernel gave up and the results are incomplete; bit 1, a length
+ * outside [0, max_len] or a page outside the pool (such slots are skipped as if
+ * masked). */
 typedef struct swl_kv4_batch {
   const int32_t* start; /* device [nseq + 1], ascending */
   const int32_t* lens;  /* device [nseq] */

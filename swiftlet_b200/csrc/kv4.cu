@@ -526,6 +526,9 @@ Kv4Batch batch_of(const swl_kv4_batch* b, const Kv4Geo& g, bool tokens) {
   if (!b) throw Error(ERR_INVALID, "kv4: null batch");
   if (b->nseq < 0 || b->nseq > 65535 || b->total < 0 || b->max_new < 0 || b->max_len < 0)
     throw Error(ERR_INVALID, "kv4: nseq (0..65535), total, max_new and max_len must not be negative");
+  // counts of tiles, units and rows are rounded up in 32 bits
+  if (b->total > 0x7fffffff - 4095 || b->max_len > 0x7fffffff - 4095)
+    throw Error(ERR_UNSUPPORTED, "kv4: total and max_len must be at most 2^31 - 4096");
   if (b->nseq > 0 && (!b->lens || (tokens && !b->start))) throw Error(ERR_INVALID, "kv4: null lens or start");
   if (reinterpret_cast<uintptr_t>(b->lens) % 4 || reinterpret_cast<uintptr_t>(b->start) % 4 ||
       reinterpret_cast<uintptr_t>(b->status) % 4)

@@ -114,3 +114,18 @@ def test_page_bytes():
     assert swl.kv4_page_bytes(2, 256, 64, 64) == 2 * 2 * 64 * (128 + 16)
     assert swl.kv4_page_bytes(8, 64, 64, 128) == 8 * 2 * 128 * (32 + 4)
     refused(swl.SWL_ERR_UNSUPPORTED, lambda: swl.kv4_page_bytes(2, 80, 64, 64))
+
+
+def test_bounds_near_the_end_of_32_bits():
+    """Bounds that tile and row counts could not be rounded up from."""
+    c = cache(table_stride=1 << 26)
+    for kw in (dict(max_len=2 ** 31 - 1), dict(max_len=2 ** 31 - 4095), dict(total=2 ** 31 - 1), dict(total=2 ** 31 - 4095)):
+        b = batch(**kw)
+        refused(swl.SWL_ERR_UNSUPPORTED, lambda: swl.kv4_append_device(c, b, P, P))
+        refused(swl.SWL_ERR_UNSUPPORTED, lambda: swl.kv4_read_device(c, b, P, P))
+        refused(swl.SWL_ERR_UNSUPPORTED, lambda: swl.kv4_attention_workspace(c, b, 16))
+        refused(swl.SWL_ERR_UNSUPPORTED, attend(c, b))
+        refused(swl.SWL_ERR_UNSUPPORTED, evict(c, b))
+        refused(swl.SWL_ERR_UNSUPPORTED, lambda: swl.kv4_evict_workspace(c, b, 5))
+    b = batch(max_len=2 ** 31 - 4096, total=2 ** 31 - 4096)
+    assert swl.kv4_attention_workspace(c, b, 16) > 0 and swl.kv4_evict_workspace(c, b, 5) == 2 * 5 * 4
