@@ -265,3 +265,44 @@ def test_queries_of_any_size(gain, new, dtype):
     assert ((lse.double() - e[1]).abs() <= lse_bound(e)).all()
     # every row's weights sum to one, each off by its score's error and that of lse
     assert ((w.double().sum(2) / (4 * new) - 1).abs() <= 2 * 16 * U * e[2].max() + 64 * U).all()
+
+
+# -------------------------------------------- NaN and lost pages, 16 bits --
+@pytest.mark.parametrize("dtype", [1, 2], ids=NAMES[1:])
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_what_16_bit_rows_do_not_see(new, dtype):
+    """A NaN key and a NaN value in the last slot, a NaN and an infinite query in the last row, a page outside the pool: the rows before
+    the last are as exact as without them, the last one is NaN where it has to be."""
+    torch, dts = _torch()
+    slots, kvh, rep, hd = 300, 2, 8, 256
+    gen = torch.Generator().manual_seed(new)
+    c = Cache(1, slots, kvh, hd, page=32)
+    k, v = (torch.randn(slots, kvh, hd, generator=gen) for _ in range(2))
+    k[-1, 0, 3], v[-1, 1, 70] = math.nan, math.inf
+    held = put(c, k, v, [slots], dtype)
+    q = torch.randn(new, kvh * rep, hd, generator=gen).to(dts[dtype]).cuda()
+    q[-1, 9, 0], q[-1, 10, 5] = math.nan, math.inf
+    out, lse = call(c, [slots], [new], q, 1 / 16, dtype)
+    assert out[-1, :8].isnan().all() and lse[-1, :8].isnan().all() and out[-1, 9:11].isnan().all()
+    assert out[-1, 8:, 64:128].isnan().all()
+    for h in (8, 11, 15):
+        assert out[-1, h, :64].isfinite().all() and out[-1, h, 128:].isfinite().all() and lse[-1, h].isfinite()
+    if new > 1:
+        e = exact(held[0, :-1], held[1, :-1], q[:-1], 1 / 16, new - 1, c.group)
+        assert ((out[:-1].double() - e[0]).abs() <= bound(e, dtype, new * rep <= 64, 0.0, slots)).all()
+        assert ((lse[:-1].double() - e[1]).abs() <= lse_bound(e)).all()
+    c.table[0, 2] = c.num  # slots 64 .. 95
+    b = c.batch([slots - 1], [new])
+    q = torch.randn(new, kvh * rep, hd, generator=gen).to(dts[dtype]).cuda()
+    nb = swl.kv4_attention_workspace(c.desc(), b, kvh * rep)
+    work = torch.full((nb,), 255, dtype=torch.uint8, device="cuda")
+    out, lse, w = torch.empty_like(q), torch.empty(new, kvh * rep, device="cuda"), torch.zeros(1, kvh, slots, device="cuda")
+    swl.kv4_attention_device(c.desc(), b, kvh * rep, q.data_ptr(), out.data_ptr(), scale=1 / 16, dtype=dtype, d_lse=lse.data_ptr(),
+                             d_weights=w.data_ptr(), weights_stride=slots, d_work=work.data_ptr(), work_bytes=nb)
+    torch.cuda.synchronize()
+    assert int(c.status) == 2 and (w[0, :, 64:96] == 0).all()
+    rest = torch.cat([held[:, :64], held[:, 96:-1]], 1)
+    e = exact(rest[0], rest[1], q, 1 / 16, new, c.group)
+    assert ((out.double() - e[0]).abs() <= bound(e, dtype, new * rep <= 64, 0.0, slots)).all()
+    assert ((lse.double() - e[1]).abs() <= lse_bound(e)).all()
+    assert ((w.double().sum(2) / (new * rep) - 1).abs() <= 2 * 16 * U * e[2].max() + 64 * U).all()
