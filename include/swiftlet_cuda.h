@@ -377,8 +377,8 @@ int swl_kv4_read_device(const swl_kv4_cache* cache, const swl_kv4_batch* batch, 
                         const swl_kv4_rows* v, void* cuda_stream);
 
 /* Attention of the batch's rows over the cache (their own keys and values are
- * appended already): query head h of `heads` reads kv head
- * h / (heads / kv_heads); token t of n new ones sees slots 0 .. len - n + t;
+ * appended already): query head h of `heads` (at most 64 a kv head) reads kv
+ * head h / (heads / kv_heads); token t of n new ones sees slots 0 .. len - n + t;
  * out = softmax(scale * q k^T) v, times sigmoid(gate) when gate.data is given
  * (QwenCPUModel.swift:345-367). A row that sees no slot gets zeros. lse (may
  * be NULL): [total][heads] the natural logarithm of each row's softmax sum
@@ -386,7 +386,14 @@ int swl_kv4_read_device(const swl_kv4_cache* cache, const swl_kv4_batch* batch, 
  * [nseq][kv_heads][weights_stride]; every slot's softmax weight, summed over
  * the new tokens and the kv head's query heads, is added to it. Sums are f32
  * in a fixed order: the same call gives the same bits, and out and lse are the
- * same with weights as without. q, out and gate have one dtype; out must not
+ * same with weights as without. Scores, lse and weights are f32 results
+ * whatever the dtype; outputs in bf16 are as near as their own rounding, in f16
+ * 1.4 times it (prompts round values, single tokens weights, to 11 bits).
+ * max_new chooses the kernels of the call: up to 64 query rows a kv head
+ * (max_new * heads / kv_heads) those for few rows, above that those for prompts,
+ * in which a single token costs what 128 rows do. A launch that has one chunk
+ * beside many single tokens is faster as two calls, and a graph captured for
+ * single tokens wants max_new 1. q, out and gate have one dtype; out must not
  * overlap q or gate. work: device memory of swl_kv4_attention_workspace bytes
  * (16-byte aligned), used by one call at a time; its contents need no
  * initialisation. */

@@ -766,12 +766,12 @@ __global__ void __launch_bounds__(AJ_THREADS) k_kv4_attn_join(const Kv4AttnArgs 
 
 // ------------------------------------------------------- accumulated weight --
 // weights[t] += sum over the columns that see slot t of exp(score - lse), the
-// scores computed again from the keys alone (half the cache's bytes; writing
-// them out and reading them back would be as much at 8 query heads a kv head
-// and would need space of rows x slots). A CTA owns 128 slots of a kv head and
-// walks all the sequence's columns, so every sum has one order. Bound: latency
-// (a single token, 16 sequences of 3000 to 8200 slots in f32: 63 us with the
-// attention, of which this is some 20).
+// scores computed again from the keys alone: 144 bytes a slot and kv head at 256
+// channels, 72 at 128, and no space of rows x slots. (Scores written out and
+// read back would be 64 bytes for the 8 query heads of a single token.) A CTA
+// owns 128 slots of a kv head and walks all the sequence's columns, so every sum
+// has one order. Bound: latency (a single token, 16 sequences of 3000 to 8200
+// slots in f32: 62 us with the attention, of which this is some 20, 28 alone).
 template <int HD, int GROUP, bool SPLIT>
 __global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs a) {
   constexpr int NG = HD / GROUP, NW = HD / 64;
@@ -849,9 +849,9 @@ __global__ void __launch_bounds__(WT_WARPS * 32) k_kv4_weights(const Kv4AttnArgs
 // Query rows a kv head up to which these kernels are used. A tile of the prompt
 // kernel costs the same for 1 to 128 rows, here every 8 rows take the item's
 // tiles once more. 32 sequences of 2000 slots (2 kv heads of 256 channels,
-// bf16): 16 rows 33 us here and 99 there, 64 rows 92 and 103, 96 rows 131 and
-// 106 (f32: 64 rows 138 and 150, 96 rows 197 and 155). One of 30000 slots: 64
-// rows 42 and 106, 96 rows 55 and 119.
+// bf16): 32 rows 55 us here and 95 there, 64 rows 96 and 97, 96 rows 137 and 99
+// (f32: 64 rows 138 and 139, 96 rows 198 and 143). One of 30000 slots: 64 rows
+// 43 and 76, 96 rows 57 and 76.
 constexpr int64_t AT_FEW = 64;
 bool few_rows(const Kv4Batch& b, int rep) { return int64_t(b.max_new) * rep <= AT_FEW; }
 

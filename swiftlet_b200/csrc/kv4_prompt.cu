@@ -28,17 +28,18 @@
 // P share columns and are double-buffered, so Q K^T of the next tile runs
 // during the softmax of this one; the running maximum moves only when it has
 // grown by 2^8 (f32: 2^4), so O in TMEM is rarely touched. Bound: the chain of copy,
-// unpack, product, softmax, product. A tile of 64 slots at 256 channels is 1536
-// cycles of MMA for bf16 (twice that for f32), and takes some 3000 (6000), with every
-// role busy for two thirds of it or more: leaving out the exponentials, the
+// unpack, product, softmax, product. A tile of 64 slots at 256 channels is some
+// 1560 cycles of MMA for bf16 (3070 for f32), and takes some 3200 (6000), with every
+// role busy for two thirds of it or more (2.7 instructions a cycle and SM, the
+// tensor pipe 47 % of the time): leaving out the exponentials, the
 // maxima, the keys' low terms or a third of the products changed it by 3 % at
 // most, the values' unpacking by 5, a second warp for the issue of products by
 // nothing. Shared memory holds two buffers of unpacked tiles at most (one for
 // f32), TMEM no second item.
 // 2048 tokens on a context of 10000 (2 kv heads of 256 channels, 16 query heads,
-// bf16): 455 us, 0.66 PFLOP/s; 8192 tokens from the first (4 kv
-// heads of 128, 16 query heads, f16, four products): 740 us, 0.37; 8 chunks of 33
-// to 200 tokens on 900 to 4100 (2 of 256, f32, six products): 218 us, 0.19.
+// bf16): 455 to 500 us, 0.60 to 0.66 PFLOP/s; 8192 tokens from the first (4 kv
+// heads of 128, 16 query heads, f16, four products): 695 to 710 us, 0.39; 8 chunks
+// of 33 to 200 tokens on 900 to 4100 (2 of 256, f32, six products): 226 us, 0.18.
 //
 // The work is shared out like that of kv4_attn.cu: equal contiguous shares of
 // all tiles of all items over 148 CTAs, parts of an item that several CTAs
@@ -63,7 +64,7 @@ constexpr int PT_MMA = (PT_SOFT + PT_UNPACK) / 32, PT_COPY = PT_MMA + 1;  // war
 // Registers a thread: 72 at launch, then 256 x 96 + 512 x 64 + 128 x 56 (= 896 x 72).
 constexpr int PT_REGS_SOFT = 96, PT_REGS_UNPACK = 64, PT_REGS_ISSUE = 56;
 // Cost of an item beside its tiles, in tiles (queries, filling the pipeline, output): 8192 tokens
-// from the first, whose early items are short, took 1487 us with one, 690 with twelve; chunks on long contexts 285 and 248.
+// from the first, whose early items are short, took 1565 us with one, 700 with twelve; chunks on long contexts 263 and 227.
 constexpr int PT_HEAD = 12;
 constexpr int PT_FLUSH = 4;                             // tiles that O of f32 inputs stays in TMEM
 // The running maximum moves when it has grown by 2^pt_slack; the weights carry
@@ -85,8 +86,8 @@ struct PtShape {
   static constexpr int KST = HD == 256 && SPLIT ? 1 : 2;   // buffers of unpacked keys, and of values
   // Copied stages, of the keys and of the values: a stage is read into registers
   // before the wait for the unpacked buffer, so that the next copy is under way
-  // meanwhile, and more of them gain nothing (two and one: a turn of 2048 tokens
-  // 458 us, one each 440). Each kind has its own, for a wait by parity tells two
+  // meanwhile, and more of them gain nothing (8192 tokens at 128 channels: two of
+  // keys 728 us, one 694). Each kind has its own, for a wait by parity tells two
   // neighbouring phases apart and no more.
   static constexpr int RK = 1, RV = 1, RST = RK + RV;
   static constexpr int QB = PT_ROWS * HD * 2;              // bytes of one term of Q
@@ -413,8 +414,8 @@ __device__ __forceinline__ void pt_unpack(uint32_t w, __half2 sb, uint4& hi, uin
 // s e + (b + 7.5 s). The first part is fl(s e) and its residual, which an FMA
 // gives exactly (15 bits in all), the group's middle a product of its own
 // (pt_middles): scores are f32 results whatever the inputs' type. (As f32
-// inputs have them, two rounded terms of the whole value, they cost 22 % more:
-// a turn of 2048 tokens on 10000 in bf16 533 us instead of 440; this way 455.)
+// inputs have them, two rounded terms of the whole value, they cost 17 % more:
+// a turn of 2048 tokens on 10000 in bf16 533 us instead of 455.)
 __device__ __forceinline__ void pt_unpack_keys(uint32_t w, __half2 sb, uint4& hi, uint4& lo) {
   uint32_t* H = &hi.x;
   uint32_t* L = &lo.x;

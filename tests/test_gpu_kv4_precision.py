@@ -11,7 +11,7 @@ With p the softmax weights, v the values and e s a value's distance from its gro
   f16 has no step below 2^-24: a weight is off by half of it relative to the factor that f16 weights carry (`floor`);
   the tensor cores' accumulators truncate: each product of 16 slots takes up to 2^-24 of the sum so far, which is at most the
       output and six of its spreads, taken twice for the alignment of the products themselves. For 16-bit prompts that is all the
-      tiles of an item (four products each, two for f16), for few rows in 16 bits the units of a warp;
+      tiles of an item (four products each, eight for f16), for few rows in 16 bits the units of a warp;
   half a step of the output type, 2^-8 (bf16), 2^-11 (f16; below 2^-14 f16's steps are 2^-24), 2^-24 (f32) of the value."""
 import math
 
